@@ -7,6 +7,7 @@ Layers, bottom up:
   flash_gemv                    the reference's ``flash_gemv`` operator API on top of ``ops``
   sparse_silu                   the reference's CATS MLP module interface on top of ``ops``
   synth                         seeded synthetic weights / inputs / thresholds for tests and benches
+  kv8                           paged 8-bit key/value cache: append, attend, fork, reorder, compact
   tp                            intermediate-dimension sharding with one all-reduce per layer
 
 Importing the package does not load CUDA; the first operator call does, and raises if the

@@ -16,13 +16,24 @@ F32, F16, BF16 = 0, 1, 2
 OUT_STORE, OUT_ACC_F32 = 0, 1
 # status codes of include/cats_b200.h
 OK, ERR_DTYPE, ERR_SHAPE, ERR_ALIGN, ERR_NULL = 0, -1, -2, -3, -4
-ERR_WORKSPACE, ERR_CUDA, ERR_MODE, ERR_STATIC_LIMIT = -5, -6, -7, -8
+ERR_WORKSPACE, ERR_CUDA, ERR_MODE, ERR_STATIC_LIMIT, ERR_RANGE = -5, -6, -7, -8, -9
 MAX_BATCH = 16
 
 _c_void_p = ctypes.c_void_p
 _c_int = ctypes.c_int
 _c_size_t = ctypes.c_size_t
 _c_float = ctypes.c_float
+
+_c_longlong = ctypes.c_longlong
+
+
+class Kv8(ctypes.Structure):
+    """``cats_kv8`` of include/cats_b200.h: the device pointers and sizes of a paged 8-bit cache."""
+    _fields_ = [(n, _c_void_p) for n in ("codes", "scales", "table", "lens", "refs", "status")] + [
+        (n, _c_int) for n in ("n_layers", "n_pages", "n_seqs", "max_pages", "n_kv_heads", "page", "head_dim")]
+
+
+_kv8_p = ctypes.POINTER(Kv8)
 
 # name -> (restype, argtypes); mirrors include/cats_b200.h one to one
 SIGNATURES = {
@@ -84,6 +95,20 @@ SIGNATURES = {
                            _c_int, _c_void_p]),
     "cats_rope_cache": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                                  _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p]),
+    "cats_kv8_grow": (_c_int, [_kv8_p, _c_void_p, _c_int, _c_void_p]),
+    "cats_kv8_append": (_c_int, [_kv8_p, _c_int, _c_void_p, _c_longlong, _c_void_p, _c_int, _c_void_p,
+                                 _c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_void_p]),
+    "cats_kv8_attend_bytes": (_c_size_t, [_kv8_p, _c_int, _c_int]),
+    "cats_kv8_attend": (_c_int, [_kv8_p, _c_int, _c_void_p, _c_longlong, _c_void_p, _c_int, _c_int,
+                                 _c_float, _c_void_p, _c_void_p, _c_size_t, _c_int, _c_void_p]),
+    "cats_kv8_reorder_bytes": (_c_size_t, [_kv8_p]),
+    "cats_kv8_reorder": (_c_int, [_kv8_p, _c_void_p, _c_void_p, _c_size_t, _c_void_p]),
+    "cats_kv8_compact_bytes": (_c_size_t, [_kv8_p]),
+    "cats_kv8_compact": (_c_int, [_kv8_p, _c_void_p, _c_void_p, _c_size_t, _c_void_p]),
+    "cats_beam_select_bytes": (_c_size_t, [_c_int, _c_int, _c_int, _c_int]),
+    "cats_beam_select": (_c_int, [_c_void_p, _c_longlong, _c_void_p, _c_void_p, _c_int, _c_int, _c_int,
+                                  _c_int, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+                                  _c_void_p, _c_size_t, _c_void_p]),
     "cats_transpose": (_c_int, [_c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_void_p]),
     "cats_read_counters": (_c_int, [_c_void_p, ctypes.POINTER(_c_int), ctypes.POINTER(_c_int),
                                     _c_void_p]),

@@ -15,6 +15,13 @@ namespace cats {
 
 int g_use_pdl = 1;
 
+thread_local cudaError_t g_last_cuda = cudaSuccess;
+int launch_status(cudaError_t e) {
+  if (e == cudaSuccess) return CATS_OK;
+  g_last_cuda = e;
+  return CATS_ERR_CUDA;
+}
+
 // Per-device properties, queried once per device (no allocation involved).
 const DevInfo& dev_info() {
   static DevInfo info[64];
@@ -61,8 +68,6 @@ namespace {
 
 using namespace cats;
 
-thread_local cudaError_t g_last_cuda = cudaSuccess;
-
 int esize(int dtype) { return dtype == CATS_F32 ? 4 : 2; }
 int vecn(int dtype) { return dtype == CATS_F32 ? 4 : 8; }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -81,11 +86,7 @@ int check_ws(void* ws, size_t ws_bytes, int H, int I, WsPtrs* p) {
   return CATS_OK;
 }
 
-int cuda_status(cudaError_t e) {
-  if (e == cudaSuccess) return CATS_OK;
-  g_last_cuda = e;
-  return CATS_ERR_CUDA;
-}
+int cuda_status(cudaError_t e) { return launch_status(e); }
 
 // FN<T>(args...) for the runtime dtype
 #define CATS_DISPATCH(dtype, FN, ...)                                  \
@@ -422,6 +423,10 @@ const char* cats_status_string(int status) {
     case CATS_ERR_STATIC_LIMIT:
       return "shape needs more scratch than the built-in array of cats_mlp_static holds "
              "(see cats_mlp_static_limit); use cats_mlp with a caller-provided workspace";
+    case CATS_ERR_RANGE:
+      return "a size is outside the range of this entry point (cache: head_dim 32, 64, 96 or 128, "
+             "page 16, 32, 64 or 128, at most 1024 sequences; beam selection: at most 32 beams and "
+             "32 results)";
     default: return "unknown status";
   }
 }

@@ -1,0 +1,230 @@
+// extern "C" entry points of the paged 8-bit cache and of beam selection: argument checks, grid
+// sizing and launches.
+#include <math.h>
+
+#include "cats_beam.cuh"
+#include "cats_kv8_attn.cuh"
+#include "cats_run.cuh"
+
+namespace {
+
+using namespace cats;
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool known_dtype(int d) { return d == CATS_F32 || d == CATS_F16 || d == CATS_BF16; }
+int esize(int dtype) { return dtype == CATS_F32 ? 4 : 2; }
+
+int check_cache(const cats_kv8* c) {
+  if (!c || !c->codes || !c->scales || !c->table || !c->lens || !c->refs || !c->status) return CATS_ERR_NULL;
+  if (!aligned16(c->codes)) return CATS_ERR_ALIGN;
+  if (c->n_layers < 1 || c->n_pages < 1 || c->n_seqs < 1 || c->n_seqs > kKvMaxSeqs || c->max_pages < 1 ||
+      c->n_kv_heads < 1 || c->n_kv_heads > 1024)
+    return CATS_ERR_RANGE;
+  if (c->page != 16 && c->page != 32 && c->page != 64 && c->page != 128) return CATS_ERR_RANGE;
+  if (c->head_dim != 32 && c->head_dim != 64 && c->head_dim != 96 && c->head_dim != 128) return CATS_ERR_RANGE;
+  if ((long long)c->max_pages * c->page > 0x7fffffffLL) return CATS_ERR_RANGE;
+  return CATS_OK;
+}
+
+// New tokens: `tokens` of them, by cu or the same number of every sequence.
+int check_tokens(const cats_kv8* c, const int* cu, int tokens, int n_heads) {
+  if (tokens < 1 || n_heads < 1 || n_heads % c->n_kv_heads || n_heads > 16384) return CATS_ERR_RANGE;
+  if ((long long)tokens * n_heads > 0x7fffffffLL) return CATS_ERR_RANGE;
+  if (!cu && tokens % c->n_seqs) return CATS_ERR_RANGE;
+  return CATS_OK;
+}
+
+template <typename T>
+cudaError_t append(const cats_kv8& c, int layer, const void* qkv, long long ld, const int* cu, int tokens,
+                   const void* cosv, const void* sinv, void* q_out, int nh, cudaStream_t st) {
+  KvAppendArgs<T> A;
+  A.qkv = (const T*)qkv;
+  A.ld = ld;
+  A.cosv = (const T*)cosv;
+  A.sinv = (const T*)sinv;
+  A.q_out = (T*)q_out;
+  A.cu = cu;
+  A.uniform = cu ? 0 : tokens / c.n_seqs;
+  A.tokens = tokens;
+  A.nh = nh;
+  A.layer = layer;
+  const int tpr = c.head_dim / 16;
+  const int threads = (c.page / 4 * tpr + 31) / 32 * 32;
+  const int rows = threads / tpr * 4;
+  const long long units = cu ? (long long)tokens / c.page + 2LL * (tokens < c.n_seqs ? tokens : c.n_seqs)
+                             : (long long)c.n_seqs * kv_units(A.uniform, c.page);
+  const long long kv_blocks = units * 2 * c.n_kv_heads;
+  const long long q_blocks = q_out ? ((long long)tokens * nh + rows - 1) / rows : 0;
+  if (kv_blocks + q_blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+  A.units = (int)units;
+  A.kv_blocks = (int)kv_blocks;
+  return launch(k_kv8_append<T>, dim3((unsigned)(kv_blocks + q_blocks)), dim3(threads), 0, st, c, A);
+}
+
+template <typename T>
+cudaError_t attend(const cats_kv8& c, int layer, const void* q, long long q_ld, const int* cu, int tokens, int nh,
+                   float scale, void* out, cudaStream_t st) {
+  KvAttnArgs<T> A;
+  A.q = (const T*)q;
+  A.q_ld = q_ld;
+  A.out = (T*)out;
+  A.cu = cu;
+  A.uniform = cu ? 0 : tokens / c.n_seqs;
+  A.tokens = tokens;
+  A.nh = nh;
+  A.layer = layer;
+  A.scale = scale * 1.4426950408889634f;
+  const long long warps = (long long)tokens * nh;
+  return launch(k_kv8_attend_simple<T>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, st, c, A);
+}
+
+size_t beam_keys(int rows, int k) { return (size_t)rows * k; }
+
+}  // namespace
+
+extern "C" {
+
+int cats_kv8_grow(const cats_kv8* cache, const int* cu, int n_new, void* stream) {
+  int s = check_cache(cache);
+  if (s) return s;
+  if (!cu && n_new < 1) return CATS_ERR_RANGE;
+  return launch_status(launch(k_kv8_grow, dim3(1), dim3(kPlanThreads), 0, (cudaStream_t)stream, *cache, cu, n_new));
+}
+
+int cats_kv8_append(const cats_kv8* cache, int layer, const void* qkv, long long ld, const int* cu, int n_tokens,
+                    const void* cos_table, const void* sin_table, int rope_len, void* q_out, int n_heads, int dtype,
+                    void* stream) {
+  if (!known_dtype(dtype)) return CATS_ERR_DTYPE;
+  int s = check_cache(cache);
+  if (s) return s;
+  if ((s = check_tokens(cache, cu, n_tokens, n_heads))) return s;
+  if (layer < 0 || layer >= cache->n_layers) return CATS_ERR_RANGE;
+  if (!qkv || (!cos_table) != (!sin_table)) return CATS_ERR_NULL;
+  if (cos_table && rope_len < cache->max_pages * cache->page) return CATS_ERR_RANGE;
+  const long long width = ((long long)n_heads + 2 * cache->n_kv_heads) * cache->head_dim;
+  if (ld < width) return CATS_ERR_RANGE;
+  if (!aligned16(qkv) || (ld * esize(dtype)) % 16 || !aligned16(cos_table) || !aligned16(sin_table) ||
+      !aligned16(q_out))
+    return CATS_ERR_ALIGN;
+  cudaStream_t st = (cudaStream_t)stream;
+  cudaError_t e;
+  if (dtype == CATS_F32)
+    e = append<float>(*cache, layer, qkv, ld, cu, n_tokens, cos_table, sin_table, q_out, n_heads, st);
+  else if (dtype == CATS_F16)
+    e = append<__half>(*cache, layer, qkv, ld, cu, n_tokens, cos_table, sin_table, q_out, n_heads, st);
+  else
+    e = append<__nv_bfloat16>(*cache, layer, qkv, ld, cu, n_tokens, cos_table, sin_table, q_out, n_heads, st);
+  return launch_status(e);
+}
+
+size_t cats_kv8_attend_bytes(const cats_kv8* cache, int n_tokens, int n_heads) {
+  (void)cache;
+  (void)n_tokens;
+  (void)n_heads;
+  return 16;
+}
+
+int cats_kv8_attend(const cats_kv8* cache, int layer, const void* q, long long q_ld, const int* cu, int n_tokens,
+                    int n_heads, float scale, void* out, void* ws, size_t ws_bytes, int dtype, void* stream) {
+  if (!known_dtype(dtype)) return CATS_ERR_DTYPE;
+  int s = check_cache(cache);
+  if (s) return s;
+  if ((s = check_tokens(cache, cu, n_tokens, n_heads))) return s;
+  if (layer < 0 || layer >= cache->n_layers || !(fabsf(scale) < INFINITY)) return CATS_ERR_RANGE;
+  if (!q || !out || !ws) return CATS_ERR_NULL;
+  if (q_ld < (long long)n_heads * cache->head_dim) return CATS_ERR_RANGE;
+  if (!aligned16(q) || (q_ld * esize(dtype)) % 16 || !aligned16(out) || !aligned16(ws)) return CATS_ERR_ALIGN;
+  if (ws_bytes < cats_kv8_attend_bytes(cache, n_tokens, n_heads)) return CATS_ERR_WORKSPACE;
+  cudaStream_t st = (cudaStream_t)stream;
+  cudaError_t e;
+  if (dtype == CATS_F32) e = attend<float>(*cache, layer, q, q_ld, cu, n_tokens, n_heads, scale, out, st);
+  else if (dtype == CATS_F16) e = attend<__half>(*cache, layer, q, q_ld, cu, n_tokens, n_heads, scale, out, st);
+  else e = attend<__nv_bfloat16>(*cache, layer, q, q_ld, cu, n_tokens, n_heads, scale, out, st);
+  return launch_status(e);
+}
+
+size_t cats_kv8_reorder_bytes(const cats_kv8* cache) {
+  return cache && cache->n_seqs > 0 ? sizeof(KvCopy) * ((size_t)cache->n_seqs + 1) : 0;
+}
+
+int cats_kv8_reorder(const cats_kv8* cache, const int* parents, void* ws, size_t ws_bytes, void* stream) {
+  int s = check_cache(cache);
+  if (s) return s;
+  if (!parents || !ws) return CATS_ERR_NULL;
+  if (!aligned16(ws)) return CATS_ERR_ALIGN;
+  if (ws_bytes < cats_kv8_reorder_bytes(cache)) return CATS_ERR_WORKSPACE;
+  cudaStream_t st = (cudaStream_t)stream;
+  int* n_copies = (int*)ws;
+  KvCopy* copies = (KvCopy*)ws + 1;
+  // a strip holds `width` columns of every row (at most 64 KB with the two arrays beside it)
+  const int n = cache->n_seqs;
+  int width = 32;
+  while (width > 8 && (size_t)n * (width + 2) * 4 > 48 * 1024) width >>= 1;
+  const size_t smem = (size_t)n * (width + 2) * sizeof(int);
+  cudaError_t e = launch(k_kv8_reorder_table, dim3((cache->max_pages + width - 1) / width), dim3(256), smem, st,
+                         *cache, parents, width);
+  if (e == cudaSuccess)
+    e = launch(k_kv8_reorder_plan, dim3(1), dim3(kPlanThreads), 0, st, *cache, parents, n_copies, copies);
+  if (e == cudaSuccess)
+    e = launch(k_kv8_copy, dim3(dev_info().sms * 4), dim3(256), 0, st, *cache, (const int*)n_copies,
+               (const KvCopy*)copies);
+  return launch_status(e);
+}
+
+size_t cats_kv8_compact_bytes(const cats_kv8* cache) {
+  return cache && cache->n_pages > 0 ? (sizeof(KvCopy) + sizeof(int)) * (size_t)cache->n_pages + sizeof(KvCopy) : 0;
+}
+
+int cats_kv8_compact(const cats_kv8* cache, int* n_live, void* ws, size_t ws_bytes, void* stream) {
+  int s = check_cache(cache);
+  if (s) return s;
+  if (!n_live || !ws) return CATS_ERR_NULL;
+  if (!aligned16(ws)) return CATS_ERR_ALIGN;
+  if (ws_bytes < cats_kv8_compact_bytes(cache)) return CATS_ERR_WORKSPACE;
+  cudaStream_t st = (cudaStream_t)stream;
+  int* n_moves = (int*)ws;
+  KvCopy* moves = (KvCopy*)ws + 1;
+  int* remap = (int*)(moves + cache->n_pages);
+  cudaError_t e = launch(k_kv8_compact_plan, dim3(1), dim3(kPlanThreads), 0, st, *cache, n_live, n_moves, moves, remap);
+  if (e == cudaSuccess)
+    e = launch(k_kv8_compact_move, dim3(dev_info().sms * 4), dim3(256), 0, st, *cache, (const int*)n_moves,
+               (const KvCopy*)moves, (const int*)remap);
+  return launch_status(e);
+}
+
+size_t cats_beam_select_bytes(int n, int beams, int vocab, int k) {
+  if (n < 1 || beams < 1 || vocab < 1 || k < 1) return 0;
+  const size_t rows = (size_t)n * beams;
+  return rows * sizeof(BeamPart) + beam_keys((int)rows, k) * sizeof(unsigned long long) + 16;
+}
+
+int cats_beam_select(const void* logits, long long ld, const float* scores, const uint8_t* done, int n, int beams,
+                     int vocab, int k, int eos, int dtype, float* out_scores, int* out_rows, long long* out_tokens,
+                     uint8_t* out_done, void* ws, size_t ws_bytes, void* stream) {
+  if (!known_dtype(dtype)) return CATS_ERR_DTYPE;
+  if (n < 1 || beams < 1 || beams > kBeamMaxBeams || vocab < 1 || k < 1 || k > kBeamMaxK || ld < vocab)
+    return CATS_ERR_RANGE;
+  if ((long long)n * beams > 0x7fffffffLL || (long long)beams * vocab < k) return CATS_ERR_RANGE;
+  if (done && (eos < 0 || eos >= vocab)) return CATS_ERR_RANGE;
+  if (!logits || !scores || !out_scores || !out_rows || !out_tokens || !ws) return CATS_ERR_NULL;
+  if (reinterpret_cast<uintptr_t>(logits) % esize(dtype) || !aligned16(ws)) return CATS_ERR_ALIGN;
+  if (ws_bytes < cats_beam_select_bytes(n, beams, vocab, k)) return CATS_ERR_WORKSPACE;
+  cudaStream_t st = (cudaStream_t)stream;
+  BeamArgs A;
+  const int rows = n * beams;
+  A.logits = logits; A.ld = ld; A.scores = scores; A.done = done;
+  A.n = n; A.beams = beams; A.vocab = vocab; A.k = k; A.eos = eos; A.splits = 1;
+  A.keys = (unsigned long long*)ws;
+  A.parts = (BeamPart*)(A.keys + beam_keys(rows, k));
+  A.out_scores = out_scores; A.out_rows = out_rows; A.out_tokens = out_tokens; A.out_done = out_done;
+  cudaError_t e;
+  const dim3 grid(rows), block(kBeamThreads);
+  if (dtype == CATS_F32) e = launch(k_beam_rows_simple<float>, grid, block, 0, st, A);
+  else if (dtype == CATS_F16) e = launch(k_beam_rows_simple<__half>, grid, block, 0, st, A);
+  else e = launch(k_beam_rows_simple<__nv_bfloat16>, grid, block, 0, st, A);
+  if (e != cudaSuccess) return launch_status(e);
+  const size_t smem = (size_t)beams * k * 8 + (size_t)beams * A.splits * k * 8 + (size_t)beams * 8 + (size_t)beams * k * 4;
+  return launch_status(launch(k_beam_join, dim3(n), block, smem, st, A));
+}
+
+}  // extern "C"

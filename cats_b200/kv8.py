@@ -1,0 +1,268 @@
+"""Paged key/value cache in 8 bits (``cats_kv8_*`` of include/cats_b200.h).
+
+A pool of pages holds the keys and values of all layers as e4m3 codes with one power-of-two scale
+per (layer, page, keys or values, head): half the memory and half the bytes per decoded token of the
+16-bit cache.  Every sequence has a row in a page table; sequences that continue the same beginning
+share its full pages.  Table, lengths and counts are device tensors and every method only launches
+kernels on the current stream (``fork``, ``free`` and ``check``, which take or give host values,
+excepted), so a decode step over the cache can sit in a CUDA graph::
+
+    cache = KVCache8(n_layers=32, n_pages=2048, n_seqs=16, max_len=4096, n_kv_heads=8, head_dim=128)
+    cache.grow(1)                                   # one more token for every sequence
+    for l in range(32):
+        q = cache.append(l, qkv, n_heads, cos, sin) # rotary embedding, keys and values into the cache
+        o = cache.attend(l, q)                      # causal attention over it
+    cache.reorder(parents)                          # sequence i continues sequence parents[i]
+
+The calls on one cache have to be ordered: one stream, or events between streams.  Its tensors keep
+their addresses; they may be read and filled in place.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Sequence, Tuple
+
+import torch
+
+from . import _lib
+from .ops import _DTYPES, _on, dtype_code
+
+PAGES, HEAD_DIMS, MAX_SEQS = (16, 32, 64, 128), (32, 64, 96, 128), 1024
+_STATUS = {1: "the pool has no free page left", 2: "a page id is out of range, or a shared page would have been written",
+           4: "a sequence is longer than the page table allows, or a length or position is negative",
+           8: "a parent is out of range", 16: "cu does not fit the number of tokens"}
+
+
+def _bad(msg: str) -> RuntimeError:
+    return RuntimeError("cats_b200.kv8: " + msg)
+
+
+class KVCache8:
+    """See the module docstring.  ``max_len``: tokens a sequence can have (rounded up to whole pages)."""
+
+    def __init__(self, n_layers: int, n_pages: int, n_seqs: int, max_len: int, n_kv_heads: int,
+                 head_dim: int, page: int = 64, device="cuda"):
+        dev = torch.device(device)
+        if dev.type != "cuda":
+            raise _bad("the cache needs a CUDA device (no CPU path)")
+        if min(n_layers, n_pages, n_seqs, max_len, n_kv_heads) < 1:
+            raise _bad("sizes must be positive")
+        if page not in PAGES or head_dim not in HEAD_DIMS or n_seqs > MAX_SEQS:
+            raise _bad(f"page must be one of {PAGES}, head_dim one of {HEAD_DIMS}, n_seqs at most {MAX_SEQS}")
+        z = lambda *s, dt: torch.zeros(s, dtype=dt, device=dev)  # noqa: E731
+        self._adopt(z(n_layers, n_pages, 2, n_kv_heads, page, head_dim, dt=torch.uint8).view(torch.float8_e4m3fn),
+                    z(n_layers, n_pages, 2, n_kv_heads, dt=torch.float32),
+                    torch.full((n_seqs, (max_len + page - 1) // page), -1, dtype=torch.int32, device=dev),
+                    z(n_seqs, dt=torch.int32), z(n_pages, dt=torch.int32))
+
+    @classmethod
+    def from_tensors(cls, codes: torch.Tensor, scales: torch.Tensor, table: torch.Tensor,
+                     lens: torch.Tensor, refs: torch.Tensor) -> "KVCache8":
+        """A cache over existing device tensors: codes [layers, pages, 2, kv_heads, page, head_dim]
+        (float8_e4m3fn or uint8), scales [layers, pages, 2, kv_heads] float32 powers of two, table
+        [seqs, max_pages], lens [seqs], refs [pages] int32.  They are used in place."""
+        self = cls.__new__(cls)
+        self._adopt(codes, scales, table, lens, refs)
+        return self
+
+    def _adopt(self, codes, scales, table, lens, refs) -> None:
+        for t, name, dts, dim in ((codes, "codes", (torch.float8_e4m3fn, torch.uint8), 6),
+                                  (scales, "scales", (torch.float32,), 4), (table, "table", (torch.int32,), 2),
+                                  (lens, "lens", (torch.int32,), 1), (refs, "refs", (torch.int32,), 1)):
+            if not isinstance(t, torch.Tensor) or t.dtype not in dts or t.dim() != dim:
+                raise _bad(f"{name} must be a {dim}-D tensor of {' or '.join(map(str, dts))}")
+            if not t.is_cuda or t.device != codes.device or not t.is_contiguous():
+                raise _bad(f"{name} must be contiguous and on the codes' CUDA device (there is no CPU path)")
+        L, P, two, nkv, page, hd = codes.shape
+        if two != 2 or tuple(scales.shape) != (L, P, 2, nkv) or lens.shape[0] != table.shape[0] or refs.shape[0] != P:
+            raise _bad("the shapes of codes, scales, table, lens and refs do not fit together")
+        if page not in PAGES or hd not in HEAD_DIMS or table.shape[0] > MAX_SEQS or min(*codes.shape, *table.shape) < 1:
+            raise _bad(f"page must be one of {PAGES}, head_dim one of {HEAD_DIMS}, sequences 1 .. {MAX_SEQS}")
+        self.codes, self.scales, self.table, self.lens, self.refs = codes, scales, table, lens, refs
+        self.status = torch.zeros(1, dtype=torch.int32, device=codes.device)
+        self.device = codes.device
+        self.n_layers, self.n_pages, self.n_kv_heads, self.page, self.head_dim = L, P, nkv, page, hd
+        self.n_seqs, self.max_pages = table.shape
+        self.max_len = self.max_pages * page
+        self._c = _lib.Kv8(codes.data_ptr(), scales.data_ptr(), table.data_ptr(), lens.data_ptr(), refs.data_ptr(),
+                           self.status.data_ptr(), L, P, self.n_seqs, self.max_pages, nkv, page, hd)
+        self._p = ctypes.byref(self._c)
+        lib = _lib.lib()
+        self._grow, self._append, self._attend = lib.cats_kv8_grow, lib.cats_kv8_append, lib.cats_kv8_attend
+        self._reorder, self._compact = lib.cats_kv8_reorder, lib.cats_kv8_compact
+        self._attend_bytes = lib.cats_kv8_attend_bytes
+        self._reorder_nbytes = int(lib.cats_kv8_reorder_bytes(self._p))
+        self._compact_nbytes = int(lib.cats_kv8_compact_bytes(self._p))
+
+    # ---- argument checks ----------------------------------------------------------------------------
+    def _stream(self) -> int:
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def _cu(self, cu: Optional[torch.Tensor]) -> Optional[int]:
+        if cu is None:
+            return None
+        if not isinstance(cu, torch.Tensor) or cu.dtype != torch.int32 or cu.device != self.device \
+                or not cu.is_contiguous() or cu.numel() != self.n_seqs + 1:
+            raise _bad(f"cu must be a contiguous int32 tensor of {self.n_seqs + 1} elements on {self.device}")
+        return cu.data_ptr()
+
+    def _tokens(self, t: torch.Tensor, name: str, cu) -> int:
+        if not isinstance(t, torch.Tensor) or t.device != self.device:
+            raise _bad(f"{name} must be a tensor on {self.device}")
+        n = t.shape[0]
+        if cu is None and n % self.n_seqs:
+            raise _bad(f"{name} has {n} rows, not a multiple of the {self.n_seqs} sequences: pass cu")
+        return n
+
+    def _layer(self, layer: int) -> None:
+        if not 0 <= layer < self.n_layers:
+            raise _bad(f"layer {layer} is out of range (0 .. {self.n_layers - 1})")
+
+    # ---- steps ------------------------------------------------------------------------------------------
+    def grow(self, n_new: int = 1, cu: Optional[torch.Tensor] = None) -> None:
+        """``lens += n_new`` (or the counts of ``cu``), taking the pages that needs (``cats_kv8_grow``)."""
+        if cu is None and n_new < 1:
+            raise _bad("n_new must be positive")
+        with _on(self.device):
+            st = self._grow(self._p, self._cu(cu), n_new, self._stream())
+        if st:
+            _lib.check(st, "cats_kv8_grow")
+
+    def append(self, layer: int, qkv: torch.Tensor, n_heads: int, cos: Optional[torch.Tensor] = None,
+               sin: Optional[torch.Tensor] = None, cu: Optional[torch.Tensor] = None,
+               q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Rotary embedding of the newest tokens' queries and keys and the quantising cache write
+        (``cats_kv8_append``).  qkv (tokens, (n_heads + 2 kv_heads) head_dim), rows may be strided;
+        cos, sin (>= max_len, head_dim), or None for no rotation; ``cu`` int32 (seqs + 1): first row of
+        every sequence, or None for the same number of rows each.  Returns the queries (tokens,
+        n_heads, head_dim)."""
+        n = self._tokens(qkv, "qkv", cu)
+        hd, dt = self.head_dim, qkv.dtype
+        code = _DTYPES[dt] if dt in _DTYPES else dtype_code(dt)
+        if qkv.dim() != 2 or qkv.shape[1] != (n_heads + 2 * self.n_kv_heads) * hd or n_heads < 1 \
+                or n_heads % self.n_kv_heads:
+            raise _bad(f"qkv must be (tokens, (n_heads + 2 * {self.n_kv_heads}) * {hd}) with n_heads a multiple of "
+                       f"{self.n_kv_heads}, got {tuple(qkv.shape)} and {n_heads} heads")
+        if qkv.stride(1) != 1:
+            raise _bad("the rows of qkv must be contiguous")
+        self._layer(layer)
+        pc = ps = None
+        rope = 0
+        if cos is not None or sin is not None:
+            for t in (cos, sin):
+                if not isinstance(t, torch.Tensor) or t.dtype != dt or t.device != self.device or t.dim() != 2 \
+                        or not t.is_contiguous() or t.shape[1] != hd or t.shape != cos.shape:
+                    raise _bad(f"cos and sin must be contiguous (positions, {hd}) tables of {dt} on {self.device}")
+            rope = cos.shape[0]
+            if rope < self.max_len:
+                raise _bad(f"cos and sin hold {rope} positions, the cache up to {self.max_len}")
+            pc, ps = cos.data_ptr(), sin.data_ptr()
+        if q_out is None:
+            q_out = torch.empty((n, n_heads, hd), dtype=dt, device=self.device)
+        elif q_out.dtype != dt or q_out.device != self.device or not q_out.is_contiguous() \
+                or q_out.numel() != n * n_heads * hd:
+            raise _bad("q_out must be contiguous with tokens * n_heads * head_dim elements of qkv's type")
+        if n == 0:
+            return q_out
+        with _on(self.device):
+            st = self._append(self._p, layer, qkv.data_ptr(), qkv.stride(0) if n > 1 else qkv.shape[1], self._cu(cu), n,
+                              pc, ps, rope, q_out.data_ptr(), n_heads, code, self._stream())
+        if st:
+            _lib.check(st, "cats_kv8_append")
+        return q_out
+
+    def attend(self, layer: int, q: torch.Tensor, cu: Optional[torch.Tensor] = None,
+               scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Causal attention of the newest tokens over the cache (``cats_kv8_attend``).  q (tokens,
+        n_heads, head_dim), tokens as in ``append``; ``scale`` defaults to head_dim ** -0.5.  Returns a
+        tensor like q.  Every token sees the positions of its sequence up to its own."""
+        n = self._tokens(q, "q", cu)
+        hd, dt = self.head_dim, q.dtype
+        code = _DTYPES[dt] if dt in _DTYPES else dtype_code(dt)
+        if q.dim() != 3 or q.shape[2] != hd or q.shape[1] % self.n_kv_heads or q.shape[1] < 1:
+            raise _bad(f"q must be (tokens, heads, {hd}) with heads a multiple of {self.n_kv_heads}, got {tuple(q.shape)}")
+        nh = q.shape[1]
+        if q.stride(2) != 1 or (q.stride(1) != hd and nh > 1):
+            raise _bad("the heads of a token must be contiguous in q")
+        self._layer(layer)
+        if out is None:
+            out = torch.empty((n, nh, hd), dtype=dt, device=self.device)
+        elif out.dtype != dt or out.device != self.device or not out.is_contiguous() or out.numel() != n * nh * hd:
+            raise _bad("out must be contiguous with as many elements as q, of q's type")
+        if n == 0:
+            return out
+        with _on(self.device):
+            nbytes = self._attend_bytes(self._p, n, nh)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+            st = self._attend(self._p, layer, q.data_ptr(), q.stride(0) if n > 1 else nh * hd, self._cu(cu), n, nh,
+                              hd ** -0.5 if scale is None else scale, out.data_ptr(), ws.data_ptr(), nbytes, code,
+                              self._stream())
+        if st:
+            _lib.check(st, "cats_kv8_attend")
+        return out
+
+    # ---- pages --------------------------------------------------------------------------------------------
+    def reorder(self, parents: torch.Tensor) -> None:
+        """Sequence i continues what sequence ``parents[i]`` (int32, on the device) was before the call,
+        -1: it becomes empty (``cats_kv8_reorder``).  Full pages are shared, the page that is still being
+        filled is copied for every child but the first."""
+        if not isinstance(parents, torch.Tensor) or parents.dtype != torch.int32 or parents.device != self.device \
+                or not parents.is_contiguous() or parents.numel() != self.n_seqs:
+            raise _bad(f"parents must be a contiguous int32 tensor of {self.n_seqs} elements on {self.device}")
+        with _on(self.device):
+            ws = torch.empty(self._reorder_nbytes, dtype=torch.uint8, device=self.device)
+            st = self._reorder(self._p, parents.data_ptr(), ws.data_ptr(), self._reorder_nbytes, self._stream())
+        if st:
+            _lib.check(st, "cats_kv8_reorder")
+
+    def _host_parents(self, changes) -> torch.Tensor:
+        parents = list(range(self.n_seqs))
+        for dst, src in changes:
+            if not 0 <= dst < self.n_seqs or not -1 <= src < self.n_seqs:
+                raise _bad(f"sequence {dst if not 0 <= dst < self.n_seqs else src} is out of range (0 .. {self.n_seqs - 1})")
+            parents[dst] = src
+        return torch.tensor(parents, dtype=torch.int32).to(self.device)
+
+    def fork(self, src: Sequence[int], dst: Sequence[int]) -> None:
+        """Sequence dst[i] becomes a continuation of src[i] (what dst[i] held is freed)."""
+        src, dst = [int(i) for i in src], [int(i) for i in dst]
+        if len(src) != len(dst) or len(set(dst)) != len(dst):
+            raise _bad("fork needs as many sources as targets, every target once")
+        if any(i < 0 for i in src):
+            raise _bad("fork sources must be sequences")
+        self.reorder(self._host_parents(zip(dst, src)))
+
+    def free(self, seqs: Sequence[int]) -> None:
+        """The sequences become empty; pages that nobody else holds are free again."""
+        self.reorder(self._host_parents((int(i), -1) for i in seqs))
+
+    def compact(self) -> torch.Tensor:
+        """Move the live pages to the front of the pool (``cats_kv8_compact``).  Returns their number
+        as a 0-dim int32 device tensor; the page ids from there on are free."""
+        with _on(self.device):
+            n = torch.empty((), dtype=torch.int32, device=self.device)
+            ws = torch.empty(self._compact_nbytes, dtype=torch.uint8, device=self.device)
+            st = self._compact(self._p, n.data_ptr(), ws.data_ptr(), self._compact_nbytes, self._stream())
+        if st:
+            _lib.check(st, "cats_kv8_compact")
+        return n
+
+    # ---- host side ---------------------------------------------------------------------------------------------
+    def check(self) -> None:
+        """Raise if a kernel found device data that does not fit (synchronises).  The status word
+        stays set until ``status.zero_()``."""
+        bits = int(self.status.item())
+        if bits:
+            raise _bad("; ".join(text for b, text in _STATUS.items() if bits & b) + f" (status {bits})")
+
+    def read(self, layer: int, seq: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        """(keys, values) of one sequence, fp32 [kv_heads, len, head_dim] (synchronises)."""
+        self._layer(layer)
+        if not 0 <= seq < self.n_seqs:
+            raise _bad(f"sequence {seq} is out of range (0 .. {self.n_seqs - 1})")
+        n = int(self.lens[seq])
+        ids = self.table[seq, :(n + self.page - 1) // self.page].long()
+        kv = self.codes.view(torch.float8_e4m3fn)[layer].view(torch.uint8)[ids].view(torch.float8_e4m3fn).float()
+        kv = (kv * self.scales[layer][ids][..., None, None]).permute(1, 2, 0, 3, 4)
+        kv = kv.reshape(2, self.n_kv_heads, ids.numel() * self.page, self.head_dim)[:, :, :n]
+        return kv[0], kv[1]

@@ -419,6 +419,50 @@ def rope_cache(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: tor
                                               dtype_code(dt), _stream(dev)), "cats_rope_cache")
 
 
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, done: Optional[torch.Tensor] = None,
+                eos: int = -1):
+    """The k best continuations of every batch item over its beams and the vocabulary
+    (``cats_beam_select``).  logits (n, beams, vocab), rows may be strided; scores (n, beams) float32,
+    the beams' log-probabilities so far; ``done`` (n, beams) bool: beams that have ended (they go on
+    with ``eos`` at their score).  Returns (scores (n, k) float32, rows (n, k) int32 = item * beams +
+    beam, tokens (n, k) int64, done (n, k) bool), best first, ties to the lowest (beam, token)."""
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda or logits.dim() != 3:
+        raise RuntimeError("cats_b200: logits must be a CUDA tensor (n, beams, vocab) (there is no CPU path)")
+    dev = logits.device
+    n, beams, vocab = logits.shape
+    s0, s1, s2 = logits.stride()
+    ld = s1 if beams > 1 else s0
+    if (s2 != 1 and vocab > 1) or (n > 1 and beams > 1 and s0 != beams * s1):
+        raise RuntimeError("cats_b200: logits must have contiguous rows at one distance from each other")
+    if n * beams <= 1:
+        ld = vocab
+    _req(scores, "scores", torch.float32, dev)
+    if scores.numel() != n * beams:
+        raise RuntimeError(f"cats_b200: scores must hold {n} x {beams} values")
+    if done is not None:
+        if done.dtype not in (torch.bool, torch.uint8) or done.device != dev or not done.is_contiguous() \
+                or done.numel() != n * beams:
+            raise RuntimeError(f"cats_b200: done must be a contiguous bool/uint8 tensor with {n} x {beams} values")
+        if not 0 <= eos < vocab:
+            raise RuntimeError("cats_b200: done needs eos, a token of the vocabulary")
+    if n < 1 or not 1 <= beams <= 32 or not 1 <= k <= min(32, beams * vocab):
+        raise RuntimeError(f"cats_b200: beam selection takes 1 .. 32 beams and 1 .. 32 results (got {n} x {beams}, k {k})")
+    out_scores = torch.empty((n, k), dtype=torch.float32, device=dev)
+    out_rows = torch.empty((n, k), dtype=torch.int32, device=dev)
+    out_tokens = torch.empty((n, k), dtype=torch.int64, device=dev)
+    out_done = torch.empty((n, k), dtype=torch.bool, device=dev)
+    L = _lib.lib()
+    with _on(dev):
+        nbytes = L.cats_beam_select_bytes(n, beams, vocab, k)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        st = L.cats_beam_select(logits.data_ptr(), ld, scores.data_ptr(), _ptr(done), n, beams, vocab, k, eos,
+                                dtype_code(logits.dtype), out_scores.data_ptr(), out_rows.data_ptr(),
+                                out_tokens.data_ptr(), out_done.data_ptr(), ws.data_ptr(), nbytes, _stream(dev))
+    if st:
+        _lib.check(st, "cats_beam_select")
+    return out_scores, out_rows, out_tokens, out_done
+
+
 def transpose(src: torch.Tensor) -> torch.Tensor:
     """(R, C) -> new contiguous (C, R) through ``cats_transpose``."""
     _req(src, "matrix")

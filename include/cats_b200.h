@@ -42,7 +42,8 @@ enum {
   CATS_ERR_WORKSPACE = -5,  /* workspace too small for (B, H, I) */
   CATS_ERR_CUDA = -6,       /* CUDA runtime reported an error at launch; see cats_last_cuda_error */
   CATS_ERR_MODE = -7,       /* unknown mode / flag combination */
-  CATS_ERR_STATIC_LIMIT = -8 /* cats_mlp_static: shape needs more scratch than its built-in array */
+  CATS_ERR_STATIC_LIMIT = -8, /* cats_mlp_static: shape needs more scratch than its built-in array */
+  CATS_ERR_RANGE = -9       /* cats_kv8_*, cats_beam_select: a size is outside the documented range */
 };
 
 /* how cats_down / cats_updown / cats_mlp deliver the result */
@@ -386,6 +387,114 @@ int cats_read_counters(const void* ws, int* n_active, int* device_status, void* 
  */
 int cats_export_list(const void* ws, size_t ws_bytes, int B, int H, int I, int dtype,
                      int64_t* idx_out, void* val_out, void* stream);
+
+/*
+ * ---- Paged key/value cache in 8 bits ------------------------------------------------------------
+ *
+ * A pool of pages holds the keys and values of all layers as e4m3 codes with one power-of-two scale
+ * for each (layer, page, keys or values, head): value = code * scale, scale = 2^e, -24 <= e <= 60
+ * (values beyond 448 * 2^60 saturate; infinities are stored as NaN).  A page holds `page` tokens of
+ * one sequence; row i of the page table lists the pages of sequence i in order, -1 behind the last;
+ * lens[i] is its number of tokens and it holds ceil(lens[i] / page) pages.  refs counts the
+ * sequences that hold a page (0: free).  Full pages may be shared between sequences, a page that is
+ * still being filled belongs to one; cats_kv8_reorder keeps that so.
+ * All arrays live in device memory, the struct itself in host memory.  A zero-initialised pool with
+ * table -1 is an empty cache.  Calls on one cache have to be ordered (one stream, or events).
+ *   page 16, 32, 64 or 128; head_dim 32, 64, 96 or 128; n_seqs <= 1024; codes 16-byte aligned.
+ * Ids and lengths are device data and are checked on the device: what does not fit is left out
+ * (never read or written out of range) and recorded in *status, bits that stay until the caller
+ * clears them: 1 the pool has no page left, 2 a page id is out of range or a page that is shared
+ * would have been written, 4 a sequence is longer than max_pages pages (or has a negative length or
+ * position), 8 a parent is out of range, 16 cu does not fit the number of tokens.
+ * No reference counterpart (the reference leaves the cache to HF's modelling code).
+ */
+typedef struct cats_kv8 {
+  void* codes;    /* [n_layers, n_pages, 2, n_kv_heads, page, head_dim] e4m3 */
+  float* scales;  /* [n_layers, n_pages, 2, n_kv_heads]                      */
+  int* table;     /* [n_seqs, max_pages]                                     */
+  int* lens;      /* [n_seqs]                                                */
+  int* refs;      /* [n_pages]                                               */
+  int* status;    /* [1]                                                     */
+  int n_layers, n_pages, n_seqs, max_pages, n_kv_heads, page, head_dim;
+} cats_kv8;
+
+/*
+ * The sequences become longer: lens[i] += n_i, with the pages that takes, the lowest free ids first
+ * in the order of the sequences.  n_i = cu[i + 1] - cu[i] (device memory, [n_seqs + 1], ascending
+ * from 0), or n_new for every sequence when cu is NULL.  Called once per step, before the layers'
+ * cats_kv8_append.  A sequence that does not get its pages keeps its length (status bit 1 or 4); so
+ * do those after it that need a page.
+ */
+int cats_kv8_grow(const cats_kv8* cache, const int* cu, int n_new, void* stream);
+
+/*
+ * The keys and values of the newest tokens enter the cache, their queries are rotated.
+ *   qkv: n_tokens rows, ld elements apart, of (n_heads + 2 n_kv_heads) * head_dim elements (q, k, v
+ *   heads in that order), sequence by sequence: those of sequence i are rows cu[i] .. cu[i + 1], or
+ *   n_tokens / n_seqs of each when cu is NULL.  They are the LAST tokens of the sequence: row j of n_i
+ *   has position lens[i] - n_i + j.
+ *   cos_table, sin_table [rope_len, head_dim], rope_len >= max_pages * page (rotate-half embedding, as
+ *   cats_rope_cache), both NULL for keys and queries that need no rotation; q_out [n_tokens, n_heads,
+ *   head_dim] or NULL.
+ * The rotation is computed in fp32; q_out is rounded once, keys and values are quantised from fp32.
+ * A page's exponent is the least that holds its largest finite magnitude within 448 codes; where a
+ * page already holds rows it only grows, and the older codes are rescaled (exact but for codes that
+ * become subnormal).  Rows must be 16-byte aligned (qkv, ld, tables, q_out).
+ */
+int cats_kv8_append(const cats_kv8* cache, int layer, const void* qkv, long long ld, const int* cu,
+                    int n_tokens, const void* cos_table, const void* sin_table, int rope_len,
+                    void* q_out, int n_heads, int dtype, void* stream);
+
+/*
+ * Causal attention of the newest tokens over the cache: for each of n_tokens (order and cu as for
+ * cats_kv8_append; q rows q_ld elements apart, [n_heads, head_dim] each) and each head h
+ *   out = sum_p softmax_p(scale * q . k_p) v_p   over the positions p of the token's sequence up to
+ * its own; key head h / (n_heads / n_kv_heads).  Scores, softmax and sums in fp32.  A token without
+ * any position (an empty sequence) gives zeros; pages listed as -1 are left out (status bit 2).
+ * Positions behind the token are never read into its result, whatever they hold.
+ *   out [n_tokens, n_heads, head_dim]; ws: cats_kv8_attend_bytes(...) bytes of scratch, contents
+ *   irrelevant before and after.
+ */
+size_t cats_kv8_attend_bytes(const cats_kv8* cache, int n_tokens, int n_heads);
+int cats_kv8_attend(const cats_kv8* cache, int layer, const void* q, long long q_ld, const int* cu,
+                    int n_tokens, int n_heads, float scale, void* out, void* ws, size_t ws_bytes,
+                    int dtype, void* stream);
+
+/*
+ * Sequences continue sequences: sequence i becomes what sequence parents[i] (device memory,
+ * [n_seqs]) was before the call; -1 makes it empty.  Forking (parents[new] = old), freeing
+ * (parents[i] = -1) and a beam search's reordering are all this call.  Full pages are shared; a page
+ * that is still being filled goes to the first child, and every other child gets the lowest free page
+ * and a copy of the filled rows in all layers.  Without a free page the child's entry is -1 (status
+ * bit 1).  ws: cats_kv8_reorder_bytes(cache) bytes of scratch.
+ */
+size_t cats_kv8_reorder_bytes(const cats_kv8* cache);
+int cats_kv8_reorder(const cats_kv8* cache, const int* parents, void* ws, size_t ws_bytes, void* stream);
+
+/*
+ * The live pages move to the front of the pool: with n live pages, the k-th live page at or above n
+ * goes to the k-th free id below n, in all layers, and the table and counts follow.  *n_live (device
+ * memory) = n; the ids from n on are free afterwards.  ws: cats_kv8_compact_bytes(cache) bytes.
+ */
+size_t cats_kv8_compact_bytes(const cats_kv8* cache);
+int cats_kv8_compact(const cats_kv8* cache, int* n_live, void* ws, size_t ws_bytes, void* stream);
+
+/*
+ * Beam search's selection.  logits [n, beams, vocab] (dtype), rows ld elements apart; scores
+ * [n, beams] fp32, the beams' log-probabilities so far; done [n, beams] or NULL, beams that have
+ * ended.  A candidate (beam w, token v) has score[w] + log_softmax(logits[w])[v]; an ended beam has
+ * the one candidate (w, eos) at its score.  The k best of an item, best first, ties to the lowest
+ * (w, v): out_scores [n, k] fp32, out_rows [n, k] = item * beams + w (parents for
+ * cats_kv8_reorder), out_tokens [n, k] int64, out_done [n, k] (may be NULL) = the beam had ended or
+ * the token is eos.  Tokens at -inf come last; a beam whose score or log-sum-exp is not finite (a NaN
+ * or +inf among its logits, all of them -inf) has only candidates at -inf.  The log-sum-exp is summed
+ * in fp32 over at most a few thousand values and in fp64 above that; candidates are compared in fp64.
+ *   beams <= 32, k <= 32, k <= beams * vocab.  ws: cats_beam_select_bytes(...) bytes of scratch.
+ */
+size_t cats_beam_select_bytes(int n, int beams, int vocab, int k);
+int cats_beam_select(const void* logits, long long ld, const float* scores, const uint8_t* done, int n,
+                     int beams, int vocab, int k, int eos, int dtype, float* out_scores, int* out_rows,
+                     long long* out_tokens, uint8_t* out_done, void* ws, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }
