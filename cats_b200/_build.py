@@ -24,6 +24,7 @@ UNITS = [("cats_abi.cu", [], "cats_abi.o")]
 for _id, _name in ((0, "f32"), (1, "f16"), (2, "bf16")):
     UNITS.append(("cats_inst_stage.cu", [f"-DCATS_ELEM_ID={_id}"], f"cats_inst_stage_{_name}.o"))
     UNITS.append(("cats_inst_mega.cu", [f"-DCATS_ELEM_ID={_id}"], f"cats_inst_mega_{_name}.o"))
+    UNITS.append(("cats_inst_kv8_attn.cu", [f"-DCATS_ELEM_ID={_id}"], f"cats_inst_kv8_attn_{_name}.o"))
 UNITS.append(("cats_inst_dense.cu", [], "cats_inst_dense.o"))
 UNITS.append(("cats_inst_kv8.cu", [], "cats_inst_kv8.o"))
 SOURCES = sorted({u[0] for u in UNITS})

@@ -3,8 +3,8 @@
 #include <math.h>
 
 #include "cats_beam.cuh"
-#include "cats_kv8_attn.cuh"
-#include "cats_run.cuh"
+#include "cats_kv8_run.cuh"
+#include "cats_kv8_steps.cuh"
 
 namespace {
 
@@ -32,6 +32,12 @@ int check_tokens(const cats_kv8* c, const int* cu, int tokens, int n_heads) {
   if ((long long)tokens * n_heads > 0x7fffffffLL) return CATS_ERR_RANGE;
   if (!cu && tokens % c->n_seqs) return CATS_ERR_RANGE;
   return CATS_OK;
+}
+
+// Units of one sequence have to fit 32 bits (cats_kv8_attn.cuh).
+bool units_fit(const cats_kv8* c, int tokens, int n_heads) {
+  const double units = (double)c->max_pages * c->page / kAttnUnit + 1;
+  return units * ((double)tokens * n_heads / kAttnRows + c->n_kv_heads) < 4294967296.0;
 }
 
 template <typename T>
@@ -63,7 +69,7 @@ cudaError_t append(const cats_kv8& c, int layer, const void* qkv, long long ld, 
 
 template <typename T>
 cudaError_t attend(const cats_kv8& c, int layer, const void* q, long long q_ld, const int* cu, int tokens, int nh,
-                   float scale, void* out, cudaStream_t st) {
+                   float scale, void* out, void* ws, cudaStream_t st) {
   KvAttnArgs<T> A;
   A.q = (const T*)q;
   A.q_ld = q_ld;
@@ -74,8 +80,9 @@ cudaError_t attend(const cats_kv8& c, int layer, const void* q, long long q_ld, 
   A.nh = nh;
   A.layer = layer;
   A.scale = scale * 1.4426950408889634f;
-  const long long warps = (long long)tokens * nh;
-  return launch(k_kv8_attend_simple<T>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, st, c, A);
+  A.parts = (float*)ws;
+  A.ctas = dev_info().sms;
+  return inst_kv8_attend<T>(c, A, st);
 }
 
 size_t beam_keys(int rows, int k) { return (size_t)rows * k; }
@@ -118,10 +125,8 @@ int cats_kv8_append(const cats_kv8* cache, int layer, const void* qkv, long long
 }
 
 size_t cats_kv8_attend_bytes(const cats_kv8* cache, int n_tokens, int n_heads) {
-  (void)cache;
-  (void)n_tokens;
-  (void)n_heads;
-  return 16;
+  if (!cache || cache->head_dim < 1 || n_tokens < 1 || n_heads < 1) return 0;
+  return sizeof(float) * 2 * (size_t)dev_info().sms * attn_part_floats(cache->head_dim);
 }
 
 int cats_kv8_attend(const cats_kv8* cache, int layer, const void* q, long long q_ld, const int* cu, int n_tokens,
@@ -131,15 +136,16 @@ int cats_kv8_attend(const cats_kv8* cache, int layer, const void* q, long long q
   if (s) return s;
   if ((s = check_tokens(cache, cu, n_tokens, n_heads))) return s;
   if (layer < 0 || layer >= cache->n_layers || !(fabsf(scale) < INFINITY)) return CATS_ERR_RANGE;
+  if (!units_fit(cache, n_tokens, n_heads)) return CATS_ERR_RANGE;
   if (!q || !out || !ws) return CATS_ERR_NULL;
   if (q_ld < (long long)n_heads * cache->head_dim) return CATS_ERR_RANGE;
   if (!aligned16(q) || (q_ld * esize(dtype)) % 16 || !aligned16(out) || !aligned16(ws)) return CATS_ERR_ALIGN;
   if (ws_bytes < cats_kv8_attend_bytes(cache, n_tokens, n_heads)) return CATS_ERR_WORKSPACE;
   cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e;
-  if (dtype == CATS_F32) e = attend<float>(*cache, layer, q, q_ld, cu, n_tokens, n_heads, scale, out, st);
-  else if (dtype == CATS_F16) e = attend<__half>(*cache, layer, q, q_ld, cu, n_tokens, n_heads, scale, out, st);
-  else e = attend<__nv_bfloat16>(*cache, layer, q, q_ld, cu, n_tokens, n_heads, scale, out, st);
+  if (dtype == CATS_F32) e = attend<float>(*cache, layer, q, q_ld, cu, n_tokens, n_heads, scale, out, ws, st);
+  else if (dtype == CATS_F16) e = attend<__half>(*cache, layer, q, q_ld, cu, n_tokens, n_heads, scale, out, ws, st);
+  else e = attend<__nv_bfloat16>(*cache, layer, q, q_ld, cu, n_tokens, n_heads, scale, out, ws, st);
   return launch_status(e);
 }
 
