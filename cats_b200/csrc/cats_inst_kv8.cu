@@ -34,10 +34,10 @@ int check_tokens(const cats_kv8* c, const int* cu, int tokens, int n_heads) {
   return CATS_OK;
 }
 
-// Units of one sequence have to fit 32 bits (cats_kv8_attn.cuh).
+// The units of a call have to fit 32 bits (cats_kv8_attn.cuh).
 bool units_fit(const cats_kv8* c, int tokens, int n_heads) {
-  const double units = (double)c->max_pages * c->page / kAttnUnit + 1;
-  return units * ((double)tokens * n_heads / kAttnRows + c->n_kv_heads) < 4294967296.0;
+  const double units = (double)c->max_pages * c->page / AttnShape<2>::kUnit + 1;
+  return units * ((double)tokens * n_heads / AttnShape<1>::kRows + (double)c->n_kv_heads * c->n_seqs) < 2147483648.0;
 }
 
 template <typename T>
@@ -126,7 +126,7 @@ int cats_kv8_append(const cats_kv8* cache, int layer, const void* qkv, long long
 
 size_t cats_kv8_attend_bytes(const cats_kv8* cache, int n_tokens, int n_heads) {
   if (!cache || cache->head_dim < 1 || n_tokens < 1 || n_heads < 1) return 0;
-  return sizeof(float) * 2 * (size_t)dev_info().sms * attn_part_floats(cache->head_dim);
+  return sizeof(float) * 2 * (size_t)dev_info().sms * attn_part_floats(kAttnMaxRows, cache->head_dim);
 }
 
 int cats_kv8_attend(const cats_kv8* cache, int layer, const void* q, long long q_ld, const int* cu, int n_tokens,

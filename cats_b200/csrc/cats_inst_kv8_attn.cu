@@ -5,12 +5,22 @@
 
 namespace cats {
 
+template <typename T, int HD, int NQ>
+static cudaError_t run_attend(const cats_kv8& c, const KvAttnArgs<T>& A, cudaStream_t st) {
+  using S = AttnShape<NQ>;
+  cudaError_t e = launch(k_kv8_attend<T, HD, NQ>, dim3(A.ctas), dim3(S::kThreads), attn_smem<NQ>(), st, c, A);
+  if (e != cudaSuccess) return e;
+  constexpr int per = kAttnJoinThreads / 32;
+  const long long ctas = ((long long)A.tokens * A.nh + per - 1) / per, most = 8LL * dev_info().sms;
+  return launch(k_kv8_attend_join<T, HD, NQ>, dim3((unsigned)(ctas < most ? ctas : most)), dim3(kAttnJoinThreads), 0,
+                st, c, A);
+}
+
 template <typename T, int HD>
 static cudaError_t run_attend(const cats_kv8& c, const KvAttnArgs<T>& A, cudaStream_t st) {
-  cudaError_t e = launch(k_kv8_attend<T, HD>, dim3(A.ctas), dim3(kAttnThreads), attn_smem(HD), st, c, A);
-  if (e != cudaSuccess) return e;
-  const long long rows = ((long long)A.tokens * A.nh + kAttnWarps - 1) / kAttnWarps, most = 8LL * dev_info().sms;
-  return launch(k_kv8_attend_join<T, HD>, dim3((unsigned)(rows < most ? rows : most)), dim3(kAttnThreads), 0, st, c, A);
+  // rows of a key head: (new tokens) x (query heads per key head), on average over the sequences
+  const long long rows = ((long long)A.tokens + c.n_seqs - 1) / c.n_seqs * (A.nh / c.n_kv_heads);
+  return rows <= 8 ? run_attend<T, HD, 1>(c, A, st) : run_attend<T, HD, 2>(c, A, st);
 }
 
 template <typename T>

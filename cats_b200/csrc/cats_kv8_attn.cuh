@@ -3,11 +3,12 @@
 //   out[t, h] = sum_p softmax_p(scale q[t, h] . k[p]) v[p],   p = 0 .. position of t
 //
 // A decode step reads every code of the cache once and does two multiply-adds with each per query
-// head of the group: HBM is the bound as long as a code costs the SM few instructions.  So the query
-// heads that share a key head (times the new tokens of the sequence) are the 16 rows of a tensor-core
-// tile (mma.m16n8k16, half precision in, fp32 out), and codes become half precision, exactly, two per
-// instruction.  tcgen05 tiles have 128 rows, of which a decode step fills 1 to 16; with this shape the
-// codes go from shared memory to the tensor cores through registers, where they are converted anyway.
+// head of the group: HBM is the bound as long as a code costs the SM few instructions.  So codes
+// become half precision, exactly, two per instruction, and go to the tensor cores (mma.m16n8k16, fp32
+// accumulation) as the 16-row operand, of which nothing is padding: positions x channels for
+// S^T = K Q^T, channels x positions for O^T = V^T P^T.  The query heads that share a key head (times
+// the new tokens of the sequence) are the eight columns.  tcgen05 tiles have 128 rows and take their
+// operands from shared memory, where converted codes would first have to be written back.
 //
 // Precision: q is scaled by a power of two per row (largest magnitude just below 1) so that half
 // precision holds fp16 and bf16 queries exactly (but for elements 2^-14 below the row's largest);
@@ -17,8 +18,8 @@
 // p' = exp2(s + ev - m) with m the running maximum of s + ev, so that p' <= 1 whatever the scales,
 // and the softmax's sum is that of p' 2^-ev.
 //
-// Work: 128 positions (a unit, 16 for each of the 8 warps) of one row tile of one key head.  All
-// units of the call in a row - sequences, heads, tiles, positions - are dealt out to one CTA per SM in
+// Work: a unit is 16 positions for each warp of one tile (8 or 16 rows) of one key head.  All units
+// of the call in a row - sequences, heads, tiles, positions - are dealt out to one CTA per SM in
 // equal, contiguous shares, whatever the lengths of the sequences, and computed from the lengths on
 // the device; a (head, tile) that one CTA has whole is written at once, the parts of the others are
 // joined by a second kernel.
@@ -28,34 +29,49 @@
 
 namespace cats {
 
-constexpr int kAttnWarps = 8;
-constexpr int kAttnThreads = kAttnWarps * 32;
-constexpr int kAttnStages = 4;                          // tiles a warp has in flight (one of them in use)
 constexpr int kAttnTile = 16;                           // positions of a warp's tile
-constexpr int kAttnUnit = kAttnWarps * kAttnTile;       // positions of a unit
-constexpr int kAttnRows = 16;                           // rows of a tile: (token, query head of the group)
-constexpr int kAttnStageBytes = 2 * kAttnTile * 128 + 16;  // keys, values (rows 128 bytes apart), two scales
+constexpr int kAttnStageBytes = 2 * kAttnTile * 128 + 16;  // keys, values (rows 128 bytes apart), scales, rows
+constexpr int kAttnJoinThreads = 256;
+
+// NQ columns of eight rows ((token, query head of the group) pairs) per tile.  Eight rows leave room
+// for 16 warps of 128 registers, which hide the latency of the chain load - convert - multiply -
+// exponential - multiply best; 16 rows need twice the accumulators.
+template <int NQ>
+struct AttnShape {
+  static constexpr int kRows = 8 * NQ;
+  static constexpr int kWarps = NQ == 1 ? 16 : 8;
+  static constexpr int kThreads = 32 * kWarps;
+  static constexpr int kStages = NQ == 1 ? 3 : 6;       // tiles a warp has in its ring (one of them in use)
+  static constexpr int kUnit = kWarps * kAttnTile;      // positions of a unit
+};
 
 template <typename T>
 struct KvAttnArgs {
   const T* q;             // [tokens, nh, hd], tokens q_ld elements apart
   long long q_ld;
   T* out;                 // [tokens, nh, hd]
-  float* parts;           // [CTAs][2][kAttnRows][hd + 2] parts of (head, tile)s that several CTAs share
+  float* parts;           // [CTAs][2][rows of a tile][hd + 2] parts of (head, tile)s that several CTAs share
   const int* cu;
   int uniform, tokens, nh, layer, ctas;
   float scale;            // of the scores, times log2(e)
 };
 
-__host__ __device__ inline size_t attn_part_floats(int hd) { return (size_t)kAttnRows * (hd + 2); }
-__host__ __device__ inline size_t attn_smem(int hd) {
-  return (size_t)kAttnWarps * kAttnStages * kAttnStageBytes + sizeof(float) * kAttnWarps * kAttnRows * (hd + 4) +
-         sizeof(float) * 2 * kAttnWarps * kAttnRows;
+constexpr int kAttnMaxRows = 16;
+__host__ __device__ inline size_t attn_part_floats(int rows, int hd) { return (size_t)rows * (hd + 2); }
+template <int NQ>
+constexpr size_t attn_smem() {
+  return (size_t)AttnShape<NQ>::kWarps * (AttnShape<NQ>::kStages * kAttnStageBytes + 2 * 8 * sizeof(float));
 }
 
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// an 8 x 8 matrix of 16-bit values, two of a row per lane, transposed
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
 // c += a (16 x 16, row) * b (16 x 8, col)
@@ -80,12 +96,11 @@ __device__ __forceinline__ uint32_t attn_swizzle(int row, uint32_t byte) {
   return (uint32_t)row * 128 + (byte ^ ((((uint32_t)row & 3) ^ (((uint32_t)row >> 2) & 1)) << 5));
 }
 
-// Units of every sequence, summed up: pre[b] = units before sequence b, pre[n_seqs] = all.
-// Called by a CTA of kAttnThreads threads; ends with a barrier.
+// The share of every sequence.
 struct AttnSeq {
-  int len, count, first, tiles, units;                  // units of one tile of one head
+  int len, count, first, tiles, units;                  // tiles of a key head, units of a tile
 };
-template <typename T>
+template <int NQ, typename T>
 __device__ __forceinline__ AttnSeq attn_seq(const cats_kv8& c, const KvAttnArgs<T>& A, int b) {
   const KvSpan sp = kv_span(A.cu, A.uniform, b);
   const int len = c.lens[b];
@@ -93,14 +108,15 @@ __device__ __forceinline__ AttnSeq attn_seq(const cats_kv8& c, const KvAttnArgs<
   const bool fits = len >= 0 && len <= c.max_pages * c.page && sp.first >= 0 &&
                     (long long)sp.first + sp.count <= A.tokens;
   if (fits && sp.count > 0) {
-    s.tiles = (int)(((long long)sp.count * (A.nh / c.n_kv_heads) + kAttnRows - 1) / kAttnRows);
-    s.units = (len + kAttnUnit - 1) / kAttnUnit;
+    s.tiles = (int)(((long long)sp.count * (A.nh / c.n_kv_heads) + 8 * NQ - 1) / (8 * NQ));
+    s.units = (len + AttnShape<NQ>::kUnit - 1) / AttnShape<NQ>::kUnit;
   }
   return s;
 }
-template <typename T>
+// pre[b] = units before sequence b, pre[n_seqs] = all.  Called by all threads; ends with a barrier.
+template <int NQ, int THREADS, typename T>
 __device__ __forceinline__ void attn_prefix(const cats_kv8& c, const KvAttnArgs<T>& A, long long* pre, long long* s_warp) {
-  constexpr int kPer = kKvMaxSeqs / kAttnThreads;
+  constexpr int kPer = kKvMaxSeqs / THREADS;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   long long mine[kPer], sum = 0;
 #pragma unroll
@@ -108,7 +124,7 @@ __device__ __forceinline__ void attn_prefix(const cats_kv8& c, const KvAttnArgs<
     const int b = threadIdx.x * kPer + i;
     mine[i] = 0;
     if (b < c.n_seqs) {
-      const AttnSeq s = attn_seq(c, A, b);
+      const AttnSeq s = attn_seq<NQ>(c, A, b);
       mine[i] = (long long)s.units * s.tiles * c.n_kv_heads;
     }
     sum += mine[i];
@@ -129,15 +145,15 @@ __device__ __forceinline__ void attn_prefix(const cats_kv8& c, const KvAttnArgs<
     if (b <= c.n_seqs) pre[b] = before;
     before += mine[i];
   }
-  if (threadIdx.x == kAttnThreads - 1 && c.n_seqs == kKvMaxSeqs) pre[kKvMaxSeqs] = before;
+  if (threadIdx.x == THREADS - 1 && c.n_seqs == kKvMaxSeqs) pre[kKvMaxSeqs] = before;
   __syncthreads();
 }
 
 // Where a unit lies: sequence, head, tile and number of the unit within them.
 struct AttnPlace {
-  int b, head, tile, unit, units;
+  int b, head, tile, unit;
 };
-template <typename T>
+template <int NQ, typename T>
 __device__ __forceinline__ AttnPlace attn_place(const cats_kv8& c, const KvAttnArgs<T>& A, const long long* pre,
                                                 long long w, AttnSeq* seq) {
   int lo = 0, hi = c.n_seqs - 1;                         // last sequence that starts at or before w
@@ -146,7 +162,7 @@ __device__ __forceinline__ AttnPlace attn_place(const cats_kv8& c, const KvAttnA
     if (pre[mid] <= w) lo = mid;
     else hi = mid - 1;
   }
-  const AttnSeq s = attn_seq(c, A, lo);
+  const AttnSeq s = attn_seq<NQ>(c, A, lo);
   const unsigned r = (unsigned)(w - pre[lo]);            // below 2^32: checked at launch
   AttnPlace p;
   p.b = lo;
@@ -154,7 +170,6 @@ __device__ __forceinline__ AttnPlace attn_place(const cats_kv8& c, const KvAttnA
   p.unit = (int)(r - at * (unsigned)s.units);
   p.head = (int)(at / (unsigned)s.tiles);
   p.tile = (int)(at - (unsigned)p.head * (unsigned)s.tiles);
-  p.units = s.units;
   *seq = s;
   return p;
 }
@@ -166,33 +181,46 @@ __device__ __forceinline__ int attn_owner(long long total, long long w, int ctas
   return (int)(((w + 1) * ctas - 1) / total);
 }
 
-// O += P V for the warp's tile.  GUARD: some row must not see all of the tile's positions and V holds
-// a NaN; zero weights would turn it into NaN in rows that do not see it, so NaN codes are taken out
-// of the product and added to the rows that do see them (`seen`, weights 1 and 0).
-template <int HD, bool SPLIT, bool GUARD>
-__device__ __forceinline__ void attn_pv(float (*o)[4], const uint32_t* p, const uint32_t* p_lo, const uint32_t* seen,
-                                        const unsigned char* vt, int g, int t) {
-  auto group = [&](uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3, float (*acc)[4]) {
-    // four channels of four positions: byte pairs (position, next position) of each channel
+// O^T += V^T P^T for the warp's tile: the codes of V are the rows operand (channels x positions),
+// the weights the columns (positions x rows of the tile).
+// GUARD: some row must not see all of the tile's positions and V holds a NaN; zero weights would turn
+// it into NaN in rows that do not see it, so NaN codes are taken out of the product and added to the
+// rows that do see them (`seen`, weights 1 and 0).
+template <int HD, int NQ, bool SPLIT, bool GUARD>
+__device__ __forceinline__ void attn_pv(float (*o)[NQ][4], const uint32_t (*p)[2], const uint32_t (*p_lo)[2],
+                                        const uint32_t (*seen)[2], const unsigned char* vt, int g, int t) {
+  // r0 .. r3: four channels at the lane's four positions (2 t, 2 t + 1, 2 t + 8, 2 t + 9)
+  auto group = [&](uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3, float (*acc)[NQ][4]) {
+    // byte pairs (position, next position) of each channel
     const uint32_t w[4] = {__byte_perm(r0, r1, 0x5140), __byte_perm(r2, r3, 0x5140), __byte_perm(r0, r1, 0x7362),
                            __byte_perm(r2, r3, 0x7362)};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t c0 = (w[j & 2] >> (16 * (j & 1))) & 0xffffu, c1 = (w[(j & 2) + 1] >> (16 * (j & 1))) & 0xffffu;
+    for (int j = 0; j < 2; ++j) {                        // channels 2 j, 2 j + 1: rows g and g + 8 of a tile
+      uint32_t a[4] = {w[2 * j] & 0xffffu, w[2 * j] >> 16, w[2 * j + 1] & 0xffffu, w[2 * j + 1] >> 16};
       if (GUARD) {
-        auto nan_bytes = [](uint32_t x) { return ((((x & 0x7f7fu) + 0x0101u) & 0x8080u) >> 7) * 0xffu; };
-        const uint32_t n0 = nan_bytes(c0), n1 = nan_bytes(c1);
-        float hit[4] = {0.f, 0.f, 0.f, 0.f};
-        mma16816(hit, seen, e4m3_to_f16x2(n0 & 0x3838u), e4m3_to_f16x2(n1 & 0x3838u));   // 0x38 is 1.0
-        c0 &= ~n0;
-        c1 &= ~n1;
+        uint32_t ind[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (hit[i] > 0.f) acc[j][i] = __uint_as_float(0x7fc00000u);
+        for (int x = 0; x < 4; ++x) {
+          const uint32_t n = ((((a[x] & 0x7f7fu) + 0x0101u) & 0x8080u) >> 7) * 0xffu;   // 0xff where NaN
+          a[x] &= ~n;
+          ind[x] = e4m3_to_f16x2(n & 0x3838u);                                          // 0x38 is 1.0
+        }
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+          float hit[4] = {0.f, 0.f, 0.f, 0.f};
+          mma16816(hit, ind, seen[n][0], seen[n][1]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (hit[i] > 0.f) acc[j][n][i] = __uint_as_float(0x7fc00000u);
+        }
       }
-      const uint32_t b0 = e4m3_to_f16x2(c0), b1 = e4m3_to_f16x2(c1);
-      mma16816(acc[j], p, b0, b1);
-      if (SPLIT) mma16816(acc[j], p_lo, b0, b1);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) a[x] = e4m3_to_f16x2(a[x]);
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        mma16816(acc[j][n], a, p[n][0], p[n][1]);
+        if (SPLIT) mma16816(acc[j][n], a, p_lo[n][0], p_lo[n][1]);
+      }
     }
   };
   const int r[4] = {2 * t, 2 * t + 1, 8 + 2 * t, 9 + 2 * t};
@@ -201,53 +229,52 @@ __device__ __forceinline__ void attn_pv(float (*o)[4], const uint32_t* p, const 
     uint2 v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint2*>(vt + attn_swizzle(r[i], 64 * q + 8 * g));
-    group(v[0].x, v[1].x, v[2].x, v[3].x, o + 8 * q);
-    group(v[0].y, v[1].y, v[2].y, v[3].y, o + 8 * q + 4);
+    group(v[0].x, v[1].x, v[2].x, v[3].x, o + 4 * q);
+    group(v[0].y, v[1].y, v[2].y, v[3].y, o + 4 * q + 2);
   }
   if (HD % 64) {
     uint32_t v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint32_t*>(vt + attn_swizzle(r[i], HD / 64 * 64 + 4 * g));
-    group(v[0], v[1], v[2], v[3], o + 8 * (HD / 64));
+    group(v[0], v[1], v[2], v[3], o + 4 * (HD / 64));
   }
 }
 
-template <typename T, int HD>
-__global__ void __launch_bounds__(kAttnThreads, 1) k_kv8_attend(const cats_kv8 c, const KvAttnArgs<T> A) {
+template <typename T, int HD, int NQ>
+__global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const cats_kv8 c, const KvAttnArgs<T> A) {
+  using S = AttnShape<NQ>;
   constexpr bool SPLIT = sizeof(T) == 4;
   constexpr int KS = HD / 16;                            // k-steps of the score product
-  constexpr int NT = HD / 8;                             // column tiles of the output
+  constexpr int MT = HD / 16;                            // row tiles of O^T
+  constexpr int kMeta = 2 * kAttnTile * 128;             // scales and rows behind a stage's codes
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ long long s_pre[kKvMaxSeqs + 1];
-  __shared__ long long s_warp[kAttnWarps];
+  __shared__ long long s_warp[S::kWarps];
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  unsigned char* ring = smem + (size_t)warp * kAttnStages * kAttnStageBytes;
-  float* s_o = reinterpret_cast<float*>(smem + (size_t)kAttnWarps * kAttnStages * kAttnStageBytes);
-  float* s_ml = s_o + kAttnWarps * kAttnRows * (HD + 4);
+  unsigned char* ring = smem + (size_t)warp * S::kStages * kAttnStageBytes;
+  float* s_ml = reinterpret_cast<float*>(smem + (size_t)S::kWarps * S::kStages * kAttnStageBytes);
   const uint32_t ring_u32 = (uint32_t)__cvta_generic_to_shared(ring);
 
-  attn_prefix(c, A, s_pre, s_warp);
+  attn_prefix<NQ, S::kThreads>(c, A, s_pre, s_warp);
   const long long total = s_pre[c.n_seqs];
   const int ctas = attn_ctas(total, A.ctas);
   if ((int)blockIdx.x >= ctas) return;
-  const long long w0 = attn_share(total, blockIdx.x, ctas), w1 = attn_share(total, blockIdx.x + 1, ctas);
+  const long long share0 = attn_share(total, blockIdx.x, ctas);
+  const int n_units = (int)(attn_share(total, blockIdx.x + 1, ctas) - share0);   // (checked at launch)
   const int group = A.nh / c.n_kv_heads;
 
   // ---- loader: lane i of the warp knows where unit `base + i` lies and which page its tile is in --
-  long long base = w0;
-  int d_id = -1, d_row = 0, d_rows = 0, d_head = 0;      // page, row in it, rows to load, head
-  auto look = [&]() {
-    const long long w = base + lane;
-    d_id = -1;
+  int d_id = 0, d_row = 0, d_rows = 0, d_head = 0;       // page, row in it, rows to load, head
+  auto look = [&](int base) {
     d_rows = 0;
-    if (w < w1) {
+    if (base + lane < n_units) {
       AttnSeq s;
-      const AttnPlace p = attn_place(c, A, s_pre, w, &s);
-      const int last = min(s.count - 1, (p.tile * kAttnRows + kAttnRows - 1) / group);
+      const AttnPlace p = attn_place<NQ>(c, A, s_pre, share0 + base + lane, &s);
+      const int last = min(s.count - 1, (p.tile * S::kRows + S::kRows - 1) / group);
       const int end = min(s.len, s.len - s.count + last + 1);        // positions that the tile's rows see
-      const int kb = p.unit * kAttnUnit + warp * kAttnTile;
+      const int kb = p.unit * S::kUnit + warp * kAttnTile;
       d_head = p.head;
       d_row = kb % c.page;
       d_rows = min(max(end - kb, 0), kAttnTile);
@@ -260,195 +287,210 @@ __global__ void __launch_bounds__(kAttnThreads, 1) k_kv8_attend(const cats_kv8 c
       }
     }
   };
-  look();
-  int stage_in = 0;
-  long long w_in = w0;
+  // 16-byte chunk `lane + 32 i` of the tile's keys (i < HD / 32), then of its values
+  constexpr int kChunks = HD / 16;                       // of a row
+  auto chunk_to = [&](int i) { return attn_swizzle((lane + 32 * i) / kChunks, (lane + 32 * i) % kChunks * 16); };
+  int stage_in = 0, n_in = 0;
   auto issue = [&]() {
-    if (w_in < w1) {
-      if (w_in - base == 32) {
-        base += 32;
-        look();
-      }
-      const int src = (int)(w_in - base);
+    if (n_in < n_units) {
+      if ((n_in & 31) == 0) look(n_in);
+      const int src = n_in & 31;
       const int rows = __shfl_sync(0xffffffffu, d_rows, src);
       const uint32_t st = ring_u32 + stage_in * kAttnStageBytes;
-      if (lane == 0)
-        *reinterpret_cast<int*>(ring + stage_in * kAttnStageBytes + 2 * kAttnTile * 128 + 8) = rows;
+      if (lane == 0) *reinterpret_cast<int*>(ring + stage_in * kAttnStageBytes + kMeta + 8) = rows;
       if (rows > 0) {
         const int id = __shfl_sync(0xffffffffu, d_id, src), row = __shfl_sync(0xffffffffu, d_row, src);
         const int head = __shfl_sync(0xffffffffu, d_head, src);
+        const size_t block = kv_block(c);
         const uint8_t* kp = kv_rows(c, A.layer, id, 0, head) + (size_t)row * HD;
-        const uint8_t* vp = kp + (size_t)c.n_kv_heads * kv_block(c);
-#pragma unroll
-        for (int i = 0; i < 2 * HD / 32; ++i) {          // 16-byte chunks: the keys', then the values'
-          const int n = lane + 32 * i;
-          const int kv = n / HD, m = n - kv * HD, r = m / (HD / 16), ch = m - r * (HD / 16);
-          const uint8_t* from = (kv ? vp : kp) + (size_t)m * 16;
-          const uint32_t to = st + kv * kAttnTile * 128 + attn_swizzle(r, ch * 16);
-          const int bytes = r < rows ? 16 : 0;           // the rest is filled with zeros, not read
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(r < rows ? from : kp), "r"(bytes)
-                       : "memory");
-        }
+        const uint8_t* vp = kp + (size_t)c.n_kv_heads * block;
         if (lane < 2)
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(st + 2 * kAttnTile * 128 + 4 * lane),
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(st + kMeta + 4 * lane),
                        "l"(kv_scale(c, A.layer, id, lane, head))
                        : "memory");
+        kp += lane * 16;
+        vp += lane * 16;
+        if (rows == kAttnTile) {
+#pragma unroll
+          for (int i = 0; i < HD / 32; ++i) {
+            const uint32_t to = st + chunk_to(i);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(kp + 512 * i) : "memory");
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + kAttnTile * 128), "l"(vp + 512 * i)
+                         : "memory");
+          }
+        } else {                                         // the last rows of a sequence: the others become zeros
+#pragma unroll
+          for (int i = 0; i < HD / 32; ++i) {
+            const uint32_t to = st + chunk_to(i);
+            const bool in = (lane + 32 * i) / kChunks < rows;
+            const int bytes = in ? 16 : 0, off = in ? 512 * i : -16 * lane;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(kp + off), "r"(bytes) : "memory");
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + kAttnTile * 128), "l"(vp + off),
+                         "r"(bytes)
+                         : "memory");
+          }
+        }
       }
-      ++w_in;
-      stage_in = stage_in + 1 == kAttnStages ? 0 : stage_in + 1;
+      ++n_in;
+      stage_in = stage_in + 1 == S::kStages ? 0 : stage_in + 1;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  for (int i = 0; i < kAttnStages - 1; ++i) issue();
+  for (int i = 0; i < S::kStages - 1; ++i) issue();
 
-  // ---- consumer ------------------------------------------------------------------------------------
-  uint32_t qa[KS][4], qb[SPLIT ? KS : 1][4];
-  float o[NT][4];
-  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, f0 = 0.f, f1 = 0.f;
-  int lim0 = 0, lim1 = 0, lim_min = 0;
+  // ---- consumer: S^T = K Q^T, so a lane has rows (columns) 2 t and 2 t + 1 of each group of eight ----
+  uint32_t qa[KS][NQ][2], qb[SPLIT ? KS : 1][NQ][2];
+  float o[MT][NQ][4];
+  float m[NQ][2], l[NQ][2], f[NQ][2];
+  int lim[NQ][2], lim_min = 0;                           // positions that a row sees, and the least of them
   AttnSeq seq;
-  AttnPlace at = attn_place(c, A, s_pre, w0, &seq);
+  AttnPlace at = attn_place<NQ>(c, A, s_pre, share0, &seq);
   bool first_seg = true, begins_here = at.unit == 0, fresh = true;
   int stage = 0;
-  for (long long w = w0; w < w1; ++w) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(kAttnStages - 2) : "memory");
+  for (int u = 0; u < n_units; ++u) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
     __syncwarp();
     issue();
 
     if (fresh) {                                         // a new (sequence, head, tile): its queries
       fresh = false;
-      const int rows = min(kAttnRows, seq.count * group - at.tile * kAttnRows);
-      float q[2][HD / 32][8];
-      float top[2] = {0.f, 0.f};
+      const int rows = min(S::kRows, seq.count * group - at.tile * S::kRows);
+      lim_min = min(seq.len, seq.len - seq.count + at.tile * S::kRows / group + 1);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = at.tile * kAttnRows + g + 8 * i, tok = r / group, hq = at.head * group + r - tok * group;
-        const bool on = g + 8 * i < rows;
+      for (int n = 0; n < NQ; ++n) {
+        const int r = at.tile * S::kRows + 8 * n + g, tok = r / group, hq = at.head * group + r - tok * group;
+        const bool on = 8 * n + g < rows;
         const T* src = A.q + (size_t)(seq.first + tok) * A.q_ld + (size_t)hq * HD + 8 * t;
+        float q[HD / 32][8], top = 0.f;
 #pragma unroll
         for (int p = 0; p < HD / 32; ++p) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) q[i][p][k] = 0.f;
-          if (on) load8_cached(src + 32 * p, q[i][p]);
+          for (int k = 0; k < 8; ++k) q[p][k] = 0.f;
+          if (on) load8_cached(src + 32 * p, q[p]);
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            const float a = fabsf(q[i][p][k]);
-            if (a <= 3.402823466e38f) top[i] = fmaxf(top[i], a);
+            const float a = fabsf(q[p][k]);
+            if (a <= 3.402823466e38f) top = fmaxf(top, a);
           }
         }
-        const int lim = on ? min(seq.len, seq.len - seq.count + tok + 1) : 0;
-        if (i) lim1 = lim;
-        else lim0 = lim;
-      }
-      lim_min = min(seq.len, seq.len - seq.count + at.tile * kAttnRows / group + 1);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = top > 0.f ? min(max(kv_exp_of(top) + 1, -126), 126) : 0;
+        const float inv = kv_pow2(-e), back = kv_pow2(e) * A.scale;
+        const int sees = on ? min(seq.len, seq.len - seq.count + tok + 1) : 0;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
-        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
-        const int e = top[i] > 0.f ? min(max(kv_exp_of(top[i]) + 1, -126), 126) : 0;
-        const float inv = kv_pow2(-e), f = kv_pow2(e) * A.scale;
-        if (i) f1 = f;
-        else f0 = f;
+        for (int x = 0; x < 2; ++x) {
+          f[n][x] = __shfl_sync(0xffffffffu, back, 4 * (2 * t + x));
+          lim[n][x] = __shfl_sync(0xffffffffu, sees, 4 * (2 * t + x));
+          m[n][x] = -INFINITY;
+          l[n][x] = 0.f;
+        }
 #pragma unroll
         for (int p = 0; p < HD / 32; ++p)
 #pragma unroll
-          for (int k = 0; k < 8; ++k) q[i][p][k] *= inv;
+          for (int k = 0; k < 8; ++k) q[p][k] *= inv;
+#pragma unroll
+        for (int p = 0; p < HD / 32; ++p)
+#pragma unroll
+          for (int e2 = 0; e2 < 2; ++e2)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const float* v = q[p] + 4 * e2 + 2 * x;
+              qa[2 * p + e2][n][x] = half2_bits(v[0], v[1]);
+              if (SPLIT) qb[SPLIT ? 2 * p + e2 : 0][n][x] = half2_rest(v[0], v[1], qa[2 * p + e2][n][x]);
+            }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) o[i][n][x] = 0.f;
       }
-#pragma unroll
-      for (int p = 0; p < HD / 32; ++p)
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const float* f = q[x & 1][p] + 4 * e + (x & 2);
-            qa[2 * p + e][x] = half2_bits(f[0], f[1]);
-            if (SPLIT) qb[SPLIT ? 2 * p + e : 0][x] = half2_rest(f[0], f[1], qa[2 * p + e][x]);
-          }
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[n][i] = 0.f;
-      m0 = m1 = -INFINITY;
-      l0 = l1 = 0.f;
     }
 
-    const int kb = at.unit * kAttnUnit + warp * kAttnTile;
-    const unsigned char* kt = ring + stage * kAttnStageBytes;
-    if (*reinterpret_cast<const int*>(kt + 2 * kAttnTile * 128 + 8) > 0) {
+    const int kb = at.unit * S::kUnit + warp * kAttnTile;
+    unsigned char* kt = ring + stage * kAttnStageBytes;
+    if (*reinterpret_cast<const int*>(kt + kMeta + 8) > 0) {
       const unsigned char* vt = kt + kAttnTile * 128;
-      const float2 sc = *reinterpret_cast<const float2*>(kt + 2 * kAttnTile * 128);
-      float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      const float2 sc = *reinterpret_cast<const float2*>(kt + kMeta);
+      float s[NQ][4];
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
 #pragma unroll
       for (int p = 0; p < HD / 32; ++p) {
+        const uint2 k0 = *reinterpret_cast<const uint2*>(kt + attn_swizzle(g, 32 * p + 8 * t));
+        const uint2 k1 = *reinterpret_cast<const uint2*>(kt + attn_swizzle(8 + g, 32 * p + 8 * t));
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const uint2 k = *reinterpret_cast<const uint2*>(kt + attn_swizzle(8 * n + g, 32 * p + 8 * t));
-          const uint32_t b0 = e4m3_to_f16x2(k.x & 0xffffu), b1 = e4m3_to_f16x2(k.x >> 16);
-          const uint32_t b2 = e4m3_to_f16x2(k.y & 0xffffu), b3 = e4m3_to_f16x2(k.y >> 16);
-          mma16816(s[n], qa[2 * p], b0, b1);
-          mma16816(s[n], qa[2 * p + 1], b2, b3);
-          if (SPLIT) {
-            mma16816(s[n], qb[SPLIT ? 2 * p : 0], b0, b1);
-            mma16816(s[n], qb[SPLIT ? 2 * p + 1 : 0], b2, b3);
+        for (int e2 = 0; e2 < 2; ++e2) {
+          const uint32_t x0 = e2 ? k0.y : k0.x, x1 = e2 ? k1.y : k1.x;
+          const uint32_t a[4] = {e4m3_to_f16x2(x0 & 0xffffu), e4m3_to_f16x2(x1 & 0xffffu), e4m3_to_f16x2(x0 >> 16),
+                                 e4m3_to_f16x2(x1 >> 16)};
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) {
+            mma16816(s[n], a, qa[2 * p + e2][n][0], qa[2 * p + e2][n][1]);
+            if (SPLIT) mma16816(s[n], a, qb[SPLIT ? 2 * p + e2 : 0][n][0], qb[SPLIT ? 2 * p + e2 : 0][n][1]);
           }
         }
       }
       const int ev = kv_exp_of(sc.y);
-      const float evf = (float)ev;
+      const float evf = (float)ev, vi = kv_pow2(-ev);
       const bool cut = kb + kAttnTile > lim_min;         // some row does not see all of the tile
+      uint32_t p[NQ][2], pl[NQ][2];
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < NQ; ++n) {
+        float top[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[n][i] *= sc.x * (i < 2 ? f0 : f1);
-          if (cut && kb + 8 * n + 2 * t + (i & 1) >= (i < 2 ? lim0 : lim1)) s[n][i] = -INFINITY;
+        for (int x = 0; x < 2; ++x) {                    // s[x], s[2 + x]: positions g, g + 8 of row 2 t + x
+          const float by = sc.x * f[n][x];
+          s[n][x] *= by;
+          s[n][2 + x] *= by;
+          if (cut) {
+            if (kb + g >= lim[n][x]) s[n][x] = -INFINITY;
+            if (kb + 8 + g >= lim[n][x]) s[n][2 + x] = -INFINITY;
+          }
+          top[x] = fmaxf(s[n][x], s[n][2 + x]);
         }
-      float n0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
-      float n1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
-      n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 1));
-      n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 1));
-      n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 2));
-      n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 2));
-      n0 += evf;
-      n1 += evf;
-      if (__any_sync(0xffffffffu, n0 > m0 || n1 > m1)) {
-        n0 = fmaxf(n0, m0);
-        n1 = fmaxf(n1, m1);
-        const float x0 = m0 == -INFINITY ? 0.f : ex2(m0 - n0), x1 = m1 == -INFINITY ? 0.f : ex2(m1 - n1);
-        m0 = n0;
-        m1 = n1;
-        l0 *= x0;
-        l1 *= x1;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          o[n][0] *= x0;
-          o[n][1] *= x0;
-          o[n][2] *= x1;
-          o[n][3] *= x1;
+        for (int w = 4; w < 32; w <<= 1) {
+          top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], w));
+          top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], w));
         }
-      }
-      // (m - ev) is the same for all tiles whose pages have the same ev: its rounding cancels
-      const float u0 = m0 == -INFINITY ? 0.f : m0 - evf, u1 = m1 == -INFINITY ? 0.f : m1 - evf;
+        top[0] += evf;
+        top[1] += evf;
+        if (__any_sync(0xffffffffu, top[0] > m[n][0] || top[1] > m[n][1])) {
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+          for (int x = 0; x < 2; ++x) {
+            const float to = fmaxf(top[x], m[n][x]), by = m[n][x] == -INFINITY ? 0.f : ex2(m[n][x] - to);
+            m[n][x] = to;
+            l[n][x] *= by;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[n][i] = ex2(s[n][i] - (i < 2 ? u0 : u1));
-      const float vi = kv_pow2(-ev);
-      l0 = fmaf((s[0][0] + s[0][1]) + (s[1][0] + s[1][1]), vi, l0);
-      l1 = fmaf((s[0][2] + s[0][3]) + (s[1][2] + s[1][3]), vi, l1);
-      uint32_t p[4], pl[4];
+            for (int i = 0; i < MT; ++i) {
+              o[i][n][x] *= by;
+              o[i][n][2 + x] *= by;
+            }
+          }
+        }
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const float* f = s[x >> 1] + 2 * (x & 1);
-        p[x] = half2_bits(f[0], f[1]);
-        pl[x] = SPLIT ? half2_rest(f[0], f[1], p[x]) : 0u;
+        for (int x = 0; x < 2; ++x) {
+          // (m - ev) is the same for all tiles whose pages have the same ev: its rounding cancels
+          const float ref = m[n][x] == -INFINITY ? 0.f : m[n][x] - evf;
+          s[n][x] = ex2(s[n][x] - ref);
+          s[n][2 + x] = ex2(s[n][2 + x] - ref);
+          l[n][x] = fmaf(s[n][x] + s[n][2 + x], vi, l[n][x]);
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {                    // positions 0 .. 7, 8 .. 15
+          const uint32_t h = half2_bits(s[n][2 * x], s[n][2 * x + 1]);
+          p[n][x] = transpose8x8(h);
+          pl[n][x] = SPLIT ? transpose8x8(half2_rest(s[n][2 * x], s[n][2 * x + 1], h)) : 0u;
+        }
       }
       bool guard = false;
       if (cut) {
         bool nan = false;
 #pragma unroll
         for (int i = 0; i < HD / 32; ++i) {
-          const uint4 v = *reinterpret_cast<const uint4*>(vt + attn_swizzle((lane + 32 * i) / (HD / 16), (lane + 32 * i) % (HD / 16) * 16));
+          const uint4 v = *reinterpret_cast<const uint4*>(vt + chunk_to(i));
           const uint32_t x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) nan |= (((x[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
@@ -456,101 +498,102 @@ __global__ void __launch_bounds__(kAttnThreads, 1) k_kv8_attend(const cats_kv8 c
         guard = __any_sync(0xffffffffu, nan);
       }
       if (guard) {
-        uint32_t seen[4];
+        uint32_t seen[NQ][2];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int k = kb + 8 * (x >> 1) + 2 * t, lim = (x & 1) ? lim1 : lim0;
-          seen[x] = half2_bits(k < lim ? 1.f : 0.f, k + 1 < lim ? 1.f : 0.f);
+        for (int n = 0; n < NQ; ++n) {                   // lane: row g, positions 2 t, 2 t + 1 (+ 8)
+          const int a = __shfl_sync(0xffffffffu, lim[n][0], g >> 1), b = __shfl_sync(0xffffffffu, lim[n][1], g >> 1);
+          const int mine = (g & 1) ? b : a;
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int k = kb + 8 * x + 2 * t;
+            seen[n][x] = half2_bits(k < mine ? 1.f : 0.f, k + 1 < mine ? 1.f : 0.f);
+          }
         }
-        attn_pv<HD, SPLIT, true>(o, p, pl, seen, vt, g, t);
+        attn_pv<HD, NQ, SPLIT, true>(o, p, pl, seen, vt, g, t);
       } else {
-        attn_pv<HD, SPLIT, false>(o, p, pl, nullptr, vt, g, t);
+        attn_pv<HD, NQ, SPLIT, false>(o, p, pl, nullptr, vt, g, t);
       }
     }
-    stage = stage + 1 == kAttnStages ? 0 : stage + 1;
+    stage = stage + 1 == S::kStages ? 0 : stage + 1;
     ++at.unit;
 
-    if (at.unit == at.units || w + 1 == w1) {            // the segment ends here: join the warps
-      const int rows = min(kAttnRows, seq.count * group - at.tile * kAttnRows);
-      l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-      l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+    if (at.unit == seq.units || u + 1 == n_units) {      // the segment ends here: join the warps
+      const int rows = min(S::kRows, seq.count * group - at.tile * S::kRows);
+      const bool whole = begins_here && at.unit == seq.units;
+      float* part = A.parts + (size_t)(blockIdx.x * 2 + (first_seg ? 0 : 1)) * attn_part_floats(S::kRows, HD);
+      // eight rows at a time, in the codes' bytes of the stage that this tile was in (free until the
+      // next call of issue): [8][HD] floats of each warp
+      const size_t pitch = (size_t)S::kStages * kAttnStageBytes;
+      __syncwarp();
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = g + 8 * i;
-        if (r >= rows) continue;
-        float* dst = s_o + (size_t)(warp * kAttnRows + r) * (HD + 4);
-        if (t == 0) {
-          s_ml[warp * kAttnRows + r] = i ? m1 : m0;
-          s_ml[kAttnWarps * kAttnRows + warp * kAttnRows + r] = i ? l1 : l0;
+      for (int n = 0; n < NQ; ++n) {
+        if (8 * n >= rows) break;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+#pragma unroll
+          for (int w = 4; w < 32; w <<= 1) l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], w);
+          if (g == 0) {
+            s_ml[(warp * 2 + 0) * 8 + 2 * t + x] = m[n][x];
+            s_ml[(warp * 2 + 1) * 8 + 2 * t + x] = l[n][x];
+          }
+          if (8 * n + 2 * t + x < rows) {
+            // row tile 4 q + i holds channels 64 q + 8 g + 2 i and the next; the rest 4 g + 2 i
+            float* dst = reinterpret_cast<float*>(kt) + (2 * t + x) * HD;
+#pragma unroll
+            for (int i = 0; i < MT; i += 2) {
+              const int d = i < 4 * (HD / 64) ? 64 * (i / 4) + 8 * g + 2 * (i % 4) : HD / 64 * 64 + 4 * g;
+              *reinterpret_cast<float4*>(dst + d) = make_float4(o[i][n][x], o[i][n][2 + x], o[i + 1][n][x], o[i + 1][n][2 + x]);
+            }
+          }
         }
-        // column tile 8 q + j holds channels 64 q + 8 n + j (n = 2 t, 2 t + 1), the rest 4 n + j
+        __syncthreads();
+        const int here = min(8, rows - 8 * n);
+        for (int e = threadIdx.x; e < here * (HD / 4); e += S::kThreads) {
+          const int r = e / (HD / 4), d = (e - r * (HD / 4)) * 4;
+          const float* src = reinterpret_cast<const float*>(smem + (kt - ring)) + r * HD + d;
+          float top = -INFINITY, sum = 0.f;
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int q = 0; q < HD / 64; ++q)
+          for (int x = 0; x < S::kWarps; ++x) top = fmaxf(top, s_ml[x * 16 + r]);
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int k = 0; k < 8; k += 4)
-              *reinterpret_cast<float4*>(dst + 64 * q + 16 * t + 8 * x + k) =
-                  make_float4(o[8 * q + k][2 * i + x], o[8 * q + k + 1][2 * i + x], o[8 * q + k + 2][2 * i + x],
-                              o[8 * q + k + 3][2 * i + x]);
-        if (HD % 64) {
-          constexpr int n = 8 * (HD / 64);
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-            *reinterpret_cast<float4*>(dst + HD / 64 * 64 + 8 * t + 4 * x) =
-                make_float4(o[n][2 * i + x], o[n + 1][2 * i + x], o[n + 2][2 * i + x], o[n + 3][2 * i + x]);
+          for (int x = 0; x < S::kWarps; ++x) {
+            const float mx = s_ml[x * 16 + r], lx = s_ml[x * 16 + 8 + r];
+            if (mx == -INFINITY && lx == 0.f) continue;  // saw nothing (a NaN sum goes on)
+            const float by = ex2(mx - (top == -INFINITY ? 0.f : top));
+            const float4 w = *reinterpret_cast<const float4*>(src + x * (pitch / sizeof(float)));
+            sum = fmaf(lx, by, sum);
+            v.x = fmaf(w.x, by, v.x);
+            v.y = fmaf(w.y, by, v.y);
+            v.z = fmaf(w.z, by, v.z);
+            v.w = fmaf(w.w, by, v.w);
+          }
+          if (whole) {
+            const int rr = at.tile * S::kRows + 8 * n + r, tok = rr / group, hq = at.head * group + rr - tok * group;
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            T* dst = A.out + ((size_t)(seq.first + tok) * A.nh + hq) * HD + d;
+            dst[0] = VecT<T>::from_f(v.x * inv);
+            dst[1] = VecT<T>::from_f(v.y * inv);
+            dst[2] = VecT<T>::from_f(v.z * inv);
+            dst[3] = VecT<T>::from_f(v.w * inv);
+          } else {
+            float* dst = part + (size_t)(8 * n + r) * (HD + 2);
+            *reinterpret_cast<float2*>(dst + d) = make_float2(v.x, v.y);
+            *reinterpret_cast<float2*>(dst + d + 2) = make_float2(v.z, v.w);
+            if (d == 0) *reinterpret_cast<float2*>(dst + HD) = make_float2(top, sum);
+          }
         }
+        __syncthreads();
       }
-      __syncthreads();
-      const bool whole = begins_here && at.unit == at.units;
-      float* part = A.parts + (size_t)(blockIdx.x * 2 + (first_seg ? 0 : 1)) * attn_part_floats(HD);
-      for (int e = threadIdx.x; e < rows * (HD / 4); e += kAttnThreads) {
-        const int r = e / (HD / 4), d = (e - r * (HD / 4)) * 4;
-        float top = -INFINITY, sum = 0.f;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int x = 0; x < kAttnWarps; ++x) top = fmaxf(top, s_ml[x * kAttnRows + r]);
-#pragma unroll
-        for (int x = 0; x < kAttnWarps; ++x) {
-          const float mx = s_ml[x * kAttnRows + r];
-          const float lx = s_ml[(kAttnWarps + x) * kAttnRows + r];
-          if (mx == -INFINITY && lx == 0.f) continue;    // saw nothing (a NaN sum goes on)
-          const float f = ex2(mx - (top == -INFINITY ? 0.f : top));
-          const float4 u = *reinterpret_cast<const float4*>(s_o + (size_t)(x * kAttnRows + r) * (HD + 4) + d);
-          sum = fmaf(lx, f, sum);
-          v.x = fmaf(u.x, f, v.x);
-          v.y = fmaf(u.y, f, v.y);
-          v.z = fmaf(u.z, f, v.z);
-          v.w = fmaf(u.w, f, v.w);
-        }
-        if (whole) {
-          const int rr = at.tile * kAttnRows + r, tok = rr / group, hq = at.head * group + rr - tok * group;
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          T* dst = A.out + ((size_t)(seq.first + tok) * A.nh + hq) * HD + d;
-          dst[0] = VecT<T>::from_f(v.x * inv);
-          dst[1] = VecT<T>::from_f(v.y * inv);
-          dst[2] = VecT<T>::from_f(v.z * inv);
-          dst[3] = VecT<T>::from_f(v.w * inv);
-        } else {
-          float* dst = part + (size_t)r * (HD + 2);
-          *reinterpret_cast<float2*>(dst + d) = make_float2(v.x, v.y);
-          *reinterpret_cast<float2*>(dst + d + 2) = make_float2(v.z, v.w);
-          if (d == 0) *reinterpret_cast<float2*>(dst + HD) = make_float2(top, sum);
-        }
-      }
-      __syncthreads();
       first_seg = false;
       fresh = true;
-      if (w + 1 < w1) at = attn_place(c, A, s_pre, w + 1, &seq);
       begins_here = true;
+      if (u + 1 < n_units) at = attn_place<NQ>(c, A, s_pre, share0 + u + 1, &seq);
     }
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-template <typename T, int HD>
+template <typename T, int HD, int NQ>
 __device__ __forceinline__ void attn_join_row(const cats_kv8& c, const KvAttnArgs<T>& A, const long long* s_pre,
                                               long long row, int lane) {
   const int tok = (int)(row / A.nh), hq = (int)(row - (long long)tok * A.nh), group = A.nh / c.n_kv_heads;
@@ -566,7 +609,7 @@ __device__ __forceinline__ void attn_join_row(const cats_kv8& c, const KvAttnArg
     }
     b = lo;
   }
-  const AttnSeq s = attn_seq(c, A, b);
+  const AttnSeq s = attn_seq<NQ>(c, A, b);
   const int i = tok - s.first;
   if (i < 0 || i >= s.count) return;                     // a row that belongs to no sequence
   T* dst = A.out + (size_t)row * HD;
@@ -576,7 +619,7 @@ __device__ __forceinline__ void attn_join_row(const cats_kv8& c, const KvAttnArg
     for (int d = lane; d < HD; d += 32) dst[d] = VecT<T>::from_f(0.f);
     return;
   }
-  const int head = hq / group, at = i * group + hq - head * group, tile = at / kAttnRows, r = at - tile * kAttnRows;
+  const int head = hq / group, at = i * group + hq - head * group, tile = at / (8 * NQ), r = at - tile * 8 * NQ;
   const long long total = s_pre[c.n_seqs];
   const long long u0 = s_pre[b] + ((long long)head * s.tiles + tile) * s.units, u1 = u0 + s.units - 1;
   const int ctas = attn_ctas(total, A.ctas), c0 = attn_owner(total, u0, ctas), c1 = attn_owner(total, u1, ctas);
@@ -584,7 +627,7 @@ __device__ __forceinline__ void attn_join_row(const cats_kv8& c, const KvAttnArg
   float top = -INFINITY;
   auto part = [&](int x) {
     const int slot = attn_share(total, x, ctas) >= u0 ? 0 : 1;
-    return A.parts + (size_t)(2 * x + slot) * attn_part_floats(HD) + (size_t)r * (HD + 2);
+    return A.parts + (size_t)(2 * x + slot) * attn_part_floats(8 * NQ, HD) + (size_t)r * (HD + 2);
   };
   for (int x = c0 + lane; x <= c1; x += 32) top = fmaxf(top, part(x)[HD]);
 #pragma unroll
@@ -609,16 +652,16 @@ __device__ __forceinline__ void attn_join_row(const cats_kv8& c, const KvAttnArg
 
 // Joins the parts of the (head, tile)s that several CTAs share: one warp per (token, query head).
 // Rows without any position become zeros here.
-template <typename T, int HD>
-__global__ void __launch_bounds__(kAttnThreads) k_kv8_attend_join(const cats_kv8 c, const KvAttnArgs<T> A) {
+template <typename T, int HD, int NQ>
+__global__ void __launch_bounds__(kAttnJoinThreads) k_kv8_attend_join(const cats_kv8 c, const KvAttnArgs<T> A) {
   __shared__ long long s_pre[kKvMaxSeqs + 1];
-  __shared__ long long s_warp[kAttnWarps];
+  __shared__ long long s_warp[kAttnJoinThreads / 32];
   pdl_wait();
-  attn_prefix(c, A, s_pre, s_warp);
+  attn_prefix<NQ, kAttnJoinThreads>(c, A, s_pre, s_warp);
   const int lane = threadIdx.x & 31;
-  const long long rows = (long long)A.tokens * A.nh, step = (long long)gridDim.x * kAttnWarps;
-  for (long long row = (long long)blockIdx.x * kAttnWarps + (threadIdx.x >> 5); row < rows; row += step)
-    attn_join_row<T, HD>(c, A, s_pre, row, lane);
+  const long long rows = (long long)A.tokens * A.nh, step = (long long)gridDim.x * (kAttnJoinThreads / 32);
+  for (long long row = (long long)blockIdx.x * (kAttnJoinThreads / 32) + (threadIdx.x >> 5); row < rows; row += step)
+    attn_join_row<T, HD, NQ>(c, A, s_pre, row, lane);
 }
 
 }  // namespace cats
