@@ -8,12 +8,7 @@ namespace cats {
 template <typename T, int HD, int NQ>
 static cudaError_t run_attend(const cats_kv8& c, const KvAttnArgs<T>& A, cudaStream_t st) {
   using S = AttnShape<NQ>;
-  cudaError_t e = launch(k_kv8_attend<T, HD, NQ>, dim3(A.ctas), dim3(S::kThreads), attn_smem<NQ>(), st, c, A);
-  if (e != cudaSuccess) return e;
-  constexpr int per = kAttnJoinThreads / 32;
-  const long long ctas = ((long long)A.tokens * A.nh + per - 1) / per, most = 8LL * dev_info().sms;
-  return launch(k_kv8_attend_join<T, HD, NQ>, dim3((unsigned)(ctas < most ? ctas : most)), dim3(kAttnJoinThreads), 0,
-                st, c, A);
+  return launch(k_kv8_attend<T, HD, NQ>, dim3(A.ctas), dim3(S::kThreads), attn_smem<NQ>(), st, c, A);
 }
 
 template <typename T, int HD>

@@ -22,7 +22,7 @@
 // of the call in a row - sequences, heads, tiles, positions - are dealt out to one CTA per SM in
 // equal, contiguous shares, whatever the lengths of the sequences, and computed from the lengths on
 // the device; a (head, tile) that one CTA has whole is written at once, the parts of the others are
-// joined by a second kernel.
+// joined by the CTA that finishes last (nobody waits).
 #pragma once
 
 #include "cats_kv8.cuh"
@@ -30,8 +30,8 @@
 namespace cats {
 
 constexpr int kAttnTile = 16;                           // positions of a warp's tile
-constexpr int kAttnStageBytes = 2 * kAttnTile * 128 + 16;  // keys, values (rows 128 bytes apart), scales, rows
-constexpr int kAttnJoinThreads = 256;
+constexpr int kAttnStageBytes = 2 * kAttnTile * 128;    // keys, values (rows 128 bytes apart)
+constexpr float kAttnSlack = 8.f;                       // see the running maximum
 
 // NQ columns of eight rows ((token, query head of the group) pairs) per tile.  Eight rows leave room
 // for 16 warps of 128 registers, which hide the latency of the chain load - convert - multiply -
@@ -51,6 +51,7 @@ struct KvAttnArgs {
   long long q_ld;
   T* out;                 // [tokens, nh, hd]
   float* parts;           // [CTAs][2][rows of a tile][hd + 2] parts of (head, tile)s that several CTAs share
+  int* counters;          // [CTAs], zero between calls
   const int* cu;
   int uniform, tokens, nh, layer, ctas;
   float scale;            // of the scores, times log2(e)
@@ -60,7 +61,7 @@ constexpr int kAttnMaxRows = 16;
 __host__ __device__ inline size_t attn_part_floats(int rows, int hd) { return (size_t)rows * (hd + 2); }
 template <int NQ>
 constexpr size_t attn_smem() {
-  return (size_t)AttnShape<NQ>::kWarps * (AttnShape<NQ>::kStages * kAttnStageBytes + 2 * 8 * sizeof(float));
+  return 128 + (size_t)AttnShape<NQ>::kWarps * (AttnShape<NQ>::kStages * (kAttnStageBytes + 16) + 2 * 8 * sizeof(float));
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -96,89 +97,117 @@ __device__ __forceinline__ uint32_t attn_swizzle(int row, uint32_t byte) {
   return (uint32_t)row * 128 + (byte ^ ((((uint32_t)row & 3) ^ (((uint32_t)row >> 2) & 1)) << 5));
 }
 
-// The share of every sequence.
+// What the CTA knows of the sequences (shared memory).
+struct AttnTable {
+  int pre[kKvMaxSeqs + 1];                              // units before sequence b; all of them
+  int len[kKvMaxSeqs], first[kKvMaxSeqs], count[kKvMaxSeqs];
+};
 struct AttnSeq {
   int len, count, first, tiles, units;                  // tiles of a key head, units of a tile
 };
-template <int NQ, typename T>
-__device__ __forceinline__ AttnSeq attn_seq(const cats_kv8& c, const KvAttnArgs<T>& A, int b) {
-  const KvSpan sp = kv_span(A.cu, A.uniform, b);
-  const int len = c.lens[b];
-  AttnSeq s = {len, sp.count, sp.first, 0, 0};
-  const bool fits = len >= 0 && len <= c.max_pages * c.page && sp.first >= 0 &&
-                    (long long)sp.first + sp.count <= A.tokens;
-  if (fits && sp.count > 0) {
-    s.tiles = (int)(((long long)sp.count * (A.nh / c.n_kv_heads) + 8 * NQ - 1) / (8 * NQ));
-    s.units = (len + AttnShape<NQ>::kUnit - 1) / AttnShape<NQ>::kUnit;
-  }
+template <int NQ>
+__device__ __forceinline__ AttnSeq attn_seq(const AttnTable& tab, int b, int group) {
+  AttnSeq s = {tab.len[b], tab.count[b], tab.first[b], 0, 0};
+  s.tiles = (int)(((long long)s.count * group + 8 * NQ - 1) / (8 * NQ));
+  s.units = (s.len + AttnShape<NQ>::kUnit - 1) / AttnShape<NQ>::kUnit;
   return s;
 }
-// pre[b] = units before sequence b, pre[n_seqs] = all.  Called by all threads; ends with a barrier.
-template <int NQ, int THREADS, typename T>
-__device__ __forceinline__ void attn_prefix(const cats_kv8& c, const KvAttnArgs<T>& A, long long* pre, long long* s_warp) {
-  constexpr int kPer = kKvMaxSeqs / THREADS;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long mine[kPer], sum = 0;
+// Fills the table (called by all threads; ends with a barrier) and zeroes the rows of the sequences
+// that hold nothing.  A sequence whose length or span does not fit counts as one of those.
+template <int NQ, int HD, typename T>
+__device__ __forceinline__ void attn_table(const cats_kv8& c, const KvAttnArgs<T>& A, AttnTable& tab, int* s_warp) {
+  constexpr int kThreads = AttnShape<NQ>::kThreads, kPer = kKvMaxSeqs / kThreads;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = A.nh / c.n_kv_heads;
+  int mine[kPer], sum = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int b = threadIdx.x * kPer + i;
     mine[i] = 0;
     if (b < c.n_seqs) {
-      const AttnSeq s = attn_seq<NQ>(c, A, b);
-      mine[i] = (long long)s.units * s.tiles * c.n_kv_heads;
+      const KvSpan sp = kv_span(A.cu, A.uniform, b);
+      int len = c.lens[b], first = sp.first, count = sp.count;
+      const bool long_ok = len >= 0 && len <= c.max_pages * c.page;
+      const bool span_ok = first >= 0 && (long long)first + count <= A.tokens;
+      if (count > 0 && !(long_ok && span_ok)) {
+        if (blockIdx.x == 0) kv_flag(c, long_ok ? KV_BAD_SPAN : KV_TOO_LONG);
+        len = 0;
+        const long long end = min((long long)first + count, (long long)A.tokens);
+        first = max(first, 0);
+        count = (int)max(end - first, 0LL);
+      }
+      tab.len[b] = len;
+      tab.first[b] = first;
+      tab.count[b] = count;
+      const AttnSeq s = attn_seq<NQ>(tab, b, group);
+      mine[i] = s.units * s.tiles * c.n_kv_heads;
     }
     sum += mine[i];
   }
-  long long incl = sum;
+  int incl = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+    const int v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
   if (lane == 31) s_warp[warp] = incl;
   __syncthreads();
-  long long before = incl - sum;
+  int before = incl - sum;
   for (int w = 0; w < warp; ++w) before += s_warp[w];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int b = threadIdx.x * kPer + i;
-    if (b <= c.n_seqs) pre[b] = before;
+    if (b <= c.n_seqs) tab.pre[b] = before;
     before += mine[i];
   }
-  if (threadIdx.x == THREADS - 1 && c.n_seqs == kKvMaxSeqs) pre[kKvMaxSeqs] = before;
+  if (threadIdx.x == kThreads - 1 && c.n_seqs == kKvMaxSeqs) tab.pre[kKvMaxSeqs] = before;
   __syncthreads();
+  for (int b = blockIdx.x; b < c.n_seqs; b += gridDim.x) {
+    if (tab.pre[b + 1] != tab.pre[b] || tab.count[b] == 0) continue;
+    T* dst = A.out + (size_t)tab.first[b] * A.nh * HD;
+    const size_t n = (size_t)tab.count[b] * A.nh * HD;
+    for (size_t k = threadIdx.x; k < n; k += kThreads) dst[k] = VecT<T>::from_f(0.f);
+  }
 }
 
 // Where a unit lies: sequence, head, tile and number of the unit within them.
 struct AttnPlace {
   int b, head, tile, unit;
 };
-template <int NQ, typename T>
-__device__ __forceinline__ AttnPlace attn_place(const cats_kv8& c, const KvAttnArgs<T>& A, const long long* pre,
-                                                long long w, AttnSeq* seq) {
-  int lo = 0, hi = c.n_seqs - 1;                         // last sequence that starts at or before w
+template <int NQ>
+__device__ __forceinline__ AttnPlace attn_place(const AttnTable& tab, int n_seqs, int group, int w, AttnSeq* seq) {
+  int lo = 0, hi = n_seqs - 1;                           // last sequence that starts at or before w
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (pre[mid] <= w) lo = mid;
+    if (tab.pre[mid] <= w) lo = mid;
     else hi = mid - 1;
   }
-  const AttnSeq s = attn_seq<NQ>(c, A, lo);
-  const unsigned r = (unsigned)(w - pre[lo]);            // below 2^32: checked at launch
+  const AttnSeq s = attn_seq<NQ>(tab, lo, group);
+  const int r = w - tab.pre[lo];
   AttnPlace p;
   p.b = lo;
-  const unsigned at = r / (unsigned)s.units;
-  p.unit = (int)(r - at * (unsigned)s.units);
-  p.head = (int)(at / (unsigned)s.tiles);
-  p.tile = (int)(at - (unsigned)p.head * (unsigned)s.tiles);
+  const int at = r / s.units;
+  p.unit = r - at * s.units;
+  p.head = at / s.tiles;
+  p.tile = at - p.head * s.tiles;
   *seq = s;
   return p;
 }
 // CTAs that get a share (at least one unit each), and where the share of CTA c begins
-__device__ __forceinline__ int attn_ctas(long long total, int ctas) { return total < ctas ? (int)total : ctas; }
-__device__ __forceinline__ long long attn_share(long long total, int c, int ctas) { return total * c / ctas; }
+__device__ __forceinline__ int attn_ctas(int total, int ctas) { return min(total, ctas); }
+__device__ __forceinline__ int attn_share(int total, int c, int ctas) { return (int)((long long)total * c / ctas); }
 // the CTA whose share holds unit w
-__device__ __forceinline__ int attn_owner(long long total, long long w, int ctas) {
-  return (int)(((w + 1) * ctas - 1) / total);
+__device__ __forceinline__ int attn_owner(int total, int w, int ctas) {
+  return (int)((((long long)w + 1) * ctas - 1) / total);
+}
+__device__ __forceinline__ uint2 lds2(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds1(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
 }
 
 // O^T += V^T P^T for the warp's tile: the codes of V are the rows operand (channels x positions),
@@ -188,7 +217,8 @@ __device__ __forceinline__ int attn_owner(long long total, long long w, int ctas
 // rows that do see them (`seen`, weights 1 and 0).
 template <int HD, int NQ, bool SPLIT, bool GUARD>
 __device__ __forceinline__ void attn_pv(float (*o)[NQ][4], const uint32_t (*p)[2], const uint32_t (*p_lo)[2],
-                                        const uint32_t (*seen)[2], const unsigned char* vt, int g, int t) {
+                                        const uint32_t (*seen)[2], uint32_t v0, uint32_t v1, uint32_t v2,
+                                        uint32_t v3) {
   // r0 .. r3: four channels at the lane's four positions (2 t, 2 t + 1, 2 t + 8, 2 t + 9)
   auto group = [&](uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3, float (*acc)[NQ][4]) {
     // byte pairs (position, next position) of each channel
@@ -223,21 +253,44 @@ __device__ __forceinline__ void attn_pv(float (*o)[NQ][4], const uint32_t (*p)[2
       }
     }
   };
-  const int r[4] = {2 * t, 2 * t + 1, 8 + 2 * t, 9 + 2 * t};
+  // v0, v1: rows 2 t and 2 t + 1 at byte 8 g; rows 8 further on have the same exchange of chunks
 #pragma unroll
   for (int q = 0; q < HD / 64; ++q) {
-    uint2 v[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint2*>(vt + attn_swizzle(r[i], 64 * q + 8 * g));
-    group(v[0].x, v[1].x, v[2].x, v[3].x, o + 4 * q);
-    group(v[0].y, v[1].y, v[2].y, v[3].y, o + 4 * q + 2);
+    const uint2 r0 = lds2(v0 ^ (64 * q)), r1 = lds2(v1 ^ (64 * q));
+    const uint2 r2 = lds2((v0 ^ (64 * q)) + 1024), r3 = lds2((v1 ^ (64 * q)) + 1024);
+    group(r0.x, r1.x, r2.x, r3.x, o + 4 * q);
+    group(r0.y, r1.y, r2.y, r3.y, o + 4 * q + 2);
   }
-  if (HD % 64) {
-    uint32_t v[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint32_t*>(vt + attn_swizzle(r[i], HD / 64 * 64 + 4 * g));
-    group(v[0], v[1], v[2], v[3], o + 4 * (HD / 64));
+  if (HD % 64) {                                         // 32 channels left: byte 4 g
+    constexpr int q = HD / 64;
+    group(lds1(v2), lds1(v3), lds1(v2 + 1024), lds1(v3 + 1024), o + 4 * q);
   }
+}
+
+// (top, sum, v) += a part with reference m, sum l and products w.  A part that saw nothing is left
+// out (a NaN sum is not: it stays NaN).
+__device__ __forceinline__ void attn_add(float m, float l, float4 w, float& top, float& sum, float4& v) {
+  if (m == -INFINITY && l == 0.f) return;
+  const float to = fmaxf(top, m), ref = to == -INFINITY ? 0.f : to;
+  const float x = ex2(m - ref), y = top == -INFINITY && sum == 0.f ? 0.f : ex2(top - ref);
+  top = to;
+  sum = fmaf(l, x, sum * y);
+  v.x = fmaf(w.x, x, v.x * y);
+  v.y = fmaf(w.y, x, v.y * y);
+  v.z = fmaf(w.z, x, v.z * y);
+  v.w = fmaf(w.w, x, v.w * y);
+}
+// four channels of row r of the tile at `at`
+template <typename T>
+__device__ __forceinline__ void attn_store(const KvAttnArgs<T>& A, const AttnSeq& seq, const AttnPlace& at, int group,
+                                           int tile_rows, int r, int d, int hd, float sum, float4 v) {
+  const int rr = at.tile * tile_rows + r, tok = rr / group, hq = at.head * group + rr - tok * group;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;        // no position seen: zeros
+  __align__(16) T w[4] = {VecT<T>::from_f(v.x * inv), VecT<T>::from_f(v.y * inv), VecT<T>::from_f(v.z * inv),
+                          VecT<T>::from_f(v.w * inv)};
+  T* dst = A.out + ((size_t)(seq.first + tok) * A.nh + hq) * hd + d;
+  if (sizeof(T) == 4) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(w);
+  else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(w);
 }
 
 template <typename T, int HD, int NQ>
@@ -246,70 +299,81 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
   constexpr bool SPLIT = sizeof(T) == 4;
   constexpr int KS = HD / 16;                            // k-steps of the score product
   constexpr int MT = HD / 16;                            // row tiles of O^T
-  constexpr int kMeta = 2 * kAttnTile * 128;             // scales and rows behind a stage's codes
-  extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ long long s_pre[kKvMaxSeqs + 1];
-  __shared__ long long s_warp[S::kWarps];
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  // (aligned by hand: the exchange of chunks is applied to whole addresses)
+  unsigned char* smem = smem_raw + ((128 - ((uint32_t)__cvta_generic_to_shared(smem_raw) & 127)) & 127);
+  __shared__ AttnTable s_tab;
+  __shared__ int s_warp[S::kWarps];
+  __shared__ int s_last;
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   unsigned char* ring = smem + (size_t)warp * S::kStages * kAttnStageBytes;
-  float* s_ml = reinterpret_cast<float*>(smem + (size_t)S::kWarps * S::kStages * kAttnStageBytes);
+  unsigned char* after = smem + (size_t)S::kWarps * S::kStages * kAttnStageBytes;
+  float4* meta = reinterpret_cast<float4*>(after) + warp * S::kStages;   // scales of keys and values, rows
+  float* s_ml = reinterpret_cast<float*>(after + (size_t)S::kWarps * S::kStages * 16);
   const uint32_t ring_u32 = (uint32_t)__cvta_generic_to_shared(ring);
+  const uint32_t meta_u32 = (uint32_t)__cvta_generic_to_shared(meta);
 
-  attn_prefix<NQ, S::kThreads>(c, A, s_pre, s_warp);
-  const long long total = s_pre[c.n_seqs];
-  const int ctas = attn_ctas(total, A.ctas);
+  attn_table<NQ, HD>(c, A, s_tab, s_warp);
+  const int total = s_tab.pre[c.n_seqs], ctas = attn_ctas(total, A.ctas);
   if ((int)blockIdx.x >= ctas) return;
-  const long long share0 = attn_share(total, blockIdx.x, ctas);
-  const int n_units = (int)(attn_share(total, blockIdx.x + 1, ctas) - share0);   // (checked at launch)
+  const int share0 = attn_share(total, blockIdx.x, ctas);
+  const int n_units = attn_share(total, blockIdx.x + 1, ctas) - share0;
   const int group = A.nh / c.n_kv_heads;
 
   // ---- loader: lane i of the warp knows where unit `base + i` lies and which page its tile is in --
-  int d_id = 0, d_row = 0, d_rows = 0, d_head = 0;       // page, row in it, rows to load, head
+  int d_rows = 0, d_scale = 0;                           // rows to load; the keys' scale in its layer
+  long long d_off = 0;                                   // the keys' first byte in the layer
+  const uint8_t* layer_codes = kv_rows(c, A.layer, 0, 0, 0);
+  const float* layer_scales = kv_scale(c, A.layer, 0, 0, 0);
   auto look = [&](int base) {
     d_rows = 0;
     if (base + lane < n_units) {
       AttnSeq s;
-      const AttnPlace p = attn_place<NQ>(c, A, s_pre, share0 + base + lane, &s);
+      const AttnPlace p = attn_place<NQ>(s_tab, c.n_seqs, group, share0 + base + lane, &s);
       const int last = min(s.count - 1, (p.tile * S::kRows + S::kRows - 1) / group);
       const int end = min(s.len, s.len - s.count + last + 1);        // positions that the tile's rows see
       const int kb = p.unit * S::kUnit + warp * kAttnTile;
-      d_head = p.head;
-      d_row = kb % c.page;
       d_rows = min(max(end - kb, 0), kAttnTile);
       if (d_rows > 0) {
-        d_id = c.table[(size_t)p.b * c.max_pages + kb / c.page];
-        if (d_id < 0 || d_id >= c.n_pages) {
+        const int id = c.table[(size_t)p.b * c.max_pages + kb / c.page];
+        if (id < 0 || id >= c.n_pages) {
           kv_flag(c, KV_BAD_PAGE);
           d_rows = 0;
+        } else {
+          d_off = ((long long)id * 2 * c.n_kv_heads + p.head) * (c.page * HD) + (kb % c.page) * HD;
+          d_scale = id * 2 * c.n_kv_heads + p.head;
         }
       }
     }
   };
-  // 16-byte chunk `lane + 32 i` of the tile's keys (i < HD / 32), then of its values
+  // 16-byte chunk `lane + 32 i` of the tile's keys (i < HD / 32) and of its values goes to byte
+  // (to0 ^ flip) + step: the exchange of chunks depends on a row's three low bits
   constexpr int kChunks = HD / 16;                       // of a row
-  auto chunk_to = [&](int i) { return attn_swizzle((lane + 32 * i) / kChunks, (lane + 32 * i) % kChunks * 16); };
+  const uint32_t to0 = ring_u32 + attn_swizzle(lane / kChunks, lane % kChunks * 16);
+  auto chunk_to = [&](int i) -> uint32_t {
+    if (HD == 128) return (to0 ^ ((i & 1) * 32)) + 512 * i;          // four rows further on
+    if (HD == 64) return to0 + 1024 * i;                              // eight rows
+    return ring_u32 + attn_swizzle((lane + 32 * i) / kChunks, (lane + 32 * i) % kChunks * 16);
+  };
+  const long long v_off = (long long)c.n_kv_heads * c.page * HD;
   int stage_in = 0, n_in = 0;
   auto issue = [&]() {
     if (n_in < n_units) {
       if ((n_in & 31) == 0) look(n_in);
       const int src = n_in & 31;
       const int rows = __shfl_sync(0xffffffffu, d_rows, src);
-      const uint32_t st = ring_u32 + stage_in * kAttnStageBytes;
-      if (lane == 0) *reinterpret_cast<int*>(ring + stage_in * kAttnStageBytes + kMeta + 8) = rows;
+      const uint32_t st = stage_in * kAttnStageBytes;
+      if (lane == 0) reinterpret_cast<int*>(meta + stage_in)[2] = rows;
       if (rows > 0) {
-        const int id = __shfl_sync(0xffffffffu, d_id, src), row = __shfl_sync(0xffffffffu, d_row, src);
-        const int head = __shfl_sync(0xffffffffu, d_head, src);
-        const size_t block = kv_block(c);
-        const uint8_t* kp = kv_rows(c, A.layer, id, 0, head) + (size_t)row * HD;
-        const uint8_t* vp = kp + (size_t)c.n_kv_heads * block;
+        const uint8_t* kp = layer_codes + __shfl_sync(0xffffffffu, d_off, src) + lane * 16;
+        const uint8_t* vp = kp + v_off;
+        const int sc = __shfl_sync(0xffffffffu, d_scale, src);
         if (lane < 2)
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(st + kMeta + 4 * lane),
-                       "l"(kv_scale(c, A.layer, id, lane, head))
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(meta_u32 + 16 * stage_in + 4 * lane),
+                       "l"(layer_scales + sc + lane * c.n_kv_heads)
                        : "memory");
-        kp += lane * 16;
-        vp += lane * 16;
         if (rows == kAttnTile) {
 #pragma unroll
           for (int i = 0; i < HD / 32; ++i) {
@@ -338,13 +402,20 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
   };
   for (int i = 0; i < S::kStages - 1; ++i) issue();
 
+  // the lane's reads of a tile (offsets in a stage): keys at rows g and g + 8, byte 8 t; values at
+  // rows 2 t, 2 t + 1 (and 8 further on), byte 8 g, and byte 4 g of the last 32 channels of 32 and 96
+  const uint32_t k_off = attn_swizzle(g, 8 * t);
+  const uint32_t v0_off = kAttnTile * 128 + attn_swizzle(2 * t, 8 * g), v1_off = kAttnTile * 128 + attn_swizzle(2 * t + 1, 8 * g);
+  const uint32_t v2_off = HD % 64 ? kAttnTile * 128 + attn_swizzle(2 * t, HD / 64 * 64 + 4 * g) : 0;
+  const uint32_t v3_off = HD % 64 ? kAttnTile * 128 + attn_swizzle(2 * t + 1, HD / 64 * 64 + 4 * g) : 0;
+
   // ---- consumer: S^T = K Q^T, so a lane has rows (columns) 2 t and 2 t + 1 of each group of eight ----
   uint32_t qa[KS][NQ][2], qb[SPLIT ? KS : 1][NQ][2];
   float o[MT][NQ][4];
   float m[NQ][2], l[NQ][2], f[NQ][2];
   int lim[NQ][2], lim_min = 0;                           // positions that a row sees, and the least of them
   AttnSeq seq;
-  AttnPlace at = attn_place<NQ>(c, A, s_pre, share0, &seq);
+  AttnPlace at = attn_place<NQ>(s_tab, c.n_seqs, group, share0, &seq);
   bool first_seg = true, begins_here = at.unit == 0, fresh = true;
   int stage = 0;
   for (int u = 0; u < n_units; ++u) {
@@ -408,9 +479,9 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
 
     const int kb = at.unit * S::kUnit + warp * kAttnTile;
     unsigned char* kt = ring + stage * kAttnStageBytes;
-    if (*reinterpret_cast<const int*>(kt + kMeta + 8) > 0) {
-      const unsigned char* vt = kt + kAttnTile * 128;
-      const float2 sc = *reinterpret_cast<const float2*>(kt + kMeta);
+    const float4 sc = meta[stage];
+    if (__float_as_int(sc.z) > 0) {
+      const uint32_t st = ring_u32 + stage * kAttnStageBytes;
       float s[NQ][4];
 #pragma unroll
       for (int n = 0; n < NQ; ++n)
@@ -418,8 +489,8 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
         for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
 #pragma unroll
       for (int p = 0; p < HD / 32; ++p) {
-        const uint2 k0 = *reinterpret_cast<const uint2*>(kt + attn_swizzle(g, 32 * p + 8 * t));
-        const uint2 k1 = *reinterpret_cast<const uint2*>(kt + attn_swizzle(8 + g, 32 * p + 8 * t));
+        const uint32_t ka = (st + k_off) ^ (32 * p);
+        const uint2 k0 = lds2(ka), k1 = lds2(ka + 1024);
 #pragma unroll
         for (int e2 = 0; e2 < 2; ++e2) {
           const uint32_t x0 = e2 ? k0.y : k0.x, x1 = e2 ? k1.y : k1.x;
@@ -457,7 +528,10 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
         }
         top[0] += evf;
         top[1] += evf;
-        if (__any_sync(0xffffffffu, top[0] > m[n][0] || top[1] > m[n][1])) {
+        // The reference m of the weights follows the running maximum only when that is more than
+        // 2^kAttnSlack ahead: weights up to 256 do half precision no harm, and the accumulators are
+        // rescaled a few times per sequence instead of at every second tile.
+        if (__any_sync(0xffffffffu, top[0] > m[n][0] + kAttnSlack || top[1] > m[n][1] + kAttnSlack)) {
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             const float to = fmaxf(top[x], m[n][x]), by = m[n][x] == -INFINITY ? 0.f : ex2(m[n][x] - to);
@@ -490,7 +564,7 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
         bool nan = false;
 #pragma unroll
         for (int i = 0; i < HD / 32; ++i) {
-          const uint4 v = *reinterpret_cast<const uint4*>(vt + chunk_to(i));
+          const uint4 v = *reinterpret_cast<const uint4*>(ring + stage * kAttnStageBytes + kAttnTile * 128 + (chunk_to(i) - ring_u32));
           const uint32_t x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) nan |= (((x[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
@@ -509,9 +583,9 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
             seen[n][x] = half2_bits(k < mine ? 1.f : 0.f, k + 1 < mine ? 1.f : 0.f);
           }
         }
-        attn_pv<HD, NQ, SPLIT, true>(o, p, pl, seen, vt, g, t);
+        attn_pv<HD, NQ, SPLIT, true>(o, p, pl, seen, st + v0_off, st + v1_off, st + v2_off, st + v3_off);
       } else {
-        attn_pv<HD, NQ, SPLIT, false>(o, p, pl, nullptr, vt, g, t);
+        attn_pv<HD, NQ, SPLIT, false>(o, p, pl, nullptr, st + v0_off, st + v1_off, st + v2_off, st + v3_off);
       }
     }
     stage = stage + 1 == S::kStages ? 0 : stage + 1;
@@ -555,26 +629,13 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
           float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
           for (int x = 0; x < S::kWarps; ++x) top = fmaxf(top, s_ml[x * 16 + r]);
-#pragma unroll
+#pragma unroll 4
           for (int x = 0; x < S::kWarps; ++x) {
-            const float mx = s_ml[x * 16 + r], lx = s_ml[x * 16 + 8 + r];
-            if (mx == -INFINITY && lx == 0.f) continue;  // saw nothing (a NaN sum goes on)
-            const float by = ex2(mx - (top == -INFINITY ? 0.f : top));
-            const float4 w = *reinterpret_cast<const float4*>(src + x * (pitch / sizeof(float)));
-            sum = fmaf(lx, by, sum);
-            v.x = fmaf(w.x, by, v.x);
-            v.y = fmaf(w.y, by, v.y);
-            v.z = fmaf(w.z, by, v.z);
-            v.w = fmaf(w.w, by, v.w);
+            attn_add(s_ml[x * 16 + r], s_ml[x * 16 + 8 + r],
+                     *reinterpret_cast<const float4*>(src + x * (pitch / sizeof(float))), top, sum, v);
           }
           if (whole) {
-            const int rr = at.tile * S::kRows + 8 * n + r, tok = rr / group, hq = at.head * group + rr - tok * group;
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            T* dst = A.out + ((size_t)(seq.first + tok) * A.nh + hq) * HD + d;
-            dst[0] = VecT<T>::from_f(v.x * inv);
-            dst[1] = VecT<T>::from_f(v.y * inv);
-            dst[2] = VecT<T>::from_f(v.z * inv);
-            dst[3] = VecT<T>::from_f(v.w * inv);
+            attn_store(A, seq, at, group, S::kRows, 8 * n + r, d, HD, sum, v);
           } else {
             float* dst = part + (size_t)(8 * n + r) * (HD + 2);
             *reinterpret_cast<float2*>(dst + d) = make_float2(v.x, v.y);
@@ -584,84 +645,67 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
         }
         __syncthreads();
       }
+      if (!whole) {
+        // The CTA that brings the last part of a (head, tile) joins them all, in the order of the
+        // CTAs.  The counter belongs to the CTA that has the first part (at most one of its
+        // segments goes on in the next CTA) and is left at zero.
+        const int u0 = share0 + u + 1 - at.unit, c0 = attn_owner(total, u0, ctas), c1 = attn_owner(total, u0 + seq.units - 1, ctas);
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) s_last = atomicAdd(A.counters + c0, 1) == c1 - c0;
+        __syncthreads();
+        if (s_last) {
+          if (threadIdx.x == 0) A.counters[c0] = 0;
+          __threadfence();
+          // `sets` threads share a (row, four channels), each takes every sets-th part
+          const int items = rows * (HD / 4), sets = max(1, min(S::kThreads / items, c1 - c0 + 1));
+          float* s_set = reinterpret_cast<float*>(kt - ring + smem);       // [warps] x a stage: six floats a thread
+          for (int e0 = 0; e0 < items; e0 += S::kThreads) {
+            const int e = sets > 1 ? threadIdx.x % items : e0 + threadIdx.x, set = sets > 1 ? threadIdx.x / items : 0;
+            float top = -INFINITY, sum = 0.f;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (e < items && set < sets) {
+              const int r = e / (HD / 4), d = (e - r * (HD / 4)) * 4;
+#pragma unroll 4
+              for (int x = c0 + set; x <= c1; x += sets) {
+                const int slot = attn_share(total, x, ctas) >= u0 ? 0 : 1;
+                const float* src = A.parts + (size_t)(2 * x + slot) * attn_part_floats(S::kRows, HD) + (size_t)r * (HD + 2);
+                const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + HD));
+                const float2 a = __ldcg(reinterpret_cast<const float2*>(src + d)), b = __ldcg(reinterpret_cast<const float2*>(src + d + 2));
+                attn_add(ml.x, ml.y, make_float4(a.x, a.y, b.x, b.y), top, sum, v);
+              }
+            }
+            if (sets > 1) {
+              float* mine = s_set + (threadIdx.x >> 5) * (S::kStages * kAttnStageBytes / 4) + (threadIdx.x & 31) * 6;
+              mine[0] = top;
+              mine[1] = sum;
+              mine[2] = v.x;
+              mine[3] = v.y;
+              mine[4] = v.z;
+              mine[5] = v.w;
+              __syncthreads();
+              if (set == 0)
+                for (int k = 1; k < sets; ++k) {
+                  const int other = threadIdx.x + k * items;
+                  const float* p = s_set + (other >> 5) * (S::kStages * kAttnStageBytes / 4) + (other & 31) * 6;
+                  attn_add(p[0], p[1], make_float4(p[2], p[3], p[4], p[5]), top, sum, v);
+                }
+            }
+            if (e < items && set == 0) {
+              const int r = e / (HD / 4), d = (e - r * (HD / 4)) * 4;
+              attn_store(A, seq, at, group, S::kRows, r, d, HD, sum, v);
+            }
+          }
+          __syncthreads();
+        }
+      }
       first_seg = false;
       fresh = true;
       begins_here = true;
-      if (u + 1 < n_units) at = attn_place<NQ>(c, A, s_pre, share0 + u + 1, &seq);
+      if (u + 1 < n_units) at = attn_place<NQ>(s_tab, c.n_seqs, group, share0 + u + 1, &seq);
     }
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
-}
-
-template <typename T, int HD, int NQ>
-__device__ __forceinline__ void attn_join_row(const cats_kv8& c, const KvAttnArgs<T>& A, const long long* s_pre,
-                                              long long row, int lane) {
-  const int tok = (int)(row / A.nh), hq = (int)(row - (long long)tok * A.nh), group = A.nh / c.n_kv_heads;
-  int b;
-  if (!A.cu) {
-    b = tok / A.uniform;
-  } else {
-    int lo = 0, hi = c.n_seqs - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (__ldg(A.cu + mid) <= tok) lo = mid;
-      else hi = mid - 1;
-    }
-    b = lo;
-  }
-  const AttnSeq s = attn_seq<NQ>(c, A, b);
-  const int i = tok - s.first;
-  if (i < 0 || i >= s.count) return;                     // a row that belongs to no sequence
-  T* dst = A.out + (size_t)row * HD;
-  if (s.units == 0 || s.tiles == 0) {
-    if (lane == 0 && i == 0 && (s.len < 0 || s.len > c.max_pages * c.page)) kv_flag(c, KV_TOO_LONG);
-    if (lane == 0 && i == 0 && (s.first < 0 || (long long)s.first + s.count > A.tokens)) kv_flag(c, KV_BAD_SPAN);
-    for (int d = lane; d < HD; d += 32) dst[d] = VecT<T>::from_f(0.f);
-    return;
-  }
-  const int head = hq / group, at = i * group + hq - head * group, tile = at / (8 * NQ), r = at - tile * 8 * NQ;
-  const long long total = s_pre[c.n_seqs];
-  const long long u0 = s_pre[b] + ((long long)head * s.tiles + tile) * s.units, u1 = u0 + s.units - 1;
-  const int ctas = attn_ctas(total, A.ctas), c0 = attn_owner(total, u0, ctas), c1 = attn_owner(total, u1, ctas);
-  if (c0 == c1) return;                                  // written already
-  float top = -INFINITY;
-  auto part = [&](int x) {
-    const int slot = attn_share(total, x, ctas) >= u0 ? 0 : 1;
-    return A.parts + (size_t)(2 * x + slot) * attn_part_floats(8 * NQ, HD) + (size_t)r * (HD + 2);
-  };
-  for (int x = c0 + lane; x <= c1; x += 32) top = fmaxf(top, part(x)[HD]);
-#pragma unroll
-  for (int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-  const float ref = top == -INFINITY ? 0.f : top;
-  float sum = 0.f, v[HD / 32];
-#pragma unroll
-  for (int k = 0; k < HD / 32; ++k) v[k] = 0.f;
-  for (int x = c0; x <= c1; ++x) {
-    const float* p = part(x);
-    const float m = p[HD], l = p[HD + 1];
-    if (m == -INFINITY && l == 0.f) continue;
-    const float f = ex2(m - ref);
-    sum = fmaf(l, f, sum);
-#pragma unroll
-    for (int k = 0; k < HD / 32; ++k) v[k] = fmaf(p[lane + 32 * k], f, v[k]);
-  }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-  for (int k = 0; k < HD / 32; ++k) dst[lane + 32 * k] = VecT<T>::from_f(v[k] * inv);
-}
-
-// Joins the parts of the (head, tile)s that several CTAs share: one warp per (token, query head).
-// Rows without any position become zeros here.
-template <typename T, int HD, int NQ>
-__global__ void __launch_bounds__(kAttnJoinThreads) k_kv8_attend_join(const cats_kv8 c, const KvAttnArgs<T> A) {
-  __shared__ long long s_pre[kKvMaxSeqs + 1];
-  __shared__ long long s_warp[kAttnJoinThreads / 32];
-  pdl_wait();
-  attn_prefix<NQ, kAttnJoinThreads>(c, A, s_pre, s_warp);
-  const int lane = threadIdx.x & 31;
-  const long long rows = (long long)A.tokens * A.nh, step = (long long)gridDim.x * (kAttnJoinThreads / 32);
-  for (long long row = (long long)blockIdx.x * (kAttnJoinThreads / 32) + (threadIdx.x >> 5); row < rows; row += step)
-    attn_join_row<T, HD, NQ>(c, A, s_pre, row, lane);
 }
 
 }  // namespace cats

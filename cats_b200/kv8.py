@@ -27,7 +27,7 @@ import torch
 from . import _lib
 from .ops import _DTYPES, _on, dtype_code
 
-PAGES, HEAD_DIMS, MAX_SEQS = (16, 32, 64, 128), (32, 64, 96, 128), 1024
+PAGES, HEAD_DIMS, MAX_SEQS, STATUS_INTS = (16, 32, 64, 128), (32, 64, 96, 128), 1024, 256
 _STATUS = {1: "the pool has no free page left", 2: "a page id is out of range, or a shared page would have been written",
            4: "a sequence is longer than the page table allows, or a length or position is negative",
            8: "a parent is out of range", 16: "cu does not fit the number of tokens"}
@@ -79,7 +79,8 @@ class KVCache8:
         if page not in PAGES or hd not in HEAD_DIMS or table.shape[0] > MAX_SEQS or min(*codes.shape, *table.shape) < 1:
             raise _bad(f"page must be one of {PAGES}, head_dim one of {HEAD_DIMS}, sequences 1 .. {MAX_SEQS}")
         self.codes, self.scales, self.table, self.lens, self.refs = codes, scales, table, lens, refs
-        self.status = torch.zeros(1, dtype=torch.int32, device=codes.device)
+        self._state = torch.zeros(STATUS_INTS, dtype=torch.int32, device=codes.device)
+        self.status = self._state[:1]
         self.device = codes.device
         self.n_layers, self.n_pages, self.n_kv_heads, self.page, self.head_dim = L, P, nkv, page, hd
         self.n_seqs, self.max_pages = table.shape

@@ -408,13 +408,15 @@ int cats_export_list(const void* ws, size_t ws_bytes, int B, int H, int I, int d
  * position), 8 a parent is out of range, 16 cu does not fit the number of tokens.
  * No reference counterpart (the reference leaves the cache to HF's modelling code).
  */
+enum { CATS_KV8_STATUS_INTS = 256 };
 typedef struct cats_kv8 {
   void* codes;    /* [n_layers, n_pages, 2, n_kv_heads, page, head_dim] e4m3 */
   float* scales;  /* [n_layers, n_pages, 2, n_kv_heads]                      */
   int* table;     /* [n_seqs, max_pages]                                     */
   int* lens;      /* [n_seqs]                                                */
   int* refs;      /* [n_pages]                                               */
-  int* status;    /* [1]                                                     */
+  int* status;    /* [CATS_KV8_STATUS_INTS], zero at first: the status word, then scratch */
+                  /* that the calls leave zero                               */
   int n_layers, n_pages, n_seqs, max_pages, n_kv_heads, page, head_dim;
 } cats_kv8;
 
