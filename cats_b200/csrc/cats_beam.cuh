@@ -34,7 +34,7 @@ __device__ __forceinline__ unsigned long long beam_key(float x, int idx) {
 
 struct BeamPart {                                      // of one row (or part of a row)
   float max;                                           // largest logit (not a NaN)
-  float sum;                                           // sum of exp(logit - max); NaN if a logit is
+  float sum;                                           // sum of exp(logit - max); NaN if one is NaN or +inf
 };
 
 struct BeamArgs {
@@ -51,6 +51,15 @@ struct BeamArgs {
   uint8_t* out_done;                                   // [n, k] or nullptr
 };
 
+constexpr int kBeamPer = 16;                           // values of a thread and tile
+constexpr int kBeamTile = kBeamThreads * kBeamPer;
+constexpr int kBeamCap = 1024;                         // candidates that a CTA can hold
+
+__device__ __forceinline__ float beam_exp(float d) {   // e^d
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * 1.4426950408889634f));
+  return r;
+}
 __device__ __forceinline__ unsigned long long beam_block_max(unsigned long long v, unsigned long long* s) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -64,35 +73,162 @@ __device__ __forceinline__ unsigned long long beam_block_max(unsigned long long 
   return v;
 }
 
-// One CTA per row: k passes that each find the largest key below the last one found.
+// One CTA per part of a row, one pass over its logits (bound: HBM; 16 values a thread in registers,
+// 16-byte loads whatever the row's alignment): the softmax's running maximum and sum, and the k
+// largest.  For those, the first tile gives a threshold that at least k of its values reach: the k-th
+// largest of the maxima of 32 groups of 128 values.  From there on a value costs one comparison; the
+// few that reach the threshold (k or a few more of the first tile, about k / 4096 of the others) are
+// put aside and ranked at the end.  Rows with more than kBeamCap of them (many equal or nothing but
+// -inf, values in rising order) take k more passes, each for the largest key below the last.
 template <typename T>
-__global__ void __launch_bounds__(kBeamThreads) k_beam_rows_simple(const BeamArgs A) {
+__global__ void __launch_bounds__(kBeamThreads) k_beam_rows(const BeamArgs A) {
+  constexpr int N = VecT<T>::N, NV = kBeamPer / N;
+  __shared__ unsigned long long s_keys[kBeamCap];
+  __shared__ unsigned long long s_group[32];
+  __shared__ float s_max[kBeamThreads / 32];
+  __shared__ double s_sum[kBeamThreads / 32];
+  __shared__ int s_count;
+  __shared__ unsigned long long s_tau;
   pdl_wait();
-  __shared__ unsigned long long s_key[kBeamThreads / 32];
-  __shared__ float s_sum[kBeamThreads / 32];
-  const int row = blockIdx.x;
+  pdl_launch_dependents();
+  const int row = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const T* x = static_cast<const T*>(A.logits) + (size_t)row * A.ld;
+  // vectors of the row counted from the 16-byte boundary at or before its first value
+  const int skip = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+  const int vecs = (int)(((long long)skip + A.vocab + N - 1) / N);
+  const int v0 = (int)((long long)vecs * blockIdx.x / A.splits), v1 = (int)((long long)vecs * (blockIdx.x + 1) / A.splits);
+  const int i0 = max(v0 * N - skip, 0), i1 = min(v1 * N - skip, A.vocab);    // its values
+  if (threadIdx.x == 0) s_count = 0;
+
+  // the vectors of the next tile are on their way while this one is worked on; the ones at the row's
+  // ends, which reach over it, are read value by value when it is their turn
+  auto whole = [&](int v) { return v < v1 && v * N - skip >= 0 && v * N - skip + N <= A.vocab; };
+  uint4 next[NV];
+  auto fetch = [&](int base) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int v = base + k * kBeamThreads + threadIdx.x;
+      if (whole(v)) next[k] = ldg_stream(reinterpret_cast<const uint4*>(x + (v * N - skip)));
+    }
+  };
+  fetch(v0);
+  float m = -CUDART_INF_F, sum = 0.f, tau = -CUDART_INF_F;
+  for (int base = v0; base < v1; base += kBeamThreads * NV) {
+    float f[NV][N];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int v = base + k * kBeamThreads + threadIdx.x, e0 = v * N - skip;
+      VecT<T>::unpack(next[k], f[k]);
+      if (!whole(v)) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[k][i] = v < v1 && e0 + i >= 0 && e0 + i < A.vocab ? VecT<T>::to_f(x[e0 + i]) : -CUDART_INF_F;
+      }
+    }
+    fetch(base + kBeamThreads * NV);
+    float top = -CUDART_INF_F;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int i = 0; i < N; ++i) top = fmaxf(top, f[k][i]);     // (drops NaN)
+    const float tile_top = top;
+    if (top > m) {
+      sum *= beam_exp(m - top);                        // m = -inf: 0
+      m = top;
+    }
+    const float ref = m == -CUDART_INF_F ? 0.f : m;
+    float part = 0.f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int i = 0; i < N; ++i) part += beam_exp(f[k][i] - ref);   // a NaN or +inf makes it NaN
+    sum += part;
+    if (base == v0) {
+      unsigned long long best = 0;
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int e = (base + k * kBeamThreads + (int)threadIdx.x) * N - skip + i;
+          if (e >= i0 && e < i1) {
+            const unsigned long long key = beam_key(f[k][i], e);
+            best = key > best ? key : best;
+          }
+        }
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) {
+        const unsigned long long u = __shfl_xor_sync(0xffffffffu, best, o);
+        best = u > best ? u : best;
+      }
+      if ((lane & 7) == 0) s_group[threadIdx.x >> 3] = best;
+      __syncthreads();
+      if (warp == 0) {
+        const unsigned long long mine = s_group[lane];
+        int rank = 0;
+#pragma unroll 8
+        for (int j = 0; j < 32; ++j) rank += s_group[j] > mine || (s_group[j] == mine && j < lane);
+        if (rank == A.k - 1) s_tau = mine;             // 0 where fewer than k groups hold a value
+      }
+      __syncthreads();
+      const unsigned long long t = s_tau;
+      tau = t == 0 ? -CUDART_INF_F : beam_value((uint32_t)(t >> 32));
+    }
+    if (tile_top < tau) continue;                      // (a NaN counts as -inf)
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float y = f[k][i] == f[k][i] ? f[k][i] : -CUDART_INF_F;
+        if (y >= tau) {
+          const int e = (base + k * kBeamThreads + (int)threadIdx.x) * N - skip + i;
+          if (e >= i0 && e < i1) {
+            const int at = atomicAdd(&s_count, 1);
+            if (at < kBeamCap) s_keys[at] = beam_key(y, e);
+          }
+        }
+      }
+  }
+  // maximum and sum of the part
+  float top = m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  double all = top == -CUDART_INF_F ? (sum == sum ? 0.0 : (double)sum) : (double)(sum * beam_exp(m - top));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+  if (lane == 0) {
+    s_max[warp] = top;
+    s_sum[warp] = all;
+  }
+  __syncthreads();
+  const size_t part = (size_t)row * A.splits + blockIdx.x;
+  if (threadIdx.x == 0) {
+    float t = -CUDART_INF_F;
+    for (int w = 0; w < kBeamThreads / 32; ++w) t = fmaxf(t, s_max[w]);
+    double total = 0;
+    for (int w = 0; w < kBeamThreads / 32; ++w)
+      total += s_max[w] == -CUDART_INF_F ? s_sum[w] : s_sum[w] * (double)expf(s_max[w] - t);
+    A.parts[part] = {t, (float)total};
+  }
+  unsigned long long* out = A.keys + part * A.k;
+  const int n = s_count;
+  if (n <= kBeamCap) {
+    for (int i = threadIdx.x; i < n; i += kBeamThreads) {
+      const unsigned long long mine = s_keys[i];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += s_keys[j] > mine;
+      if (rank < A.k) out[rank] = mine;
+    }
+    for (int i = n + threadIdx.x; i < A.k; i += kBeamThreads) out[i] = 0;
+    return;
+  }
   unsigned long long last = ~0ull;
-  float top = 0.f;
   for (int k = 0; k < A.k; ++k) {
     unsigned long long best = 0;
-    for (int i = threadIdx.x; i < A.vocab; i += kBeamThreads) {
+    for (int i = i0 + threadIdx.x; i < i1; i += kBeamThreads) {
       const unsigned long long key = beam_key(VecT<T>::to_f(x[i]), i);
       if (key < last && key > best) best = key;
     }
-    last = beam_block_max(best, s_key);
-    if (k == 0) top = beam_value((uint32_t)(last >> 32));
-    if (threadIdx.x == 0) A.keys[(size_t)row * A.k + k] = last;
-  }
-  float sum = 0.f;
-  for (int i = threadIdx.x; i < A.vocab; i += kBeamThreads) sum += expf(VecT<T>::to_f(x[i]) - top);
-  sum = warp_sum(sum);
-  if ((threadIdx.x & 31) == 0) s_sum[threadIdx.x >> 5] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    double t = 0;
-    for (int w = 0; w < kBeamThreads / 32; ++w) t += s_sum[w];
-    A.parts[row] = {top, (float)t};
+    last = beam_block_max(best, s_keys);
+    if (threadIdx.x == 0) out[k] = last;
   }
 }
 
@@ -110,14 +246,19 @@ __global__ void __launch_bounds__(kBeamThreads) k_beam_join(const BeamArgs A) {
   for (int i = threadIdx.x; i < rows * per_row; i += blockDim.x)
     s_key[i] = A.keys[(size_t)row0 * per_row + i];
   for (int i = threadIdx.x; i < rows * A.k; i += blockDim.x) s_tok[i] = -1;
-  for (int r = threadIdx.x; r < rows; r += blockDim.x) {
+  for (int r = threadIdx.x >> 5; r < rows; r += kBeamThreads / 32) {     // a warp per row
     const BeamPart* p = A.parts + (size_t)(row0 + r) * A.splits;
+    const int lane = threadIdx.x & 31;
     float top = -CUDART_INF_F;
-    for (int s = 0; s < A.splits; ++s) top = fmaxf(top, p[s].max);
+    for (int s = lane; s < A.splits; s += 32) top = fmaxf(top, p[s].max);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     double sum = 0;
-    for (int s = 0; s < A.splits; ++s)
-      if (!(p[s].max == -CUDART_INF_F && p[s].sum == 0.f)) sum += (double)p[s].sum * exp((double)p[s].max - (double)top);
-    s_lse[r] = (double)top + log(sum);
+    for (int s = lane; s < A.splits; s += 32)
+      if (!(p[s].max == -CUDART_INF_F && p[s].sum == 0.f)) sum += (double)p[s].sum * (double)expf(p[s].max - top);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) s_lse[r] = (double)top + log(sum);
   }
   __syncthreads();
   // the k largest logits of each row, in order

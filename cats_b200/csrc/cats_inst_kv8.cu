@@ -86,7 +86,15 @@ cudaError_t attend(const cats_kv8& c, int layer, const void* q, long long q_ld, 
   return inst_kv8_attend<T>(c, A, st);
 }
 
-size_t beam_keys(int rows, int k) { return (size_t)rows * k; }
+// Parts of a row: enough CTAs for four per SM, no part below a tile of the kernel, and the keys of an
+// item's parts (8 bytes, `beams * splits * k` of them) within 48 KB of the joining CTA.
+int beam_splits(long long rows, int beams, int vocab, int k) {
+  const long long want = (4LL * dev_info().sms + rows - 1) / rows, tiles = ((long long)vocab + kBeamTile - 1) / kBeamTile;
+  const long long most = 6144 / ((long long)beams * k);
+  long long s = want < tiles ? want : tiles;
+  if (s > most) s = most;
+  return s < 1 ? 1 : (int)s;
+}
 
 }  // namespace
 
@@ -201,8 +209,8 @@ int cats_kv8_compact(const cats_kv8* cache, int* n_live, void* ws, size_t ws_byt
 
 size_t cats_beam_select_bytes(int n, int beams, int vocab, int k) {
   if (n < 1 || beams < 1 || vocab < 1 || k < 1) return 0;
-  const size_t rows = (size_t)n * beams;
-  return rows * sizeof(BeamPart) + beam_keys((int)rows, k) * sizeof(unsigned long long) + 16;
+  const size_t parts = (size_t)n * beams * beam_splits((long long)n * beams, beams, vocab, k);
+  return parts * (sizeof(BeamPart) + k * sizeof(unsigned long long));
 }
 
 int cats_beam_select(const void* logits, long long ld, const float* scores, const uint8_t* done, int n, int beams,
@@ -211,7 +219,7 @@ int cats_beam_select(const void* logits, long long ld, const float* scores, cons
   if (!known_dtype(dtype)) return CATS_ERR_DTYPE;
   if (n < 1 || beams < 1 || beams > kBeamMaxBeams || vocab < 1 || k < 1 || k > kBeamMaxK || ld < vocab)
     return CATS_ERR_RANGE;
-  if ((long long)n * beams > 0x7fffffffLL || (long long)beams * vocab < k) return CATS_ERR_RANGE;
+  if ((long long)n * beams > 65535 || (long long)beams * vocab < k) return CATS_ERR_RANGE;
   if (done && (eos < 0 || eos >= vocab)) return CATS_ERR_RANGE;
   if (!logits || !scores || !out_scores || !out_rows || !out_tokens || !ws) return CATS_ERR_NULL;
   if (reinterpret_cast<uintptr_t>(logits) % esize(dtype) || !aligned16(ws)) return CATS_ERR_ALIGN;
@@ -220,15 +228,16 @@ int cats_beam_select(const void* logits, long long ld, const float* scores, cons
   BeamArgs A;
   const int rows = n * beams;
   A.logits = logits; A.ld = ld; A.scores = scores; A.done = done;
-  A.n = n; A.beams = beams; A.vocab = vocab; A.k = k; A.eos = eos; A.splits = 1;
+  A.n = n; A.beams = beams; A.vocab = vocab; A.k = k; A.eos = eos;
+  A.splits = beam_splits(rows, beams, vocab, k);
   A.keys = (unsigned long long*)ws;
-  A.parts = (BeamPart*)(A.keys + beam_keys(rows, k));
+  A.parts = (BeamPart*)(A.keys + (size_t)rows * A.splits * k);
   A.out_scores = out_scores; A.out_rows = out_rows; A.out_tokens = out_tokens; A.out_done = out_done;
   cudaError_t e;
-  const dim3 grid(rows), block(kBeamThreads);
-  if (dtype == CATS_F32) e = launch(k_beam_rows_simple<float>, grid, block, 0, st, A);
-  else if (dtype == CATS_F16) e = launch(k_beam_rows_simple<__half>, grid, block, 0, st, A);
-  else e = launch(k_beam_rows_simple<__nv_bfloat16>, grid, block, 0, st, A);
+  const dim3 grid(A.splits, rows), block(kBeamThreads);
+  if (dtype == CATS_F32) e = launch(k_beam_rows<float>, grid, block, 0, st, A);
+  else if (dtype == CATS_F16) e = launch(k_beam_rows<__half>, grid, block, 0, st, A);
+  else e = launch(k_beam_rows<__nv_bfloat16>, grid, block, 0, st, A);
   if (e != cudaSuccess) return launch_status(e);
   const size_t smem = (size_t)beams * k * 8 + (size_t)beams * A.splits * k * 8 + (size_t)beams * 8 + (size_t)beams * k * 4;
   return launch_status(launch(k_beam_join, dim3(n), block, smem, st, A));
