@@ -55,9 +55,10 @@ constexpr int kBeamPer = 16;                           // values of a thread and
 constexpr int kBeamTile = kBeamThreads * kBeamPer;
 constexpr int kBeamCap = 1024;                         // candidates that a CTA can hold
 
-__device__ __forceinline__ float beam_exp(float d) {   // e^d
+constexpr float kLog2e = 1.4426950408889634f, kFar = 1e37f;
+__device__ __forceinline__ float beam_exp2(float d) {
   float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * 1.4426950408889634f));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
   return r;
 }
 __device__ __forceinline__ unsigned long long beam_block_max(unsigned long long v, unsigned long long* s) {
@@ -112,7 +113,7 @@ __global__ void __launch_bounds__(kBeamThreads) k_beam_rows(const BeamArgs A) {
     }
   };
   fetch(v0);
-  float m = -CUDART_INF_F, sum = 0.f, tau = -CUDART_INF_F;
+  float m = -CUDART_INF_F, ref = 0.f, sum = 0.f, tau = -CUDART_INF_F;
   for (int base = v0; base < v1; base += kBeamThreads * NV) {
     float f[NV][N];
 #pragma unroll
@@ -130,30 +131,52 @@ __global__ void __launch_bounds__(kBeamThreads) k_beam_rows(const BeamArgs A) {
     for (int k = 0; k < NV; ++k)
 #pragma unroll
       for (int i = 0; i < N; ++i) top = fmaxf(top, f[k][i]);     // (drops NaN)
-    const float tile_top = top;
     if (top > m) {
-      sum *= beam_exp(m - top);                        // m = -inf: 0
+      const float to = top * kLog2e;
+      sum *= beam_exp2(fabsf(ref) <= kFar && fabsf(to) <= kFar ? ref - to : (m - top) * kLog2e);
+      if (m == -CUDART_INF_F && sum == sum) sum = 0.f;
       m = top;
+      ref = to;
     }
-    const float ref = m == -CUDART_INF_F ? 0.f : m;
+    // 2^(x log2e - ref), one rounding: ref is only near m log2e, which the end of the kernel makes up
+    // for.  Next to the type's ends (masks of its lowest value) m log2e is not a number any more.
     float part = 0.f;
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-      for (int i = 0; i < N; ++i) part += beam_exp(f[k][i] - ref);   // a NaN or +inf makes it NaN
-    sum += part;
-    if (base == v0) {
-      unsigned long long best = 0;
+    if (fabsf(ref) <= kFar) {
 #pragma unroll
       for (int k = 0; k < NV; ++k)
 #pragma unroll
+        for (int i = 0; i < N; ++i) part += beam_exp2(fmaf(f[k][i], kLog2e, -ref));   // a NaN makes it NaN
+    } else {                                           // m = +inf: NaN
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int i = 0; i < N; ++i) part += beam_exp2((f[k][i] - m) * kLog2e);
+    }
+    sum += part;
+    // bit k N + i: the value is this row's and reaches the threshold (a NaN counts as -inf)
+    auto reaching = [&](float t) {
+      uint32_t bits = 0;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int v = base + k * kBeamThreads + threadIdx.x;
+#pragma unroll
         for (int i = 0; i < N; ++i) {
-          const int e = (base + k * kBeamThreads + (int)threadIdx.x) * N - skip + i;
-          if (e >= i0 && e < i1) {
-            const unsigned long long key = beam_key(f[k][i], e);
-            best = key > best ? key : best;
+          if (t == -CUDART_INF_F ? !(f[k][i] > t) || f[k][i] > t : f[k][i] >= t) bits |= 1u << (k * N + i);
+        }
+        if (!whole(v)) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            const int e = v * N - skip + i;
+            if (v >= v1 || e < 0 || e >= A.vocab) bits &= ~(1u << (k * N + i));
           }
         }
+      }
+      return bits;
+    };
+    auto index = [&](int bit) { return (base + (bit / N) * kBeamThreads + (int)threadIdx.x) * N - skip + bit % N; };
+    if (base == v0) {
+      const uint32_t bits = reaching(top);             // the first of the thread's largest
+      unsigned long long best = bits ? beam_key(top, index(__ffs(bits) - 1)) : 0;
 #pragma unroll
       for (int o = 1; o < 8; o <<= 1) {
         const unsigned long long u = __shfl_xor_sync(0xffffffffu, best, o);
@@ -172,26 +195,20 @@ __global__ void __launch_bounds__(kBeamThreads) k_beam_rows(const BeamArgs A) {
       const unsigned long long t = s_tau;
       tau = t == 0 ? -CUDART_INF_F : beam_value((uint32_t)(t >> 32));
     }
-    if (tile_top < tau) continue;                      // (a NaN counts as -inf)
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float y = f[k][i] == f[k][i] ? f[k][i] : -CUDART_INF_F;
-        if (y >= tau) {
-          const int e = (base + k * kBeamThreads + (int)threadIdx.x) * N - skip + i;
-          if (e >= i0 && e < i1) {
-            const int at = atomicAdd(&s_count, 1);
-            if (at < kBeamCap) s_keys[at] = beam_key(y, e);
-          }
-        }
-      }
+    if (top < tau) continue;
+    for (uint32_t bits = reaching(tau); bits; bits &= bits - 1) {
+      const int e = index(__ffs(bits) - 1), at = atomicAdd(&s_count, 1);
+      if (at < kBeamCap) s_keys[at] = beam_key(VecT<T>::to_f(x[e]), e);
+    }
   }
+  // Sum relative to m instead of 2^ref: both products are with the same constant, so what is left of
+  // its error is a factor of (x - m)
+  if (m > -CUDART_INF_F && fabsf(ref) <= kFar) sum *= beam_exp2(-fmaf(m, kLog2e, -ref));
   // maximum and sum of the part
   float top = m;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  double all = top == -CUDART_INF_F ? (sum == sum ? 0.0 : (double)sum) : (double)(sum * beam_exp(m - top));
+  double all = top == -CUDART_INF_F ? (sum == sum ? 0.0 : (double)sum) : (double)(sum * beam_exp2((m - top) * kLog2e));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
   if (lane == 0) {
@@ -241,11 +258,11 @@ __global__ void __launch_bounds__(kBeamThreads) k_beam_join(const BeamArgs A) {
   double* s_c = reinterpret_cast<double*>(smem);                       // [rows * k]
   unsigned long long* s_key = reinterpret_cast<unsigned long long*>(s_c + rows * A.k);  // [rows * per_row]
   double* s_lse = reinterpret_cast<double*>(s_key + (size_t)rows * per_row);            // [rows]
-  int* s_tok = reinterpret_cast<int*>(s_lse + rows);                   // [rows * k]
+  long long* s_flat = reinterpret_cast<long long*>(s_lse + rows);      // [rows * k] beam * vocab + token, -1: none
   const int item = blockIdx.x, row0 = item * A.beams;
   for (int i = threadIdx.x; i < rows * per_row; i += blockDim.x)
     s_key[i] = A.keys[(size_t)row0 * per_row + i];
-  for (int i = threadIdx.x; i < rows * A.k; i += blockDim.x) s_tok[i] = -1;
+  for (int i = threadIdx.x; i < rows * A.k; i += blockDim.x) s_flat[i] = -1;
   for (int r = threadIdx.x >> 5; r < rows; r += kBeamThreads / 32) {     // a warp per row
     const BeamPart* p = A.parts + (size_t)(row0 + r) * A.splits;
     const int lane = threadIdx.x & 31;
@@ -288,21 +305,20 @@ __global__ void __launch_bounds__(kBeamThreads) k_beam_join(const BeamArgs A) {
       v = -CUDART_INF;
     }
     s_c[r * A.k + rank] = v;
-    s_tok[r * A.k + rank] = tok;
+    s_flat[r * A.k + rank] = (long long)r * A.vocab + tok;
   }
   __syncthreads();
   for (int i = threadIdx.x; i < rows * A.k; i += blockDim.x) {
-    const int tok = s_tok[i], r = i / A.k;
-    if (tok < 0) continue;                             // fewer than k tokens in the vocabulary
+    const long long flat = s_flat[i];
+    if (flat < 0) continue;                            // fewer than k tokens in the vocabulary
     const double v = s_c[i];
     int rank = 0;
-    for (int j = 0; j < rows * A.k; ++j) {
-      if (s_tok[j] < 0) continue;
-      const int q = j / A.k;
-      rank += s_c[j] > v || (s_c[j] == v && (q < r || (q == r && s_tok[j] < tok)));
-    }
+#pragma unroll 4
+    for (int j = 0; j < rows * A.k; ++j)
+      rank += s_flat[j] >= 0 && (s_c[j] > v || (s_c[j] == v && s_flat[j] < flat));
     if (rank >= A.k) continue;
     const size_t o = (size_t)item * A.k + rank;
+    const int r = i / A.k, tok = (int)(flat - (long long)r * A.vocab);
     A.out_scores[o] = (float)v;
     A.out_rows[o] = row0 + r;
     A.out_tokens[o] = tok;

@@ -239,7 +239,7 @@ int cats_beam_select(const void* logits, long long ld, const float* scores, cons
   else if (dtype == CATS_F16) e = launch(k_beam_rows<__half>, grid, block, 0, st, A);
   else e = launch(k_beam_rows<__nv_bfloat16>, grid, block, 0, st, A);
   if (e != cudaSuccess) return launch_status(e);
-  const size_t smem = (size_t)beams * k * 8 + (size_t)beams * A.splits * k * 8 + (size_t)beams * 8 + (size_t)beams * k * 4;
+  const size_t smem = (size_t)beams * k * 8 + (size_t)beams * A.splits * k * 8 + (size_t)beams * 8 + (size_t)beams * k * 8;
   return launch_status(launch(k_beam_join, dim3(n), block, smem, st, A));
 }
 
