@@ -79,10 +79,10 @@ __device__ __forceinline__ unsigned long long beam_block_max(unsigned long long 
 // largest.  For those, the first tile gives a threshold that at least k of its values reach: the k-th
 // largest of the maxima of 32 groups of 128 values.  From there on a value costs one comparison; the
 // few that reach the threshold (k or a few more of the first tile, about k / 4096 of the others) are
-// put aside and ranked at the end.  Rows with more than kBeamCap of them (many equal or nothing but
+// put aside and ranked at the end; the threshold follows them after 2, 4, 8 ... tiles.  Rows with more than kBeamCap of them (many equal or nothing but
 // -inf, values in rising order) take k more passes, each for the largest key below the last.
 template <typename T>
-__global__ void __launch_bounds__(kBeamThreads) k_beam_rows(const BeamArgs A) {
+__global__ void __launch_bounds__(kBeamThreads, 4) k_beam_rows(const BeamArgs A) {
   constexpr int N = VecT<T>::N, NV = kBeamPer / N;
   __shared__ unsigned long long s_keys[kBeamCap];
   __shared__ unsigned long long s_group[32];
@@ -195,10 +195,26 @@ __global__ void __launch_bounds__(kBeamThreads) k_beam_rows(const BeamArgs A) {
       const unsigned long long t = s_tau;
       tau = t == 0 ? -CUDART_INF_F : beam_value((uint32_t)(t >> 32));
     }
-    if (top < tau) continue;
-    for (uint32_t bits = reaching(tau); bits; bits &= bits - 1) {
-      const int e = index(__ffs(bits) - 1), at = atomicAdd(&s_count, 1);
-      if (at < kBeamCap) s_keys[at] = beam_key(VecT<T>::to_f(x[e]), e);
+    if (top >= tau) {
+      for (uint32_t bits = reaching(tau); bits; bits &= bits - 1) {
+        const int e = index(__ffs(bits) - 1), at = atomicAdd(&s_count, 1);
+        if (at < kBeamCap) s_keys[at] = beam_key(VecT<T>::to_f(x[e]), e);
+      }
+    }
+    // after 2, 4, 8 ... tiles: the k-th largest so far is the threshold of the next
+    const int tiles = (base - v0) / (kBeamThreads * NV) + 1;
+    if (tiles > 1 && (tiles & (tiles - 1)) == 0 && base + kBeamThreads * NV < v1) {
+      __syncthreads();
+      const int n = s_count;
+      if (n <= kBeamThreads && (int)threadIdx.x < n) {
+        const unsigned long long mine = s_keys[threadIdx.x];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += s_keys[j] > mine;
+        if (rank == A.k - 1) s_tau = mine;
+      }
+      __syncthreads();
+      const unsigned long long t = s_tau;
+      tau = t == 0 ? -CUDART_INF_F : beam_value((uint32_t)(t >> 32));
     }
   }
   // Sum relative to m instead of 2^ref: both products are with the same constant, so what is left of

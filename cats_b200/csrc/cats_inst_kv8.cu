@@ -86,10 +86,11 @@ cudaError_t attend(const cats_kv8& c, int layer, const void* q, long long q_ld, 
   return inst_kv8_attend<T>(c, A, st);
 }
 
-// Parts of a row: enough CTAs for four per SM, no part below a tile of the kernel, and the keys of an
+// Parts of a row: as many CTAs as run at once (four per SM; a second, partly filled round costs up to
+// a third), no part below a tile of the kernel, and the keys of an
 // item's parts (8 bytes, `beams * splits * k` of them) within 48 KB of the joining CTA.
 int beam_splits(long long rows, int beams, int vocab, int k) {
-  const long long want = (4LL * dev_info().sms + rows - 1) / rows, tiles = ((long long)vocab + kBeamTile - 1) / kBeamTile;
+  const long long want = 4LL * dev_info().sms / rows, tiles = ((long long)vocab + kBeamTile - 1) / kBeamTile;
   const long long most = 6144 / ((long long)beams * k);
   long long s = want < tiles ? want : tiles;
   if (s > most) s = most;
