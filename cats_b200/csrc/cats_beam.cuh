@@ -103,14 +103,16 @@ __global__ void __launch_bounds__(kBeamThreads, 4) k_beam_rows(const BeamArgs A)
 
   // the vectors of the next tile are on their way while this one is worked on; the ones at the row's
   // ends, which reach over it, are read value by value when it is their turn
-  auto whole = [&](int v) { return v < v1 && v * N - skip >= 0 && v * N - skip + N <= A.vocab; };
+  const int whole0 = max(v0, skip ? 1 : 0);            // vectors that lie inside the row
+  const unsigned wholes = (unsigned)max(min(v1, (int)(((long long)skip + A.vocab) / N)) - whole0, 0);
+  auto whole = [&](int v) { return (unsigned)(v - whole0) < wholes; };
   uint4 next[NV];
+  const uint4* from = reinterpret_cast<const uint4*>(x - skip) + v0 + threadIdx.x;   // (never read before the row)
   auto fetch = [&](int base) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int v = base + k * kBeamThreads + threadIdx.x;
-      if (whole(v)) next[k] = ldg_stream(reinterpret_cast<const uint4*>(x + (v * N - skip)));
-    }
+    for (int k = 0; k < NV; ++k)
+      if (whole(base + k * kBeamThreads + (int)threadIdx.x)) next[k] = ldg_stream(from + k * kBeamThreads);
+    from += kBeamThreads * NV;
   };
   fetch(v0);
   float m = -CUDART_INF_F, ref = 0.f, sum = 0.f, tau = -CUDART_INF_F;

@@ -134,8 +134,8 @@ int cats_kv8_append(const cats_kv8* cache, int layer, const void* qkv, long long
   return launch_status(e);
 }
 
-size_t cats_kv8_attend_bytes(const cats_kv8* cache, int n_tokens, int n_heads) {
-  if (!cache || cache->head_dim < 1 || n_tokens < 1 || n_heads < 1) return 0;
+size_t cats_kv8_attend_bytes(const cats_kv8* cache) {
+  if (!cache || cache->head_dim < 1) return 0;
   return sizeof(float) * 2 * (size_t)dev_info().sms * attn_part_floats(kAttnMaxRows, cache->head_dim);
 }
 
@@ -150,7 +150,7 @@ int cats_kv8_attend(const cats_kv8* cache, int layer, const void* q, long long q
   if (!q || !out || !ws) return CATS_ERR_NULL;
   if (q_ld < (long long)n_heads * cache->head_dim) return CATS_ERR_RANGE;
   if (!aligned16(q) || (q_ld * esize(dtype)) % 16 || !aligned16(out) || !aligned16(ws)) return CATS_ERR_ALIGN;
-  if (ws_bytes < cats_kv8_attend_bytes(cache, n_tokens, n_heads)) return CATS_ERR_WORKSPACE;
+  if (ws_bytes < cats_kv8_attend_bytes(cache)) return CATS_ERR_WORKSPACE;
   cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e;
   if (dtype == CATS_F32) e = attend<float>(*cache, layer, q, q_ld, cu, n_tokens, n_heads, scale, out, ws, st);

@@ -8,7 +8,17 @@ namespace cats {
 template <typename T, int HD, int NQ>
 static cudaError_t run_attend(const cats_kv8& c, const KvAttnArgs<T>& A, cudaStream_t st) {
   using S = AttnShape<NQ>;
-  return launch(k_kv8_attend<T, HD, NQ>, dim3(A.ctas), dim3(S::kThreads), attn_smem<NQ>(), st, c, A);
+  // (the attribute stays with the kernel: once per device; two threads at once set the same value)
+  static bool ready[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !ready[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(k_kv8_attend<T, HD, NQ>),
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, (int)attn_smem<NQ>());
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) ready[dev] = true;
+  }
+  return launch_ready(k_kv8_attend<T, HD, NQ>, dim3(A.ctas), dim3(S::kThreads), attn_smem<NQ>(), st, c, A);
 }
 
 template <typename T, int HD>

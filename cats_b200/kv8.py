@@ -25,7 +25,9 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from . import _lib
-from .ops import _DTYPES, _on, dtype_code
+from .ops import _DTYPES, _raw_stream, dtype_code
+
+_current_device = torch._C._cuda_getDevice
 
 PAGES, HEAD_DIMS, MAX_SEQS, STATUS_INTS = (16, 32, 64, 128), (32, 64, 96, 128), 1024, 256
 _STATUS = {1: "the pool has no free page left", 2: "a page id is out of range, or a shared page would have been written",
@@ -88,17 +90,25 @@ class KVCache8:
         self._c = _lib.Kv8(codes.data_ptr(), scales.data_ptr(), table.data_ptr(), lens.data_ptr(), refs.data_ptr(),
                            self.status.data_ptr(), L, P, self.n_seqs, self.max_pages, nkv, page, hd)
         self._p = ctypes.byref(self._c)
+        self._index = codes.device.index
         lib = _lib.lib()
-        self._grow, self._append, self._attend = lib.cats_kv8_grow, lib.cats_kv8_append, lib.cats_kv8_attend
-        self._reorder, self._compact = lib.cats_kv8_reorder, lib.cats_kv8_compact
-        self._attend_bytes = lib.cats_kv8_attend_bytes
+        with torch.cuda.device(self._index):
+            self._attend_nbytes = int(lib.cats_kv8_attend_bytes(self._p))
         self._reorder_nbytes = int(lib.cats_kv8_reorder_bytes(self._p))
         self._compact_nbytes = int(lib.cats_kv8_compact_bytes(self._p))
 
-    # ---- argument checks ----------------------------------------------------------------------------
-    def _stream(self) -> int:
-        return torch.cuda.current_stream(self.device).cuda_stream
+    def _call(self, what: str, *args) -> None:
+        """One C call on the current stream of the cache's device."""
+        i = self._index
+        if _current_device() == i:
+            st = getattr(_lib.lib(), what)(self._p, *args, _raw_stream(i))
+        else:
+            with torch.cuda.device(i):
+                st = getattr(_lib.lib(), what)(self._p, *args, _raw_stream(i))
+        if st:
+            _lib.check(st, what)
 
+    # ---- argument checks ----------------------------------------------------------------------------
     def _cu(self, cu: Optional[torch.Tensor]) -> Optional[int]:
         if cu is None:
             return None
@@ -124,10 +134,7 @@ class KVCache8:
         """``lens += n_new`` (or the counts of ``cu``), taking the pages that needs (``cats_kv8_grow``)."""
         if cu is None and n_new < 1:
             raise _bad("n_new must be positive")
-        with _on(self.device):
-            st = self._grow(self._p, self._cu(cu), n_new, self._stream())
-        if st:
-            _lib.check(st, "cats_kv8_grow")
+        self._call("cats_kv8_grow", self._cu(cu), n_new)
 
     def append(self, layer: int, qkv: torch.Tensor, n_heads: int, cos: Optional[torch.Tensor] = None,
                sin: Optional[torch.Tensor] = None, cu: Optional[torch.Tensor] = None,
@@ -159,17 +166,14 @@ class KVCache8:
                 raise _bad(f"cos and sin hold {rope} positions, the cache up to {self.max_len}")
             pc, ps = cos.data_ptr(), sin.data_ptr()
         if q_out is None:
-            q_out = torch.empty((n, n_heads, hd), dtype=dt, device=self.device)
+            q_out = torch.empty_strided((n, n_heads, hd), (n_heads * hd, hd, 1), dtype=dt, device=self.device)
         elif q_out.dtype != dt or q_out.device != self.device or not q_out.is_contiguous() \
                 or q_out.numel() != n * n_heads * hd:
             raise _bad("q_out must be contiguous with tokens * n_heads * head_dim elements of qkv's type")
         if n == 0:
             return q_out
-        with _on(self.device):
-            st = self._append(self._p, layer, qkv.data_ptr(), qkv.stride(0) if n > 1 else qkv.shape[1], self._cu(cu), n,
-                              pc, ps, rope, q_out.data_ptr(), n_heads, code, self._stream())
-        if st:
-            _lib.check(st, "cats_kv8_append")
+        self._call("cats_kv8_append", layer, qkv.data_ptr(), qkv.stride(0) if n > 1 else qkv.shape[1], self._cu(cu), n,
+                   pc, ps, rope, q_out.data_ptr(), n_heads, code)
         return q_out
 
     def attend(self, layer: int, q: torch.Tensor, cu: Optional[torch.Tensor] = None,
@@ -187,19 +191,15 @@ class KVCache8:
             raise _bad("the heads of a token must be contiguous in q")
         self._layer(layer)
         if out is None:
-            out = torch.empty((n, nh, hd), dtype=dt, device=self.device)
+            out = torch.empty_strided((n, nh, hd), (nh * hd, hd, 1), dtype=dt, device=self.device)
         elif out.dtype != dt or out.device != self.device or not out.is_contiguous() or out.numel() != n * nh * hd:
             raise _bad("out must be contiguous with as many elements as q, of q's type")
         if n == 0:
             return out
-        with _on(self.device):
-            nbytes = self._attend_bytes(self._p, n, nh)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-            st = self._attend(self._p, layer, q.data_ptr(), q.stride(0) if n > 1 else nh * hd, self._cu(cu), n, nh,
-                              hd ** -0.5 if scale is None else scale, out.data_ptr(), ws.data_ptr(), nbytes, code,
-                              self._stream())
-        if st:
-            _lib.check(st, "cats_kv8_attend")
+        nbytes = self._attend_nbytes
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        self._call("cats_kv8_attend", layer, q.data_ptr(), q.stride(0) if n > 1 else nh * hd, self._cu(cu), n, nh,
+                   hd ** -0.5 if scale is None else scale, out.data_ptr(), ws.data_ptr(), nbytes, code)
         return out
 
     # ---- pages --------------------------------------------------------------------------------------------
@@ -210,11 +210,8 @@ class KVCache8:
         if not isinstance(parents, torch.Tensor) or parents.dtype != torch.int32 or parents.device != self.device \
                 or not parents.is_contiguous() or parents.numel() != self.n_seqs:
             raise _bad(f"parents must be a contiguous int32 tensor of {self.n_seqs} elements on {self.device}")
-        with _on(self.device):
-            ws = torch.empty(self._reorder_nbytes, dtype=torch.uint8, device=self.device)
-            st = self._reorder(self._p, parents.data_ptr(), ws.data_ptr(), self._reorder_nbytes, self._stream())
-        if st:
-            _lib.check(st, "cats_kv8_reorder")
+        ws = torch.empty(self._reorder_nbytes, dtype=torch.uint8, device=self.device)
+        self._call("cats_kv8_reorder", parents.data_ptr(), ws.data_ptr(), self._reorder_nbytes)
 
     def _host_parents(self, changes) -> torch.Tensor:
         parents = list(range(self.n_seqs))
@@ -240,12 +237,9 @@ class KVCache8:
     def compact(self) -> torch.Tensor:
         """Move the live pages to the front of the pool (``cats_kv8_compact``).  Returns their number
         as a 0-dim int32 device tensor; the page ids from there on are free."""
-        with _on(self.device):
-            n = torch.empty((), dtype=torch.int32, device=self.device)
-            ws = torch.empty(self._compact_nbytes, dtype=torch.uint8, device=self.device)
-            st = self._compact(self._p, n.data_ptr(), ws.data_ptr(), self._compact_nbytes, self._stream())
-        if st:
-            _lib.check(st, "cats_kv8_compact")
+        n = torch.empty((), dtype=torch.int32, device=self.device)
+        ws = torch.empty(self._compact_nbytes, dtype=torch.uint8, device=self.device)
+        self._call("cats_kv8_compact", n.data_ptr(), ws.data_ptr(), self._compact_nbytes)
         return n
 
     # ---- host side ---------------------------------------------------------------------------------------------

@@ -48,6 +48,9 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream   # device index -> handle of its current stream
+
+
 def _stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
@@ -447,17 +450,18 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, done: Option
             raise RuntimeError("cats_b200: done needs eos, a token of the vocabulary")
     if n < 1 or not 1 <= beams <= 32 or not 1 <= k <= min(32, beams * vocab):
         raise RuntimeError(f"cats_b200: beam selection takes 1 .. 32 beams and 1 .. 32 results (got {n} x {beams}, k {k})")
-    out_scores = torch.empty((n, k), dtype=torch.float32, device=dev)
-    out_rows = torch.empty((n, k), dtype=torch.int32, device=dev)
-    out_tokens = torch.empty((n, k), dtype=torch.int64, device=dev)
-    out_done = torch.empty((n, k), dtype=torch.bool, device=dev)
+    size, stride, new = (n, k), (k, 1), torch.empty_strided
+    out_scores = new(size, stride, dtype=torch.float32, device=dev)
+    out_rows = new(size, stride, dtype=torch.int32, device=dev)
+    out_tokens = new(size, stride, dtype=torch.int64, device=dev)
+    out_done = new(size, stride, dtype=torch.bool, device=dev)
     L = _lib.lib()
     with _on(dev):
         nbytes = L.cats_beam_select_bytes(n, beams, vocab, k)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         st = L.cats_beam_select(logits.data_ptr(), ld, scores.data_ptr(), _ptr(done), n, beams, vocab, k, eos,
                                 dtype_code(logits.dtype), out_scores.data_ptr(), out_rows.data_ptr(),
-                                out_tokens.data_ptr(), out_done.data_ptr(), ws.data_ptr(), nbytes, _stream(dev))
+                                out_tokens.data_ptr(), out_done.data_ptr(), ws.data_ptr(), nbytes, _raw_stream(dev.index))
     if st:
         _lib.check(st, "cats_beam_select")
     return out_scores, out_rows, out_tokens, out_done

@@ -457,7 +457,7 @@ int cats_kv8_append(const cats_kv8* cache, int layer, const void* qkv, long long
  *   out [n_tokens, n_heads, head_dim]; ws: cats_kv8_attend_bytes(...) bytes of scratch, contents
  *   irrelevant before and after.
  */
-size_t cats_kv8_attend_bytes(const cats_kv8* cache, int n_tokens, int n_heads);
+size_t cats_kv8_attend_bytes(const cats_kv8* cache);
 int cats_kv8_attend(const cats_kv8* cache, int layer, const void* q, long long q_ld, const int* cu,
                     int n_tokens, int n_heads, float scale, void* out, void* ws, size_t ws_bytes,
                     int dtype, void* stream);
@@ -491,7 +491,7 @@ int cats_kv8_compact(const cats_kv8* cache, int* n_live, void* ws, size_t ws_byt
  * the token is eos.  Tokens at -inf come last; a beam whose score or log-sum-exp is not finite (a NaN
  * or +inf among its logits, all of them -inf) has only candidates at -inf.  The log-sum-exp is summed
  * in fp32 over at most a few thousand values and in fp64 above that; candidates are compared in fp64.
- *   beams <= 32, k <= 32, k <= beams * vocab.  ws: cats_beam_select_bytes(...) bytes of scratch.
+ *   beams <= 32, k <= 32, k <= beams * vocab, n * beams <= 65535.  ws: cats_beam_select_bytes(...) bytes of scratch.
  */
 size_t cats_beam_select_bytes(int n, int beams, int vocab, int k);
 int cats_beam_select(const void* logits, long long ld, const float* scores, const uint8_t* done, int n,
