@@ -54,17 +54,29 @@ cudaError_t append(const cats_kv8& c, int layer, const void* qkv, long long ld, 
   A.tokens = tokens;
   A.nh = nh;
   A.layer = layer;
+  // One new token of every sequence (a decode step): a warp per block of rows; else half a page's
+  // rows (a quarter of a 128-row page's) side by side, two (four) of them in a thread's registers.
+  const bool single = !cu && A.uniform == 1;
   const int tpr = c.head_dim / 16;
-  const int threads = (c.page / 4 * tpr + 31) / 32 * 32;
-  const int rows = threads / tpr * 4;
+  const int rpt = single ? 1 : c.page == 128 ? 4 : 2;
+  const int threads = single ? 32 : (c.page / rpt * tpr + 31) / 32 * 32;
   const long long units = cu ? (long long)tokens / c.page + 2LL * (tokens < c.n_seqs ? tokens : c.n_seqs)
                              : (long long)c.n_seqs * kv_units(A.uniform, c.page);
-  const long long kv_blocks = units * 2 * c.n_kv_heads;
-  const long long q_blocks = q_out ? ((long long)tokens * nh + rows - 1) / rows : 0;
+  // A CTA goes through several blocks of rows, the next one's loads under way, where that still leaves
+  // four CTAs per SM and more (finding the page costs as long as a block's load).
+  A.kv_heads = 1;
+  while (!single && A.kv_heads < 16 && units * 2 * c.n_kv_heads / (2 * A.kv_heads) >= 4LL * dev_info().sms) A.kv_heads *= 2;
+  const long long kv_blocks = units * ((2 * c.n_kv_heads + A.kv_heads - 1) / A.kv_heads);
+  // query CTAs: a thread keeps its token's rotation for as many heads as still leave work for all SMs
+  const long long tiles = (tokens + threads / tpr - 1) / (threads / tpr);
+  A.q_heads = tiles * ((nh + 15) / 16) >= 4LL * dev_info().sms ? 16 : 4;
+  const long long q_blocks = q_out ? tiles * ((nh + A.q_heads - 1) / A.q_heads) : 0;
   if (kv_blocks + q_blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-  A.units = (int)units;
   A.kv_blocks = (int)kv_blocks;
-  return launch(k_kv8_append<T>, dim3((unsigned)(kv_blocks + q_blocks)), dim3(threads), 0, st, c, A);
+  const dim3 grid((unsigned)(kv_blocks + q_blocks)), block(threads);
+  if (single) return launch(k_kv8_append<T, 1>, grid, block, 0, st, c, A);
+  if (rpt == 4) return launch(k_kv8_append<T, 4>, grid, block, 0, st, c, A);
+  return launch(k_kv8_append<T, 2>, grid, block, 0, st, c, A);
 }
 
 template <typename T>

@@ -9,12 +9,12 @@ namespace cats {
 // ---------------------------------------------------------------------------------------------
 // append: rotary embedding + quantising write
 // ---------------------------------------------------------------------------------------------
-// One CTA per (sequence, touched page, keys or values, head): the scale belongs to that block of
-// rows, so the CTA that takes the rows' largest magnitude is the one that writes them, and the new
-// rows are read once and stay in registers between the two (at most four rows of a thread: the
-// CTA has page / 4 rows side by side).  hd / 16 threads share a row; a thread holds eight values
-// of the row's first half and the eight that the rotation pairs them with.  The query heads are
-// rotated by further CTAs of the same launch.
+// One CTA per (sequence, touched page) and some of its blocks of rows (keys or values, head), one after
+// the other: a scale belongs to a block, so the CTA that takes the rows' largest magnitude is the one that writes them, and the new
+// rows are read once and stay in registers between the two (at most RPT rows of a thread).  hd / 16
+// threads share a row; a thread holds eight values of the row's first half and the eight that the
+// rotation pairs them with.  Further CTAs of the same launch rotate the queries: a thread keeps its
+// token's cosines and sines and goes through the heads, two of them on their way.
 // Rounding: products and sums of the rotation are each rounded to fp32 (no contraction), the query
 // once more to its type; keys and values go from fp32 straight to e4m3.  Infinities are stored as
 // NaN (e4m3 has none) and neither sets a scale.
@@ -26,76 +26,121 @@ struct KvAppendArgs {
   const T* sinv;
   T* q_out;               // [tokens, nh, hd] or nullptr
   const int* cu;
-  int uniform, tokens, nh, layer, units, kv_blocks;
+  int uniform, tokens, nh, layer, kv_blocks;
+  int kv_heads, q_heads;  // blocks of rows (keys' and values' heads) and query heads of a CTA
 };
 
-// f[0..8) and f[8..16) are the paired values of one head's halves at columns col and col + hd / 2
+// sixteen values as they lie in memory: columns col .. col + 8 and col + half .. col + half + 8
 template <typename T>
-__device__ __forceinline__ void rotate16(float* f, const T* c, const T* s, int col, int half) {
-  float c1[8], c2[8], s1[8], s2[8];
-  load8_cached(c + col, c1);
-  load8_cached(c + col + half, c2);
-  load8_cached(s + col, s1);
-  load8_cached(s + col + half, s2);
+struct Raw16 {
+  static constexpr int K = sizeof(T) / 2;
+  uint4 v[2 * K];
+  __device__ __forceinline__ void load(const T* p, int half) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float a = f[i], b = f[8 + i];
-    f[i] = __fadd_rn(__fmul_rn(a, c1[i]), __fmul_rn(-b, s1[i]));
-    f[8 + i] = __fadd_rn(__fmul_rn(b, c2[i]), __fmul_rn(a, s2[i]));
+    for (int k = 0; k < K; ++k) {
+      v[k] = ldg_stream(reinterpret_cast<const uint4*>(p) + k);
+      v[K + k] = ldg_stream(reinterpret_cast<const uint4*>(p + half) + k);
+    }
+  }
+  __device__ __forceinline__ void load_cached(const T* p, int half) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      v[k] = __ldg(reinterpret_cast<const uint4*>(p) + k);
+      v[K + k] = __ldg(reinterpret_cast<const uint4*>(p + half) + k);
+    }
+  }
+  __device__ __forceinline__ void unpack(float* f) const {
+#pragma unroll
+    for (int k = 0; k < 2 * K; ++k) VecT<T>::unpack(v[k], f + k * VecT<T>::N);
+  }
+};
+
+// A token's cosines and sines at sixteen columns.
+struct Turn {
+  float c[16], s[16];
+  template <typename T>
+  __device__ __forceinline__ void load(const T* cosv, const T* sinv, int half) {
+    Raw16<T> cr, sr;
+    cr.load_cached(cosv, half);
+    sr.load_cached(sinv, half);
+    cr.unpack(c);
+    sr.unpack(s);
+  }
+  __device__ __forceinline__ void apply(float* f) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float a = f[i], b = f[8 + i];
+      f[i] = __fadd_rn(__fmul_rn(a, c[i]), __fmul_rn(-b, s[i]));
+      f[8 + i] = __fadd_rn(__fmul_rn(b, c[8 + i]), __fmul_rn(a, s[8 + i]));
+    }
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void append_queries(const cats_kv8& c, const KvAppendArgs<T>& A, int block) {
+  const int hd = c.head_dim, half = hd >> 1, tpr = hd >> 4;
+  const int side = blockDim.x / tpr, r0 = threadIdx.x / tpr, col = (threadIdx.x - r0 * tpr) * 8;
+  const int chunks = (A.nh + A.q_heads - 1) / A.q_heads;
+  const int tile = block / chunks, h0 = (block - tile * chunks) * A.q_heads, h1 = min(h0 + A.q_heads, A.nh);
+  const int t = tile * side + r0;
+  if (r0 >= side || t >= A.tokens) return;
+  const T* src = A.qkv + (size_t)t * A.ld + col;
+  T* dst = A.q_out + (size_t)t * A.nh * hd + col;
+  constexpr int kAhead = 2;                              // heads on their way
+  Raw16<T> x[kAhead];
+  Turn rot;
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k)
+    if (h0 + k < h1) x[k].load(src + (size_t)(h0 + k) * hd, half);
+  bool turn = A.cosv != nullptr;
+  if (turn) {
+    int b;
+    if (!A.cu) {
+      b = t / A.uniform;
+    } else {                                             // last b with cu[b] <= t
+      int lo = 0, hi = c.n_seqs - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (__ldg(A.cu + mid) <= t) lo = mid;
+        else hi = mid - 1;
+      }
+      b = lo;
+    }
+    const KvSpan sp = kv_span(A.cu, A.uniform, b);
+    const int pos = c.lens[b] - sp.count + (t - sp.first);
+    turn = pos >= 0 && pos < c.max_pages * c.page;
+    if (turn) rot.load(A.cosv + (size_t)pos * hd + col, A.sinv + (size_t)pos * hd + col, half);
+    else kv_flag(c, KV_TOO_LONG);
+  }
+  for (int h = h0; h < h1; h += kAhead) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (h + k >= h1) continue;
+      float f[16];
+      x[k].unpack(f);
+      if (h + k + kAhead < h1) x[k].load(src + (size_t)(h + k + kAhead) * hd, half);
+      if (turn) rot.apply(f);
+      store8(dst + (size_t)(h + k) * hd, f);
+      store8(dst + (size_t)(h + k) * hd + half, f + 8);
+    }
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) k_kv8_append(const cats_kv8 c, const KvAppendArgs<T> A) {
+template <typename T, int RPT>
+__global__ void __launch_bounds__(RPT == 1 ? 32 : 256, RPT == 1 ? 16 : RPT == 2 ? 3 : 2) k_kv8_append(const cats_kv8 c, const KvAppendArgs<T> A) {
   pdl_wait();
-  __shared__ float s_max[8];
-  const int hd = c.head_dim, half = hd >> 1, tpr = hd >> 4, nkv = c.n_kv_heads;
-  const int rows_side = blockDim.x / tpr;
-  const int r0 = threadIdx.x / tpr, col = (threadIdx.x - r0 * tpr) * 8;
-  const int max_len = c.max_pages * c.page;
-  const bool on = r0 < rows_side;
-
-  if ((int)blockIdx.x >= A.kv_blocks) {               // query heads
-    const long long rows = (long long)A.tokens * A.nh;
-    const long long base = (long long)(blockIdx.x - A.kv_blocks) * rows_side * 4;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const long long r = base + k * rows_side + r0;
-      if (!on || r >= rows) continue;
-      const int t = (int)(r / A.nh), h = (int)(r - (long long)t * A.nh);
-      int b;
-      if (!A.cu) {
-        b = t / A.uniform;
-      } else {                                         // last b with cu[b] <= t
-        int lo = 0, hi = c.n_seqs - 1;
-        while (lo < hi) {
-          const int mid = (lo + hi + 1) >> 1;
-          if (__ldg(A.cu + mid) <= t) lo = mid;
-          else hi = mid - 1;
-        }
-        b = lo;
-      }
-      const KvSpan sp = kv_span(A.cu, A.uniform, b);
-      const int pos = c.lens[b] - sp.count + (t - sp.first);
-      T* dst = A.q_out + r * hd;
-      float f[16];
-      const T* src = A.qkv + (size_t)t * A.ld + (size_t)h * hd;
-      load8(src + col, f);
-      load8(src + col + half, f + 8);
-      if (A.cosv) {
-        if (pos >= 0 && pos < max_len)
-          rotate16(f, A.cosv + (size_t)pos * hd, A.sinv + (size_t)pos * hd, col, half);
-        else
-          kv_flag(c, KV_TOO_LONG);
-      }
-      store8(dst + col, f);
-      store8(dst + col + half, f + 8);
-    }
+  pdl_launch_dependents();
+  if ((int)blockIdx.x >= A.kv_blocks) {
+    append_queries(c, A, blockIdx.x - A.kv_blocks);
     return;
   }
-
-  const int unit = blockIdx.x / (2 * nkv), x = blockIdx.x - unit * 2 * nkv;
-  const int kv = x / nkv, head = x - kv * nkv;
+  __shared__ float s_max[8];
+  const int hd = c.head_dim, half = hd >> 1, tpr = hd >> 4, nkv = c.n_kv_heads;
+  const int side = blockDim.x / tpr;
+  const int r0 = threadIdx.x / tpr, col = (threadIdx.x - r0 * tpr) * 8;
+  const int max_len = c.max_pages * c.page;
+  const int chunks = (2 * nkv + A.kv_heads - 1) / A.kv_heads;
+  const int unit = blockIdx.x / chunks, x0 = (blockIdx.x - unit * chunks) * A.kv_heads, x1 = min(x0 + A.kv_heads, 2 * nkv);
   int b, j;                                            // sequence, and which of its touched pages
   if (!A.cu) {
     const int per = kv_units(A.uniform, c.page);
@@ -132,74 +177,110 @@ __global__ void __launch_bounds__(256) k_kv8_append(const cats_kv8 c, const KvAp
     if (threadIdx.x == 0) kv_flag(c, start < 0 || len > max_len ? KV_TOO_LONG : KV_BAD_SPAN);
     return;
   }
+  const int row0 = page_i * c.page;                    // position of the page's first row
+  const int first = max(start - row0, 0), last = min(len - row0, c.page);   // its new rows
+
+  // the first head's new rows and the page's number are on their way together; from then on the next
+  // head's rows while this one's are worked on
+  Raw16<T> raw[RPT];
+  const T* src = A.qkv + ((long long)sp.first + row0 - start) * A.ld + (size_t)A.nh * hd + col;
+  auto fetch = [&](int x) {
+#pragma unroll
+    for (int k = 0; k < RPT; ++k) {
+      const int r = first + k * side + r0;
+      if (r0 < side && r < last) raw[k].load(src + (long long)r * A.ld + (size_t)x * hd, half);
+    }
+  };
+  fetch(x0);
   const int page = c.table[(size_t)b * c.max_pages + page_i];
   // a page that another sequence holds too is never written
   if (page < 0 || page >= c.n_pages || c.refs[page] != 1) {
     if (threadIdx.x == 0) kv_flag(c, KV_BAD_PAGE);
     return;
   }
-  const int row0 = page_i * c.page;                    // position of the page's first row
-  const int first = max(start - row0, 0), last = min(len - row0, c.page);   // its new rows
-  const size_t head_off = (size_t)(A.nh + kv * nkv + head) * hd;
-
-  float f[4][16];
-  float amax = 0.f;
+  auto block_max = [&](float v) {
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int r = first + k * rows_side + r0;
-    if (!on || r >= last) continue;
-    const int pos = row0 + r;
-    const T* src = A.qkv + (size_t)(sp.first + pos - start) * A.ld + head_off;
-    load8(src + col, f[k]);
-    load8(src + col + half, f[k] + 8);
-    if (kv == 0 && A.cosv) rotate16(f[k], A.cosv + (size_t)pos * hd, A.sinv + (size_t)pos * hd, col, half);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const bool fin = (__float_as_uint(f[k][i]) & 0x7f800000u) != 0x7f800000u;
-      f[k][i] = fin ? f[k][i] : __uint_as_float(0x7fc00000u);
-      amax = fmaxf(amax, fabsf(f[k][i]));              // fmaxf drops the NaN
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if (RPT > 1) {
+      __syncthreads();
+      if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = v;
+      __syncthreads();
+      for (int w = 0; w < (int)(blockDim.x >> 5); ++w) v = fmaxf(v, s_max[w]);
     }
-  }
-  float* sc = kv_scale(c, A.layer, page, kv, head);
-  const int e_old = first > 0 ? kv_exp_of(*sc) : kKvExpMin;
+    return v;
+  };
+  for (int x = x0; x < x1; ++x) {
+    const bool turn = x < nkv && A.cosv != nullptr;
+    float f[RPT][16];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = amax;
-  __syncthreads();
-  for (int w = 0; w < (int)(blockDim.x >> 5); ++w) amax = fmaxf(amax, s_max[w]);
-  const int e = max(kv_exponent(amax), e_old);
-  const float inv = kv_pow2(-e);
-  uint8_t* rows = kv_rows(c, A.layer, page, kv, head);
+    for (int k = 0; k < RPT; ++k) {
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int r = first + k * rows_side + r0;
-    if (!on || r >= last) continue;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float* g = f[k] + 8 * h;
-      uint2 v;
-      v.x = e4m3x4(g[0] * inv, g[1] * inv, g[2] * inv, g[3] * inv);
-      v.y = e4m3x4(g[4] * inv, g[5] * inv, g[6] * inv, g[7] * inv);
-      *reinterpret_cast<uint2*>(rows + (size_t)r * hd + col + h * half) = v;
+      for (int i = 0; i < 16; ++i) f[k][i] = 0.f;
+      if (r0 < side && first + k * side + r0 < last) raw[k].unpack(f[k]);
     }
-  }
-  if (first > 0 && e > e_old) {                        // the older rows, at the new scale
-    const float down = kv_pow2(max(e_old - e, -126));
-    uint4* p = reinterpret_cast<uint4*>(rows);
-    for (int i = threadIdx.x; i < first * hd / 16; i += blockDim.x) {
-      uint4 v = p[i];
-      uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+    if (x + 1 < x1) fetch(x + 1);
+    float amax = 0.f;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t lo = e4m3_to_f16x2(w[k] & 0xffffu), hi = e4m3_to_f16x2(w[k] >> 16);
-        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo));
-        const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-        w[k] = e4m3x4(a.x * down, a.y * down, d.x * down, d.y * down);
+    for (int k = 0; k < RPT; ++k) {
+      const int r = first + k * side + r0;
+      if (r0 >= side || r >= last) continue;
+      if (turn) {
+        Turn rot;
+        rot.load(A.cosv + (size_t)(row0 + r) * hd + col, A.sinv + (size_t)(row0 + r) * hd + col, half);
+        rot.apply(f[k]);
       }
-      p[i] = v;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(f[k][i]));         // (drops NaN)
     }
+    float* sc = kv_scale(c, A.layer, page, 0, x);
+    const int e_old = first > 0 ? kv_exp_of(*sc) : kKvExpMin;
+    amax = block_max(amax);
+    if (amax > 3.402823466e38f) {                        // an infinity: a NaN from here on
+      amax = 0.f;
+#pragma unroll
+      for (int k = 0; k < RPT; ++k)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if (fabsf(f[k][i]) > 3.402823466e38f) f[k][i] = __uint_as_float(0x7fc00000u);
+          amax = fmaxf(amax, fabsf(f[k][i]));
+        }
+      amax = block_max(amax);
+    }
+    if (RPT == 1) __syncwarp();                          // every lane has read the old scale
+    const int e = max(kv_exponent(amax), e_old);
+    const float inv = kv_pow2(-e);
+    uint8_t* rows = kv_rows(c, A.layer, page, 0, x);
+#pragma unroll
+    for (int k = 0; k < RPT; ++k) {
+      const int r = first + k * side + r0;
+      if (r0 >= side || r >= last) continue;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float* g = f[k] + 8 * h;
+        uint2 v;
+        v.x = e4m3x4(g[0] * inv, g[1] * inv, g[2] * inv, g[3] * inv);
+        v.y = e4m3x4(g[4] * inv, g[5] * inv, g[6] * inv, g[7] * inv);
+        *reinterpret_cast<uint2*>(rows + (size_t)r * hd + col + h * half) = v;
+      }
+    }
+    if (first > 0 && e > e_old) {                        // the older rows, at the new scale
+      const float down = kv_pow2(max(e_old - e, -126));
+      uint4* p = reinterpret_cast<uint4*>(rows);
+      for (int i = threadIdx.x; i < first * hd / 16; i += blockDim.x) {
+        uint4 v = p[i];
+        uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t lo = e4m3_to_f16x2(w[k] & 0xffffu), hi = e4m3_to_f16x2(w[k] >> 16);
+          const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+          const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+          w[k] = e4m3x4(a.x * down, a.y * down, d.x * down, d.y * down);
+        }
+        p[i] = v;
+      }
+    }
+    if (threadIdx.x == 0) *sc = kv_pow2(e);
   }
-  if (threadIdx.x == 0) *sc = kv_pow2(e);
 }
 
 // ---------------------------------------------------------------------------------------------
