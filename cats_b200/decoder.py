@@ -18,6 +18,10 @@ from the model's weight tensors:
   out of the MLP kernel;
 * prefill runs the reference's rule for T > 1, the dense thresholded MLP
   (experiments/models/sparse_silu/ugly_utils.py:900-904);
+* ``cache="paged8"`` keeps keys and values in a paged 8-bit cache (``kv8.KVCache8``) instead: half
+  the memory and half the attention bytes of a token, attention by the library's own kernel over
+  exactly the cached positions (one graph for all positions), and ``beam_search``, whose beams
+  share pages;
 * ``mlp="dense"`` runs the same loop with the plain SiLU-gated MLP (cuBLAS), the baseline;
   ``mlp="masked"`` the dense thresholded MLP in PyTorch (``sp_method = 0``), the parity reference.
 
@@ -33,7 +37,7 @@ from typing import List, Optional
 import torch
 import torch.nn.functional as F
 
-from . import _lib, ops
+from . import _lib, kv8, ops
 
 BUCKET = 256
 
@@ -53,12 +57,17 @@ class CatsDecoder:
     ``MistralForCausalLM`` (or the Sparse* subclasses) that lives on one CUDA device.
 
     ``thresholds``: per-layer CATS thresholds; default: each layer's ``mlp.dead_threshold``.
+    ``cache``: "static" (16-bit, one buffer per layer) or "paged8" (8 bits, pages of ``page``
+    tokens, a pool of ``n_pages``; default: enough for ``batch`` sequences of ``max_len``).
     """
 
     def __init__(self, model, batch: int, max_len: int, mlp: str = "cats",
-                 thresholds: Optional[List[float]] = None):
+                 thresholds: Optional[List[float]] = None, cache: str = "static", page: int = 64,
+                 n_pages: Optional[int] = None):
         if mlp not in ("cats", "dense", "masked"):
             raise RuntimeError(f"cats_b200.decoder: unknown mlp mode {mlp!r}")
+        if cache not in ("static", "paged8"):
+            raise RuntimeError(f"cats_b200.decoder: unknown cache {cache!r}")
         cfg = model.config
         self.model, self.mode = model, mlp
         self.B, self.max_len = batch, (max_len + BUCKET - 1) // BUCKET * BUCKET
@@ -93,8 +102,14 @@ class CatsDecoder:
         self.cos, self.sin = (embd.cos() * scale).to(self.dt), (embd.sin() * scale).to(self.dt)
 
         z = lambda *s, dt=self.dt: torch.zeros(s, dtype=dt, device=self.dev)
-        self.kc = z(self.L, batch, self.nkv, self.max_len, self.hd)
-        self.vc = z(self.L, batch, self.nkv, self.max_len, self.hd)
+        self.kv = None
+        if cache == "paged8":
+            per_seq = (self.max_len + page - 1) // page
+            self.kv = kv8.KVCache8(self.L, n_pages or batch * per_seq, batch, self.max_len, self.nkv, self.hd,
+                                   page, self.dev)
+        else:
+            self.kc = z(self.L, batch, self.nkv, self.max_len, self.hd)
+            self.vc = z(self.L, batch, self.nkv, self.max_len, self.hd)
         self.tok = z(batch, dt=torch.int64)
         self.pos = z(1, dt=torch.int64)                 # cache position of the token in self.tok
         self.h = z(batch, self.H)                       # residual stream of the current token
@@ -126,6 +141,9 @@ class CatsDecoder:
     def _attn_decode(self, l: int, x: torch.Tensor, bucket: int, cos, sin, mask) -> torch.Tensor:
         B, nh, nkv, hd = self.B, self.nh, self.nkv, self.hd
         qkv = F.linear(x, self.wqkv[l])
+        if self.kv is not None:
+            q = self.kv.append(l, qkv, nh, self.cos, self.sin, q_out=self.q)
+            return F.linear(self.kv.attend(l, q).view(B, nh * hd), self.wo[l])
         if self.dev.type == "cuda":
             # RoPE + cache write in one launch (cats_rope_cache) instead of a dozen
             q = self.q
@@ -177,15 +195,18 @@ class CatsDecoder:
             self.x.copy_(_rmsnorm(self.h, nw, self.eps))
 
     @torch.no_grad()
-    def _step(self, bucket: int) -> None:
-        """One decode step on device state: consumes self.tok at self.pos, leaves the next token
-        in self.tok and advances self.pos."""
+    def _forward(self, bucket: int) -> None:
+        """The tokens in self.tok through the decoder: leaves their logits in self.logits."""
         self.h.copy_(self.embed.index_select(0, self.tok))
         self.x.copy_(_rmsnorm(self.h, self.ln1[0], self.eps))
         # position-dependent pieces once per step, not once per layer
-        cos, sin = self.cos.index_select(0, self.pos), self.sin.index_select(0, self.pos)  # [1, hd]
-        mask = torch.where(self.ar[:bucket] <= self.pos, 0.0, float("-inf")).to(self.dt)
-        mask = mask.view(1, 1, 1, bucket)
+        cos = sin = mask = None
+        if self.kv is not None:
+            self.kv.grow(1)
+        else:
+            cos, sin = self.cos.index_select(0, self.pos), self.sin.index_select(0, self.pos)  # [1, hd]
+            mask = torch.where(self.ar[:bucket] <= self.pos, 0.0, float("-inf")).to(self.dt)
+            mask = mask.view(1, 1, 1, bucket)
         for l in range(self.L):
             a = self._attn_decode(l, self.x, bucket, cos, sin, mask)
             if self.dev.type == "cuda":
@@ -197,6 +218,12 @@ class CatsDecoder:
                 self.x2.copy_(_rmsnorm(self.h, self.ln2[l], self.eps))
             self._mlp_tail(l)
         torch.matmul(self.x, self.lm_head.t(), out=self.logits)
+
+    @torch.no_grad()
+    def _step(self, bucket: int) -> None:
+        """One decode step on device state: consumes self.tok at self.pos, leaves the next token
+        in self.tok and advances self.pos."""
+        self._forward(bucket)
         self.tok.copy_(self.logits.argmax(-1))
         self.pos.add_(1)
 
@@ -208,7 +235,21 @@ class CatsDecoder:
         "dense"), as the reference's module does for prefill."""
         B, T = input_ids.shape
         assert B == self.B and T < self.max_len
+        logits = self._prefill(input_ids, 1)
+        self.tok.copy_(logits.argmax(-1))
+        return logits
+
+    def _prefill(self, input_ids: torch.Tensor, every: int) -> torch.Tensor:
+        """The prompts into every ``every``-th sequence of the cache (the others stay empty)."""
+        B, T = input_ids.shape
         nh, nkv, hd = self.nh, self.nkv, self.hd
+        cu = None
+        if self.kv is not None:
+            self.kv.reset()
+            if every > 1:
+                first = torch.arange(self.B + 1, device=self.dev, dtype=torch.int32)
+                cu = (first + every - 1).div(every, rounding_mode="floor").mul_(T).to(torch.int32)
+            self.kv.grow(T, cu=cu)
         h = self.embed[input_ids]                                     # [B, T, H]
         cos, sin = self.cos[:T].view(1, 1, T, hd), self.sin[:T].view(1, 1, T, hd)
         for l in range(self.L):
@@ -220,8 +261,12 @@ class CatsDecoder:
             v = v.view(B, T, nkv, hd).transpose(1, 2)
             q = q * cos + _rotate_half(q) * sin
             k = k * cos + _rotate_half(k) * sin
-            self.kc[l][:, :, :T] = k
-            self.vc[l][:, :, :T] = v
+            if self.kv is not None:
+                # (the prompt's own attention below reads the keys and values as they are)
+                self.kv.append(l, qkv.view(B * T, -1), nh, self.cos, self.sin, cu=cu, queries=False)
+            else:
+                self.kc[l][:, :, :T] = k
+                self.vc[l][:, :, :T] = v
             o = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=nh != nkv)
             h = h + F.linear(o.transpose(1, 2).reshape(B, T, nh * hd), self.wo[l])
             x2 = _rmsnorm(h, self.ln2[l], self.eps)
@@ -230,13 +275,14 @@ class CatsDecoder:
                 p = torch.where(p.abs() <= self.thr[l], torch.zeros_like(p), p)
             h = h + F.linear(p * F.linear(x2, self.wu[l]), self.wd[l])
         logits = F.linear(_rmsnorm(h[:, -1], self.final_norm, self.eps), self.lm_head)
-        self.tok.copy_(logits.argmax(-1))
         self.pos.fill_(T)
         self.n_pos = T
         return logits
 
     # ---- decode -----------------------------------------------------------------------------------
     def _bucket(self, n_pos: int) -> int:
+        if self.kv is not None:
+            return self.max_len                # attention reads the cached positions only
         return min(self.max_len, (n_pos + 1 + BUCKET - 1) // BUCKET * BUCKET)
 
     @torch.no_grad()
@@ -244,23 +290,35 @@ class CatsDecoder:
         """Record the decode step into CUDA graphs, one per cache bucket that positions
         first_pos..last_pos touch.  Runs two eager steps first (library warm-up) and restores the
         state they changed; capturing itself executes nothing."""
-        keep = (self.tok.clone(), self.pos.clone(), self.h.clone(), self.x.clone())
+        self._capture(sorted({self._bucket(p) for p in range(first_pos, last_pos + 1)}), first_pos, self._step)
+
+    def _capture(self, keys, first_pos: int, step) -> None:
+        """``step(key)`` into ``self.graphs[key]``, for every key that is not there yet."""
+        state = [self.tok, self.pos, self.h, self.x]
+        keep = [t.clone() for t in state]
+        kv = self.kv
         side = torch.cuda.Stream(self.dev)
         side.wait_stream(torch.cuda.current_stream(self.dev))
         with torch.cuda.stream(side):
             self.pos.fill_(min(first_pos, self.max_len - 3))
+            if kv is not None:
+                # the warm-up's tokens go into a cache of their own: rows that leave a page again may
+                # have raised its scale
+                self.kv = kv8.KVCache8(self.L, self.B, self.B, kv.page, self.nkv, self.hd, kv.page, self.dev)
             for _ in range(2):
-                self._step(self._bucket(first_pos))
+                step(keys[0])
+            self.kv = kv
         torch.cuda.current_stream(self.dev).wait_stream(side)
         torch.cuda.synchronize(self.dev)
-        for b in sorted({self._bucket(p) for p in range(first_pos, last_pos + 1)}):
-            if b in self.graphs:
+        for k in keys:
+            if k in self.graphs:
                 continue
             g = torch.cuda.CUDAGraph()
             with torch.cuda.graph(g):
-                self._step(b)
-            self.graphs[b] = g
-        self.tok.copy_(keep[0]); self.pos.copy_(keep[1]); self.h.copy_(keep[2]); self.x.copy_(keep[3])
+                step(k)
+            self.graphs[k] = g
+        for t, v in zip(state, keep):
+            t.copy_(v)
         torch.cuda.synchronize(self.dev)
 
     @torch.no_grad()
@@ -292,6 +350,75 @@ class CatsDecoder:
         dt_ms = t0.elapsed_time(t1)
         tps = (n_tokens - 1) * self.B / (dt_ms * 1e-3) if n_tokens > 1 and dt_ms > 0 else float("nan")
         return torch.stack(toks, 1), tps, logs
+
+    # ---- beam search ------------------------------------------------------------------------------
+    @torch.no_grad()
+    def beam_search(self, input_ids: torch.Tensor, beams: int, n_tokens: int, eos: Optional[int] = None,
+                    length_penalty: float = 1.0, use_graph: bool = True):
+        """Beam search over ``input_ids`` (P, T) with ``cache="paged8"`` and P * beams == batch: every
+        step picks the ``beams`` best of beams x vocabulary by summed log-probability
+        (``ops.beam_select``); the beams' caches follow by sharing pages (``KVCache8.reorder``).  A beam
+        that has produced ``eos`` keeps its score and its place.  Returns (tokens (P, beams, n_tokens),
+        ``eos`` behind the end; scores (P, beams), summed log-probability over length **
+        length_penalty), best first.  Steps run on the device alone; nothing is read back."""
+        if self.kv is None:
+            raise RuntimeError('cats_b200.decoder: beam search needs cache="paged8"')
+        P, T = input_ids.shape
+        if beams < 1 or P * beams != self.B:
+            raise RuntimeError(f"cats_b200.decoder: {P} prompts x {beams} beams do not make the batch of {self.B}")
+        if n_tokens < 1 or T + n_tokens > self.max_len:
+            raise RuntimeError("cats_b200.decoder: the KV cache is too short for this many tokens")
+        end = -1 if eos is None else int(eos)
+        if eos is not None and not 0 <= end < self.logits.shape[1]:
+            raise RuntimeError(f"cats_b200.decoder: eos {end} is not a token of the vocabulary")
+        logits = self._prefill(input_ids, beams)
+        scores, rows, toks, done = ops.beam_select(logits.view(P, 1, -1), torch.zeros((P, 1), device=self.dev), beams,
+                                                   eos=end)
+        self.tok.copy_(toks.view(-1))
+        history = [(None, toks.clone())]
+        first = torch.arange(self.B, device=self.dev, dtype=torch.int32)
+        self.kv.reorder(first.div(beams, rounding_mode="floor").mul_(beams).to(torch.int32))
+        state = (scores, done, torch.empty_like(scores, dtype=torch.int32), toks)
+
+        def step(_key):
+            scores, done, rows, toks = state
+            self._forward(self.max_len)
+            s, r, t, d = ops.beam_select(self.logits.view(P, beams, -1), scores, beams,
+                                         done=done if eos is not None else None, eos=end)
+            self.kv.reorder(r.view(-1))
+            for to, what in zip(state, (s, d, r, t)):
+                to.copy_(what)
+            self.tok.copy_(t.view(-1))
+
+        key = ("beam", P, beams, end)
+        if use_graph and n_tokens > 1:
+            keep = [t.clone() for t in state]
+            self.graphs.pop(key, None)         # a graph holds its own state tensors
+            self._capture([key], T, step)
+            for t, v in zip(state, keep):
+                t.copy_(v)
+        for _ in range(n_tokens - 1):
+            if use_graph:
+                self.graphs[key].replay()
+            else:
+                step(key)
+            history.append((state[2].clone(), state[3].clone()))
+        self.n_pos = T + n_tokens - 1
+        # from the last step back along the parents
+        out = []
+        row = torch.arange(self.B, device=self.dev).view(P, beams)
+        for parents, toks in reversed(history):
+            out.append(toks.view(-1)[row])
+            if parents is not None:
+                row = parents.view(-1)[row].long()
+        tokens = torch.stack(out[::-1], -1)
+        lengths = torch.full((P, beams), n_tokens, device=self.dev)
+        if eos is not None:
+            ended = (tokens == end).int().cumsum(-1) > 0
+            lengths = (n_tokens + 1 - ended.sum(-1)).clamp(max=n_tokens)
+        final = state[0] / lengths.to(torch.float32) ** length_penalty
+        order = final.argsort(dim=-1, descending=True, stable=True)
+        return tokens.gather(1, order[..., None].expand_as(tokens)), final.gather(1, order)
 
 
 # ---- model construction (random init: there are no checkpoints offline) ---------------------------

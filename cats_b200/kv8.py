@@ -138,12 +138,12 @@ class KVCache8:
 
     def append(self, layer: int, qkv: torch.Tensor, n_heads: int, cos: Optional[torch.Tensor] = None,
                sin: Optional[torch.Tensor] = None, cu: Optional[torch.Tensor] = None,
-               q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+               q_out: Optional[torch.Tensor] = None, queries: bool = True) -> Optional[torch.Tensor]:
         """Rotary embedding of the newest tokens' queries and keys and the quantising cache write
         (``cats_kv8_append``).  qkv (tokens, (n_heads + 2 kv_heads) head_dim), rows may be strided;
         cos, sin (>= max_len, head_dim), or None for no rotation; ``cu`` int32 (seqs + 1): first row of
         every sequence, or None for the same number of rows each.  Returns the queries (tokens,
-        n_heads, head_dim)."""
+        n_heads, head_dim); with ``queries=False`` only keys and values are dealt with."""
         n = self._tokens(qkv, "qkv", cu)
         hd, dt = self.head_dim, qkv.dtype
         code = _DTYPES[dt] if dt in _DTYPES else dtype_code(dt)
@@ -165,7 +165,9 @@ class KVCache8:
             if rope < self.max_len:
                 raise _bad(f"cos and sin hold {rope} positions, the cache up to {self.max_len}")
             pc, ps = cos.data_ptr(), sin.data_ptr()
-        if q_out is None:
+        if not queries:
+            q_out = None
+        elif q_out is None:
             q_out = torch.empty_strided((n, n_heads, hd), (n_heads * hd, hd, 1), dtype=dt, device=self.device)
         elif q_out.dtype != dt or q_out.device != self.device or not q_out.is_contiguous() \
                 or q_out.numel() != n * n_heads * hd:
@@ -173,7 +175,7 @@ class KVCache8:
         if n == 0:
             return q_out
         self._call("cats_kv8_append", layer, qkv.data_ptr(), qkv.stride(0) if n > 1 else qkv.shape[1], self._cu(cu), n,
-                   pc, ps, rope, q_out.data_ptr(), n_heads, code)
+                   pc, ps, rope, None if q_out is None else q_out.data_ptr(), n_heads, code)
         return q_out
 
     def attend(self, layer: int, q: torch.Tensor, cu: Optional[torch.Tensor] = None,
@@ -241,6 +243,12 @@ class KVCache8:
         ws = torch.empty(self._compact_nbytes, dtype=torch.uint8, device=self.device)
         self._call("cats_kv8_compact", n.data_ptr(), ws.data_ptr(), self._compact_nbytes)
         return n
+
+    def reset(self) -> None:
+        """All sequences empty, all pages free."""
+        self.table.fill_(-1)
+        self.lens.zero_()
+        self.refs.zero_()
 
     # ---- host side ---------------------------------------------------------------------------------------------
     def check(self) -> None:
