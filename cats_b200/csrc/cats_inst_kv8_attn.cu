@@ -25,7 +25,11 @@ template <typename T, int HD>
 static cudaError_t run_attend(const cats_kv8& c, const KvAttnArgs<T>& A, cudaStream_t st) {
   // rows of a key head: (new tokens) x (query heads per key head), on average over the sequences
   const long long rows = ((long long)A.tokens + c.n_seqs - 1) / c.n_seqs * (A.nh / c.n_kv_heads);
-  return rows <= 8 ? run_attend<T, HD, 1>(c, A, st) : run_attend<T, HD, 2>(c, A, st);
+  if (rows <= 8) return run_attend<T, HD, 1>(c, A, st);
+  if constexpr (sizeof(T) == 2) {                       // (fp32 queries are two halves: no room)
+    if (rows > 16) return run_attend<T, HD, 4>(c, A, st);
+  }
+  return run_attend<T, HD, 2>(c, A, st);
 }
 
 template <typename T>

@@ -35,7 +35,9 @@ constexpr float kAttnSlack = 8.f;                       // see the running maxim
 
 // NQ columns of eight rows ((token, query head of the group) pairs) per tile.  Eight rows leave room
 // for 16 warps of 128 registers, which hide the latency of the chain load - convert - multiply -
-// exponential - multiply best; 16 rows need twice the accumulators.
+// exponential - multiply best; 16 rows need twice the accumulators; 32 rows (many new tokens: the
+// conversions are shared by four products) leave no registers for the queries, which are read from
+// shared memory then.
 template <int NQ>
 struct AttnShape {
   static constexpr int kRows = 8 * NQ;
@@ -43,6 +45,7 @@ struct AttnShape {
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kStages = NQ == 1 ? 3 : 6;       // tiles a warp has in its ring (one of them in use)
   static constexpr int kUnit = kWarps * kAttnTile;      // positions of a unit
+  static constexpr bool kQueriesShared = NQ == 4;
 };
 
 template <typename T>
@@ -57,11 +60,12 @@ struct KvAttnArgs {
   float scale;            // of the scores, times log2(e)
 };
 
-constexpr int kAttnMaxRows = 16;
+constexpr int kAttnMaxRows = 32;
 __host__ __device__ inline size_t attn_part_floats(int rows, int hd) { return (size_t)rows * (hd + 2); }
 template <int NQ>
 constexpr size_t attn_smem() {
-  return 128 + (size_t)AttnShape<NQ>::kWarps * (AttnShape<NQ>::kStages * (kAttnStageBytes + 16) + 2 * 8 * sizeof(float));
+  return 128 + (size_t)AttnShape<NQ>::kWarps * (AttnShape<NQ>::kStages * (kAttnStageBytes + 16) + 2 * 8 * sizeof(float)) +
+         (AttnShape<NQ>::kQueriesShared ? NQ * 128 / 32 * 32 * sizeof(uint4) : 0);
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -312,6 +316,7 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
   unsigned char* after = smem + (size_t)S::kWarps * S::kStages * kAttnStageBytes;
   float4* meta = reinterpret_cast<float4*>(after) + warp * S::kStages;   // scales of keys and values, rows
   float* s_ml = reinterpret_cast<float*>(after + (size_t)S::kWarps * S::kStages * 16);
+  uint4* s_q = reinterpret_cast<uint4*>(s_ml + S::kWarps * 16);         // [HD / 32][NQ][32 lanes], where shared
   const uint32_t ring_u32 = (uint32_t)__cvta_generic_to_shared(ring);
   const uint32_t meta_u32 = (uint32_t)__cvta_generic_to_shared(meta);
 
@@ -410,7 +415,7 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
   const uint32_t v3_off = HD % 64 ? kAttnTile * 128 + attn_swizzle(2 * t + 1, HD / 64 * 64 + 4 * g) : 0;
 
   // ---- consumer: S^T = K Q^T, so a lane has rows (columns) 2 t and 2 t + 1 of each group of eight ----
-  uint32_t qa[KS][NQ][2], qb[SPLIT ? KS : 1][NQ][2];
+  uint32_t qa[S::kQueriesShared ? 1 : KS][NQ][2], qb[SPLIT ? KS : 1][NQ][2];
   float o[MT][NQ][4];
   float m[NQ][2], l[NQ][2], f[NQ][2];
   int lim[NQ][2], lim_min = 0;                           // positions that a row sees, and the least of them
@@ -460,21 +465,32 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
         for (int p = 0; p < HD / 32; ++p)
 #pragma unroll
           for (int k = 0; k < 8; ++k) q[p][k] *= inv;
+        if (S::kQueriesShared) {                         // the same for all warps: each writes its share
 #pragma unroll
-        for (int p = 0; p < HD / 32; ++p)
+          for (int p = 0; p < HD / 32; ++p)
+            if ((p * NQ + n) % S::kWarps == warp)
+              s_q[(p * NQ + n) * 32 + lane] = make_uint4(half2_bits(q[p][0], q[p][1]), half2_bits(q[p][2], q[p][3]),
+                                                         half2_bits(q[p][4], q[p][5]), half2_bits(q[p][6], q[p][7]));
+        } else {
 #pragma unroll
-          for (int e2 = 0; e2 < 2; ++e2)
+          for (int p = 0; p < HD / 32; ++p)
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const float* v = q[p] + 4 * e2 + 2 * x;
-              qa[2 * p + e2][n][x] = half2_bits(v[0], v[1]);
-              if (SPLIT) qb[SPLIT ? 2 * p + e2 : 0][n][x] = half2_rest(v[0], v[1], qa[2 * p + e2][n][x]);
-            }
+            for (int e2 = 0; e2 < 2; ++e2)
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const float* v = q[p] + 4 * e2 + 2 * x;
+                constexpr int last = S::kQueriesShared ? 0 : KS - 1;
+                uint32_t& to = qa[2 * p + e2 < last ? 2 * p + e2 : last][n][x];
+                to = half2_bits(v[0], v[1]);
+                if (SPLIT) qb[SPLIT ? 2 * p + e2 : 0][n][x] = half2_rest(v[0], v[1], to);
+              }
+        }
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
           for (int x = 0; x < 4; ++x) o[i][n][x] = 0.f;
       }
+      if (S::kQueriesShared) __syncthreads();            // (all warps are at the same unit)
     }
 
     const int kb = at.unit * S::kUnit + warp * kAttnTile;
@@ -491,15 +507,29 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
       for (int p = 0; p < HD / 32; ++p) {
         const uint32_t ka = (st + k_off) ^ (32 * p);
         const uint2 k0 = lds2(ka), k1 = lds2(ka + 1024);
+        uint32_t a[2][4];
 #pragma unroll
         for (int e2 = 0; e2 < 2; ++e2) {
           const uint32_t x0 = e2 ? k0.y : k0.x, x1 = e2 ? k1.y : k1.x;
-          const uint32_t a[4] = {e4m3_to_f16x2(x0 & 0xffffu), e4m3_to_f16x2(x1 & 0xffffu), e4m3_to_f16x2(x0 >> 16),
-                                 e4m3_to_f16x2(x1 >> 16)};
+          a[e2][0] = e4m3_to_f16x2(x0 & 0xffffu);
+          a[e2][1] = e4m3_to_f16x2(x1 & 0xffffu);
+          a[e2][2] = e4m3_to_f16x2(x0 >> 16);
+          a[e2][3] = e4m3_to_f16x2(x1 >> 16);
+        }
 #pragma unroll
-          for (int n = 0; n < NQ; ++n) {
-            mma16816(s[n], a, qa[2 * p + e2][n][0], qa[2 * p + e2][n][1]);
-            if (SPLIT) mma16816(s[n], a, qb[SPLIT ? 2 * p + e2 : 0][n][0], qb[SPLIT ? 2 * p + e2 : 0][n][1]);
+        for (int n = 0; n < NQ; ++n) {
+          if (S::kQueriesShared) {
+            const uint4 q = s_q[(p * NQ + n) * 32 + lane];
+            mma16816(s[n], a[0], q.x, q.y);
+            mma16816(s[n], a[1], q.z, q.w);
+          } else {
+#pragma unroll
+            for (int e2 = 0; e2 < 2; ++e2) {
+              constexpr int last = S::kQueriesShared ? 0 : KS - 1;
+              const int k = 2 * p + e2 < last ? 2 * p + e2 : last;
+              mma16816(s[n], a[e2], qa[k][n][0], qa[k][n][1]);
+              if (SPLIT) mma16816(s[n], a[e2], qb[SPLIT ? k : 0][n][0], qb[SPLIT ? k : 0][n][1]);
+            }
           }
         }
       }

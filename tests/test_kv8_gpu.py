@@ -142,23 +142,34 @@ def test_scores_of_any_size(cuda_device):
     attend_and_compare(c, [2, 1], 2, torch.float32)
 
 
-def test_what_lies_behind_a_token_does_not_reach_it(cuda_device):
+@pytest.mark.parametrize("dt,heads", [("f32", 4), ("f16", 2), ("bf16", 4), ("bf16", 2)])
+def test_what_lies_behind_a_token_does_not_reach_it(dt, heads, cuda_device):
     """NaN values (and keys) of the later tokens of the same call: the earlier rows stay what they are."""
     for where in (0, 1):
-        c = filled(cuda_device, [50, 90], 32, 2, 64)
-        counts = [20, 33]
-        clean = c.attend(0, torch.ones((53, 4, 64), device=cuda_device), cu=cu_of(counts, cuda_device))
-        page = int(c.table[0, 45 // 32])
-        c.codes.view(torch.uint8)[0, page, where, 1, 45 % 32, 7] = 127          # position 45, head 1
-        got = c.attend(0, torch.ones((53, 4, 64), device=cuda_device), cu=cu_of(counts, cuda_device))
-        first = 45 - 30                                                        # the row at position 45
-        hit = torch.zeros_like(got, dtype=torch.bool)
-        if where == 0:
-            hit[first:20, 2:4] = True                                          # its score is NaN: the whole row
-        else:
-            hit[first:20, 2:4, 7] = True
-        assert torch.equal(got.isnan(), hit)
-        assert torch.equal(got[~hit], clean[~hit])
+        for counts in ([20, 33], [20, 3]):                                     # many rows per key head, few
+            c = filled(cuda_device, [50, 60 + counts[1]], 32, 2, 64)
+            q = torch.ones((sum(counts), heads, 64), device=cuda_device, dtype=TYPES[dt])
+            clean = c.attend(0, q, cu=cu_of(counts, cuda_device))
+            page = int(c.table[0, 45 // 32])
+            c.codes.view(torch.uint8)[0, page, where, 1, 45 % 32, 7] = 127     # position 45, key head 1
+            got = c.attend(0, q, cu=cu_of(counts, cuda_device))
+            first = 45 - 30                                                    # the row at position 45
+            hit = torch.zeros_like(got, dtype=torch.bool)
+            if where == 0:
+                hit[first:20, heads // 2:] = True                              # its score is NaN: the whole row
+            else:
+                hit[first:20, heads // 2:, 7] = True
+            assert torch.equal(got.isnan(), hit)
+            assert torch.equal(got[~hit], clean[~hit])
+
+
+def test_one_new_token_behind_stale_nan_rows(cuda_device):
+    """Rows of a sequence's last page behind its length hold NaN codes (see ``filled``): two tokens of
+    eight rows, in the tile with the end of the sequence."""
+    for dt in TYPES.values():
+        c = filled(cuda_device, [33, 47, 5], 64, 1, 64)
+        attend_and_compare(c, [2, 2, 2], 4, dt)
+        attend_and_compare(c, [3, 1, 4], 2, dt)
 
 
 def test_empty_sequences_give_zeros_and_bad_ids_are_reported(cuda_device):
