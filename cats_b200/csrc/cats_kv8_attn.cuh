@@ -45,6 +45,7 @@ struct AttnShape {
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kStages = NQ == 1 ? 3 : 6;       // tiles a warp has in its ring (one of them in use)
   static constexpr int kUnit = kWarps * kAttnTile;      // positions of a unit
+  static constexpr int kJoin = 512 / kUnit;             // joining parts takes about as long as 512 positions
   static constexpr bool kQueriesShared = NQ == 4;
 };
 
@@ -104,6 +105,7 @@ __device__ __forceinline__ uint32_t attn_swizzle(int row, uint32_t byte) {
 // What the CTA knows of the sequences (shared memory).
 struct AttnTable {
   int pre[kKvMaxSeqs + 1];                              // units before sequence b; all of them
+  int ctas[kKvMaxSeqs + 1];                             // CTAs before sequence b, where they are dealt out by segments
   int len[kKvMaxSeqs], first[kKvMaxSeqs], count[kKvMaxSeqs];
 };
 struct AttnSeq {
@@ -116,43 +118,109 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnTable& tab, int b, int gro
   s.units = (s.len + AttnShape<NQ>::kUnit - 1) / AttnShape<NQ>::kUnit;
   return s;
 }
-// Fills the table (called by all threads; ends with a barrier) and zeroes the rows of the sequences
-// that hold nothing.  A sequence whose length or span does not fit counts as one of those.
-template <int NQ, int HD, typename T>
-__device__ __forceinline__ void attn_table(const cats_kv8& c, const KvAttnArgs<T>& A, AttnTable& tab, int* s_warp) {
-  constexpr int kThreads = AttnShape<NQ>::kThreads, kPer = kKvMaxSeqs / kThreads;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = A.nh / c.n_kv_heads;
-  int mine[kPer], sum = 0;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int b = threadIdx.x * kPer + i;
-    mine[i] = 0;
-    if (b < c.n_seqs) {
-      const KvSpan sp = kv_span(A.cu, A.uniform, b);
-      int len = c.lens[b], first = sp.first, count = sp.count;
-      const bool long_ok = len >= 0 && len <= c.max_pages * c.page;
-      const bool span_ok = first >= 0 && (long long)first + count <= A.tokens;
-      if (count > 0 && !(long_ok && span_ok)) {
-        if (blockIdx.x == 0) kv_flag(c, long_ok ? KV_BAD_SPAN : KV_TOO_LONG);
-        len = 0;
-        const long long end = min((long long)first + count, (long long)A.tokens);
-        first = max(first, 0);
-        count = (int)max(end - first, 0LL);
-      }
-      tab.len[b] = len;
-      tab.first[b] = first;
-      tab.count[b] = count;
-      const AttnSeq s = attn_seq<NQ>(tab, b, group);
-      mine[i] = s.units * s.tiles * c.n_kv_heads;
-    }
-    sum += mine[i];
+// How the units are dealt out to the CTAs.
+// By segments ((head, tile)s of a sequence), when there are no more of them than CTAs: every segment
+// gets one CTA and a part of the spare ones by its length, and no CTA has two.  Otherwise in equal
+// shares of the row of all units, whose borders give way to a segment's border that is next to them
+// while shares are short.  A unit takes 1.3 us, joining parts 2.7 us and a second segment in a CTA
+// 3.7 us (measured, head_dim 128): equal shares, where a CTA mostly has two segments and joins one, win
+// only where dealing out by segments makes the largest share that much larger (measured: 64 segments
+// of 1024 positions 16.7 us in equal shares, 12.1 us by segments).
+struct AttnPlan {
+  int total, ctas, spare;                               // units, CTAs with a share; spare < 0: equal shares
+};
+// CTAs of a segment: one and its part of the spare ones, or one where the others do not bring more
+// than the joining costs.
+template <int NQ>
+__device__ __forceinline__ int attn_pieces(const AttnPlan& p, int units) {
+  const int n = min(1 + (int)((float)units * (float)p.spare / (float)p.total), units);
+  return (units + n - 1) / n + AttnShape<NQ>::kJoin >= units ? 1 : n;
+}
+// the time of a segment's CTA, in units
+template <int NQ>
+__device__ __forceinline__ int attn_load(int units, int pieces) {
+  return (units + pieces - 1) / pieces + (pieces > 1 ? AttnShape<NQ>::kJoin : 0);
+}
+template <int NQ>
+__device__ __forceinline__ AttnPlan attn_equal(int total, int ctas) {
+  return {total, min(total, ctas), -1};
+}
+template <int NQ>
+__device__ __forceinline__ bool attn_by_segments(int largest, int dealt, int total, int ctas) {
+  // (`dealt` can be one or two too many where a quotient was rounded up)
+  return dealt <= ctas && largest <= total / ctas + AttnShape<NQ>::kJoin * 5 / 2;
+}
+
+// Sequence b into the table; its units and segments.  A sequence whose length or span does not fit
+// counts as one that holds nothing.
+template <int NQ, typename T>
+__device__ __forceinline__ AttnSeq attn_enter(const cats_kv8& c, const KvAttnArgs<T>& A, AttnTable& tab, int b, int group) {
+  const KvSpan sp = kv_span(A.cu, A.uniform, b);
+  int len = c.lens[b], first = sp.first, count = sp.count;
+  const bool long_ok = len >= 0 && len <= c.max_pages * c.page;
+  const bool span_ok = first >= 0 && (long long)first + count <= A.tokens;
+  if (count > 0 && !(long_ok && span_ok)) {
+    if (blockIdx.x == 0) kv_flag(c, long_ok ? KV_BAD_SPAN : KV_TOO_LONG);
+    len = 0;
+    const long long end = min((long long)first + count, (long long)A.tokens);
+    first = max(first, 0);
+    count = (int)max(end - first, 0LL);
   }
+  if (len < 0) len = 0;
+  tab.len[b] = len;
+  tab.first[b] = first;
+  tab.count[b] = count;
+  return attn_seq<NQ>(tab, b, group);
+}
+
+// Up to 32 sequences: one warp, a lane each, no barrier in between.
+template <int NQ, typename T>
+__device__ __forceinline__ AttnPlan attn_plan_warp(const cats_kv8& c, const KvAttnArgs<T>& A, AttnTable& tab, int group) {
+  const int lane = threadIdx.x & 31;
+  AttnSeq s = {0, 0, 0, 0, 0};
+  if (lane < c.n_seqs) s = attn_enter<NQ>(c, A, tab, lane, group);
+  auto scan = [&](int v) {
+    int incl = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += u;
+    }
+    return incl;
+  };
+  const int segments = s.units ? s.tiles * c.n_kv_heads : 0, mine = s.units * segments;
+  const int incl = scan(mine), total = __shfl_sync(0xffffffffu, incl, 31);
+  if (lane < c.n_seqs) tab.pre[lane + 1] = incl;
+  if (lane == 0) tab.pre[0] = 0;
+  const int all = __reduce_add_sync(0xffffffffu, segments);
+  if (all <= A.ctas && total > 0) {
+    AttnPlan plan = {total, 0, A.ctas - all};
+    const int n = segments ? attn_pieces<NQ>(plan, s.units) : 0;
+    const int ctas = scan(n * segments);
+    if (lane < c.n_seqs) tab.ctas[lane + 1] = ctas;
+    if (lane == 0) tab.ctas[0] = 0;
+    plan.ctas = __shfl_sync(0xffffffffu, ctas, 31);
+    const int largest = __reduce_max_sync(0xffffffffu, n ? attn_load<NQ>(s.units, n) : 0);
+    if (attn_by_segments<NQ>(largest, plan.ctas, total, A.ctas)) return plan;
+  }
+  return attn_equal<NQ>(total, A.ctas);
+}
+
+// Exclusive scan over the values that the threads hold for their sequences; all of them together.
+template <int THREADS>
+__device__ __forceinline__ int attn_scan(const int* mine, int* pre, int n_seqs, int* s_warp) {
+  constexpr int kPer = kKvMaxSeqs / THREADS;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int sum = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) sum += mine[i];
   int incl = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
+  __syncthreads();                                      // s_warp may still be read
   if (lane == 31) s_warp[warp] = incl;
   __syncthreads();
   int before = incl - sum;
@@ -160,17 +228,89 @@ __device__ __forceinline__ void attn_table(const cats_kv8& c, const KvAttnArgs<T
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int b = threadIdx.x * kPer + i;
-    if (b <= c.n_seqs) tab.pre[b] = before;
+    if (b <= n_seqs) pre[b] = before;
     before += mine[i];
   }
-  if (threadIdx.x == kThreads - 1 && c.n_seqs == kKvMaxSeqs) tab.pre[kKvMaxSeqs] = before;
+  if (threadIdx.x == THREADS - 1 && n_seqs == kKvMaxSeqs) pre[kKvMaxSeqs] = before;
   __syncthreads();
+  return pre[n_seqs];
+}
+// Any number of sequences: all threads.
+template <int NQ, typename T>
+__device__ __forceinline__ AttnPlan attn_plan_block(const cats_kv8& c, const KvAttnArgs<T>& A, AttnTable& tab, int group,
+                                                    int* s_warp) {
+  constexpr int kThreads = AttnShape<NQ>::kThreads, kPer = kKvMaxSeqs / kThreads;
+  int mine[kPer], segments = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int b = threadIdx.x * kPer + i;
+    mine[i] = 0;
+    if (b < c.n_seqs) {
+      const AttnSeq s = attn_enter<NQ>(c, A, tab, b, group);
+      mine[i] = s.units * s.tiles * c.n_kv_heads;
+      if (s.units) segments += s.tiles * c.n_kv_heads;
+    }
+  }
+  const int total = attn_scan<kThreads>(mine, tab.pre, c.n_seqs, s_warp);
+  // (the threads' numbers go through the same words as the scan's)
+  auto all_of = [&](int v, bool sum) {
+    v = sum ? __reduce_add_sync(0xffffffffu, v) : __reduce_max_sync(0xffffffffu, v);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) s_warp[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0;
+    for (int w = 0; w < kThreads / 32; ++w) v = sum ? v + s_warp[w] : max(v, s_warp[w]);
+    return v;
+  };
+  const int all = all_of(segments, true);
+  if (all <= A.ctas && total > 0) {
+    AttnPlan plan = {total, 0, A.ctas - all};
+    int largest = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int b = threadIdx.x * kPer + i;
+      mine[i] = 0;
+      if (b < c.n_seqs) {
+        const AttnSeq s = attn_seq<NQ>(tab, b, group);
+        if (s.units && s.tiles) {
+          const int n = attn_pieces<NQ>(plan, s.units);
+          mine[i] = n * s.tiles * c.n_kv_heads;
+          largest = max(largest, attn_load<NQ>(s.units, n));
+        }
+      }
+    }
+    plan.ctas = attn_scan<kThreads>(mine, tab.ctas, c.n_seqs, s_warp);
+    largest = all_of(largest, false);
+    if (attn_by_segments<NQ>(largest, plan.ctas, total, A.ctas)) return plan;
+  }
+  return attn_equal<NQ>(total, A.ctas);
+}
+
+// The plan and its table (called by all threads; ends with a barrier); zeroes the rows of the
+// sequences that hold nothing.
+template <int NQ, int HD, typename T>
+__device__ __forceinline__ AttnPlan attn_table(const cats_kv8& c, const KvAttnArgs<T>& A, AttnTable& tab, AttnPlan* s_plan,
+                                               int* s_warp) {
+  constexpr int kThreads = AttnShape<NQ>::kThreads;
+  const int group = A.nh / c.n_kv_heads;
+  AttnPlan plan;
+  if (c.n_seqs <= 32) {
+    if (threadIdx.x < 32) {
+      plan = attn_plan_warp<NQ>(c, A, tab, group);
+      if (threadIdx.x == 0) *s_plan = plan;
+    }
+    __syncthreads();
+    plan = *s_plan;
+  } else {
+    plan = attn_plan_block<NQ>(c, A, tab, group, s_warp);
+  }
   for (int b = blockIdx.x; b < c.n_seqs; b += gridDim.x) {
     if (tab.pre[b + 1] != tab.pre[b] || tab.count[b] == 0) continue;
     T* dst = A.out + (size_t)tab.first[b] * A.nh * HD;
     const size_t n = (size_t)tab.count[b] * A.nh * HD;
     for (size_t k = threadIdx.x; k < n; k += kThreads) dst[k] = VecT<T>::from_f(0.f);
   }
+  return plan;
 }
 
 // Where a unit lies: sequence, head, tile and number of the unit within them.
@@ -191,17 +331,55 @@ __device__ __forceinline__ AttnPlace attn_place(const AttnTable& tab, int n_seqs
   p.b = lo;
   const int at = r / s.units;
   p.unit = r - at * s.units;
-  p.head = at / s.tiles;
+  p.head = s.tiles == 1 ? at : at / s.tiles;
   p.tile = at - p.head * s.tiles;
   *seq = s;
   return p;
 }
-// CTAs that get a share (at least one unit each), and where the share of CTA c begins
-__device__ __forceinline__ int attn_ctas(int total, int ctas) { return min(total, ctas); }
-__device__ __forceinline__ int attn_share(int total, int c, int ctas) { return (int)((long long)total * c / ctas); }
-// the CTA whose share holds unit w
-__device__ __forceinline__ int attn_owner(int total, int w, int ctas) {
-  return (int)((((long long)w + 1) * ctas - 1) / total);
+// Where the share of CTA c begins.
+template <int NQ>
+__device__ __forceinline__ int attn_share(const AttnTable& tab, const AttnPlan& p, int n_seqs, int group, int c) {
+  if (p.spare >= 0) {
+    if (c >= p.ctas) return p.total;
+    int lo = 0, hi = n_seqs - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (tab.ctas[mid] <= c) lo = mid;
+      else hi = mid - 1;
+    }
+    const AttnSeq s = attn_seq<NQ>(tab, lo, group);
+    const int n = attn_pieces<NQ>(p, s.units), r = c - tab.ctas[lo], seg = r / n, piece = r - seg * n;
+    const int q = s.units / n;
+    return tab.pre[lo] + seg * s.units + q * piece + min(piece, s.units - q * n);
+  }
+  if (c >= p.ctas) return p.total;
+  const int q = p.total / p.ctas, w = q * c + (int)((unsigned)(p.total - q * p.ctas) * (unsigned)c / (unsigned)p.ctas);
+  constexpr int kNear = 256 / AttnShape<NQ>::kUnit;
+  if (q >= 8 * kNear) return w;
+  AttnSeq s;
+  const AttnPlace at = attn_place<NQ>(tab, n_seqs, group, w, &s);
+  if (at.unit <= kNear) return w - at.unit;
+  if (s.units - at.unit <= kNear) return w + s.units - at.unit;
+  return w;
+}
+// The CTAs that have units u0 (a segment's first) and u0 + units - 1.
+template <int NQ>
+__device__ __forceinline__ void attn_owners(const AttnTable& tab, const AttnPlan& p, int n_seqs, int group, int b, int u0,
+                                            int units, int* c0, int* c1) {
+  if (p.spare >= 0) {
+    const int n = attn_pieces<NQ>(p, units);
+    *c0 = tab.ctas[b] + (u0 - tab.pre[b]) / units * n;
+    *c1 = *c0 + n - 1;
+    return;
+  }
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int w = x ? u0 + units - 1 : u0;
+    int c = min((int)((float)w * (float)p.ctas / (float)p.total), p.ctas - 1);
+    while (c > 0 && attn_share<NQ>(tab, p, n_seqs, group, c) > w) --c;
+    while (c + 1 < p.ctas && attn_share<NQ>(tab, p, n_seqs, group, c + 1) <= w) ++c;
+    *(x ? c1 : c0) = c;
+  }
 }
 __device__ __forceinline__ uint2 lds2(uint32_t addr) {
   uint2 v;
@@ -309,6 +487,7 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
   __shared__ AttnTable s_tab;
   __shared__ int s_warp[S::kWarps];
   __shared__ int s_last;
+  __shared__ AttnPlan s_plan;
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -320,12 +499,12 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
   const uint32_t ring_u32 = (uint32_t)__cvta_generic_to_shared(ring);
   const uint32_t meta_u32 = (uint32_t)__cvta_generic_to_shared(meta);
 
-  attn_table<NQ, HD>(c, A, s_tab, s_warp);
-  const int total = s_tab.pre[c.n_seqs], ctas = attn_ctas(total, A.ctas);
-  if ((int)blockIdx.x >= ctas) return;
-  const int share0 = attn_share(total, blockIdx.x, ctas);
-  const int n_units = attn_share(total, blockIdx.x + 1, ctas) - share0;
+  const AttnPlan plan = attn_table<NQ, HD>(c, A, s_tab, &s_plan, s_warp);
+  if ((int)blockIdx.x >= plan.ctas) return;
   const int group = A.nh / c.n_kv_heads;
+  const int share0 = attn_share<NQ>(s_tab, plan, c.n_seqs, group, blockIdx.x);
+  const int n_units = attn_share<NQ>(s_tab, plan, c.n_seqs, group, blockIdx.x + 1) - share0;
+  if (n_units <= 0) return;
 
   // ---- loader: lane i of the warp knows where unit `base + i` lies and which page its tile is in --
   int d_rows = 0, d_scale = 0;                           // rows to load; the keys' scale in its layer
@@ -424,10 +603,6 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
   bool first_seg = true, begins_here = at.unit == 0, fresh = true;
   int stage = 0;
   for (int u = 0; u < n_units; ++u) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
-    __syncwarp();
-    issue();
-
     if (fresh) {                                         // a new (sequence, head, tile): its queries
       fresh = false;
       const int rows = min(S::kRows, seq.count * group - at.tile * S::kRows);
@@ -492,6 +667,9 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
       }
       if (S::kQueriesShared) __syncthreads();            // (all warps are at the same unit)
     }
+    asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
+    __syncwarp();
+    issue();
 
     const int kb = at.unit * S::kUnit + warp * kAttnTile;
     unsigned char* kt = ring + stage * kAttnStageBytes;
@@ -659,10 +837,18 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
           float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
           for (int x = 0; x < S::kWarps; ++x) top = fmaxf(top, s_ml[x * 16 + r]);
+          const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll 4
           for (int x = 0; x < S::kWarps; ++x) {
-            attn_add(s_ml[x * 16 + r], s_ml[x * 16 + 8 + r],
-                     *reinterpret_cast<const float4*>(src + x * (pitch / sizeof(float))), top, sum, v);
+            const float mx = s_ml[x * 16 + r], lx = s_ml[x * 16 + 8 + r];
+            if (mx == -INFINITY && lx == 0.f) continue;  // saw nothing (a NaN sum goes on)
+            const float by = ex2(mx - ref);
+            const float4 w = *reinterpret_cast<const float4*>(src + x * (pitch / sizeof(float)));
+            sum = fmaf(lx, by, sum);
+            v.x = fmaf(w.x, by, v.x);
+            v.y = fmaf(w.y, by, v.y);
+            v.z = fmaf(w.z, by, v.z);
+            v.w = fmaf(w.w, by, v.w);
           }
           if (whole) {
             attn_store(A, seq, at, group, S::kRows, 8 * n + r, d, HD, sum, v);
@@ -679,9 +865,11 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
         // The CTA that brings the last part of a (head, tile) joins them all, in the order of the
         // CTAs.  The counter belongs to the CTA that has the first part (at most one of its
         // segments goes on in the next CTA) and is left at zero.
-        const int u0 = share0 + u + 1 - at.unit, c0 = attn_owner(total, u0, ctas), c1 = attn_owner(total, u0 + seq.units - 1, ctas);
+        const int u0 = share0 + u + 1 - at.unit;
         __threadfence();
         __syncthreads();
+        int c0, c1;
+        attn_owners<NQ>(s_tab, plan, c.n_seqs, group, at.b, u0, seq.units, &c0, &c1);
         if (threadIdx.x == 0) s_last = atomicAdd(A.counters + c0, 1) == c1 - c0;
         __syncthreads();
         if (s_last) {
@@ -689,6 +877,7 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
           __threadfence();
           // `sets` threads share a (row, four channels), each takes every sets-th part
           const int items = rows * (HD / 4), sets = max(1, min(S::kThreads / items, c1 - c0 + 1));
+          const int first_begins = attn_share<NQ>(s_tab, plan, c.n_seqs, group, c0);
           float* s_set = reinterpret_cast<float*>(kt - ring + smem);       // [warps] x a stage: six floats a thread
           for (int e0 = 0; e0 < items; e0 += S::kThreads) {
             const int e = sets > 1 ? threadIdx.x % items : e0 + threadIdx.x, set = sets > 1 ? threadIdx.x / items : 0;
@@ -698,7 +887,7 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
               const int r = e / (HD / 4), d = (e - r * (HD / 4)) * 4;
 #pragma unroll 4
               for (int x = c0 + set; x <= c1; x += sets) {
-                const int slot = attn_share(total, x, ctas) >= u0 ? 0 : 1;
+                const int slot = x > c0 || first_begins >= u0 ? 0 : 1;     // only c0 can have another segment first
                 const float* src = A.parts + (size_t)(2 * x + slot) * attn_part_floats(S::kRows, HD) + (size_t)r * (HD + 2);
                 const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + HD));
                 const float2 a = __ldcg(reinterpret_cast<const float2*>(src + d)), b = __ldcg(reinterpret_cast<const float2*>(src + d + 2));
