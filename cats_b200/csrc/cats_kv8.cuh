@@ -67,6 +67,13 @@ __device__ __forceinline__ uint32_t e4m3_to_f16x2(uint32_t two) {
   return r;
 }
 
+// four e4m3 codes -> two f16x2 (codes 0, 1 and 2, 3), exact
+__device__ __forceinline__ void e4m3x4_to_f16x2(uint32_t four, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(four));
+}
+
 // New tokens of sequence b: [first, first + count) of the packed tokens.  cu == nullptr: every
 // sequence has `uniform` of them.
 struct KvSpan {

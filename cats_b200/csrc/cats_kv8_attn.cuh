@@ -408,15 +408,15 @@ __device__ __forceinline__ void attn_pv(float (*o)[NQ][4], const uint32_t (*p)[2
                            __byte_perm(r2, r3, 0x7362)};
 #pragma unroll
     for (int j = 0; j < 2; ++j) {                        // channels 2 j, 2 j + 1: rows g and g + 8 of a tile
-      uint32_t a[4] = {w[2 * j] & 0xffffu, w[2 * j] >> 16, w[2 * j + 1] & 0xffffu, w[2 * j + 1] >> 16};
+      uint32_t a[4], x = w[2 * j], y = w[2 * j + 1];
       if (GUARD) {
+        auto nan_bytes = [](uint32_t v) { return ((((v & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu; };
+        const uint32_t nx = nan_bytes(x), ny = nan_bytes(y);
         uint32_t ind[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const uint32_t n = ((((a[x] & 0x7f7fu) + 0x0101u) & 0x8080u) >> 7) * 0xffu;   // 0xff where NaN
-          a[x] &= ~n;
-          ind[x] = e4m3_to_f16x2(n & 0x3838u);                                          // 0x38 is 1.0
-        }
+        e4m3x4_to_f16x2(nx & 0x38383838u, ind[0], ind[1]);   // 0x38 is 1.0
+        e4m3x4_to_f16x2(ny & 0x38383838u, ind[2], ind[3]);
+        x &= ~nx;
+        y &= ~ny;
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
           float hit[4] = {0.f, 0.f, 0.f, 0.f};
@@ -426,8 +426,8 @@ __device__ __forceinline__ void attn_pv(float (*o)[NQ][4], const uint32_t (*p)[2
             if (hit[i] > 0.f) acc[j][n][i] = __uint_as_float(0x7fc00000u);
         }
       }
-#pragma unroll
-      for (int x = 0; x < 4; ++x) a[x] = e4m3_to_f16x2(a[x]);
+      e4m3x4_to_f16x2(x, a[0], a[1]);
+      e4m3x4_to_f16x2(y, a[2], a[3]);
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
         mma16816(acc[j][n], a, p[n][0], p[n][1]);
@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
   unsigned char* smem = smem_raw + ((128 - ((uint32_t)__cvta_generic_to_shared(smem_raw) & 127)) & 127);
   __shared__ AttnTable s_tab;
   __shared__ int s_warp[S::kWarps];
-  __shared__ int s_last;
+  __shared__ int s_last, s_owners[2];
   __shared__ AttnPlan s_plan;
   pdl_wait();
   pdl_launch_dependents();
@@ -689,10 +689,8 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
 #pragma unroll
         for (int e2 = 0; e2 < 2; ++e2) {
           const uint32_t x0 = e2 ? k0.y : k0.x, x1 = e2 ? k1.y : k1.x;
-          a[e2][0] = e4m3_to_f16x2(x0 & 0xffffu);
-          a[e2][1] = e4m3_to_f16x2(x1 & 0xffffu);
-          a[e2][2] = e4m3_to_f16x2(x0 >> 16);
-          a[e2][3] = e4m3_to_f16x2(x1 >> 16);
+          e4m3x4_to_f16x2(x0, a[e2][0], a[e2][2]);
+          e4m3x4_to_f16x2(x1, a[e2][1], a[e2][3]);
         }
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
@@ -868,12 +866,14 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
         const int u0 = share0 + u + 1 - at.unit;
         __threadfence();
         __syncthreads();
-        int c0, c1;
-        attn_owners<NQ>(s_tab, plan, c.n_seqs, group, at.b, u0, seq.units, &c0, &c1);
-        if (threadIdx.x == 0) s_last = atomicAdd(A.counters + c0, 1) == c1 - c0;
+        if (threadIdx.x == 0) {
+          attn_owners<NQ>(s_tab, plan, c.n_seqs, group, at.b, u0, seq.units, &s_owners[0], &s_owners[1]);
+          s_last = atomicAdd(A.counters + s_owners[0], 1) == s_owners[1] - s_owners[0];
+          if (s_last) A.counters[s_owners[0]] = 0;
+        }
         __syncthreads();
         if (s_last) {
-          if (threadIdx.x == 0) A.counters[c0] = 0;
+          const int c0 = s_owners[0], c1 = s_owners[1];
           __threadfence();
           // `sets` threads share a (row, four channels), each takes every sets-th part
           const int items = rows * (HD / 4), sets = max(1, min(S::kThreads / items, c1 - c0 + 1));
