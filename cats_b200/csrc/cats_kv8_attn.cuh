@@ -46,6 +46,7 @@ struct AttnShape {
   static constexpr int kStages = NQ == 1 ? 3 : 6;       // tiles a warp has in its ring (one of them in use)
   static constexpr int kUnit = kWarps * kAttnTile;      // positions of a unit
   static constexpr int kJoin = 512 / kUnit;             // joining parts takes about as long as 512 positions
+  static constexpr int kSwitch = 768 / kUnit;           // going over to another segment, as long as 768
   static constexpr bool kQueriesShared = NQ == 4;
 };
 
@@ -105,7 +106,8 @@ __device__ __forceinline__ uint32_t attn_swizzle(int row, uint32_t byte) {
 // What the CTA knows of the sequences (shared memory).
 struct AttnTable {
   int pre[kKvMaxSeqs + 1];                              // units before sequence b; all of them
-  int ctas[kKvMaxSeqs + 1];                             // CTAs before sequence b, where they are dealt out by segments
+  int cost[kKvMaxSeqs + 1];                             // CTAs before sequence b where they are dealt out by
+                                                        // segments, else the cost (below) of what is before it
   int len[kKvMaxSeqs], first[kKvMaxSeqs], count[kKvMaxSeqs];
 };
 struct AttnSeq {
@@ -120,14 +122,16 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnTable& tab, int b, int gro
 }
 // How the units are dealt out to the CTAs.
 // By segments ((head, tile)s of a sequence), when there are no more of them than CTAs: every segment
-// gets one CTA and a part of the spare ones by its length, and no CTA has two.  Otherwise in equal
-// shares of the row of all units, whose borders give way to a segment's border that is next to them
-// while shares are short.  A unit takes 1.3 us, joining parts 2.7 us and a second segment in a CTA
+// gets one CTA and a part of the spare ones by its length, and no CTA has two.  Otherwise in shares of
+// the row of all units that cost the same, counting kSwitch units for every segment (its queries, the
+// join of its warps: a batch of uneven lengths took 130 us with shares of as many units each, since
+// some CTAs had a dozen short segments); a share's border gives way to a segment's border that is
+// next to it while shares are short.  A unit takes 1.3 us, joining parts 2.7 us and a second segment in a CTA
 // 3.7 us (measured, head_dim 128): equal shares, where a CTA mostly has two segments and joins one, win
 // only where dealing out by segments makes the largest share that much larger (measured: 64 segments
 // of 1024 positions 16.7 us in equal shares, 12.1 us by segments).
 struct AttnPlan {
-  int total, ctas, spare;                               // units, CTAs with a share; spare < 0: equal shares
+  int total, ctas, spare;                               // units (equal shares: their cost), CTAs; spare < 0: equal shares
 };
 // CTAs of a segment: one and its part of the spare ones, or one where the others do not bring more
 // than the joining costs.
@@ -140,10 +144,6 @@ __device__ __forceinline__ int attn_pieces(const AttnPlan& p, int units) {
 template <int NQ>
 __device__ __forceinline__ int attn_load(int units, int pieces) {
   return (units + pieces - 1) / pieces + (pieces > 1 ? AttnShape<NQ>::kJoin : 0);
-}
-template <int NQ>
-__device__ __forceinline__ AttnPlan attn_equal(int total, int ctas) {
-  return {total, min(total, ctas), -1};
 }
 template <int NQ>
 __device__ __forceinline__ bool attn_by_segments(int largest, int dealt, int total, int ctas) {
@@ -197,13 +197,17 @@ __device__ __forceinline__ AttnPlan attn_plan_warp(const cats_kv8& c, const KvAt
     AttnPlan plan = {total, 0, A.ctas - all};
     const int n = segments ? attn_pieces<NQ>(plan, s.units) : 0;
     const int ctas = scan(n * segments);
-    if (lane < c.n_seqs) tab.ctas[lane + 1] = ctas;
-    if (lane == 0) tab.ctas[0] = 0;
+    if (lane < c.n_seqs) tab.cost[lane + 1] = ctas;
+    if (lane == 0) tab.cost[0] = 0;
     plan.ctas = __shfl_sync(0xffffffffu, ctas, 31);
     const int largest = __reduce_max_sync(0xffffffffu, n ? attn_load<NQ>(s.units, n) : 0);
     if (attn_by_segments<NQ>(largest, plan.ctas, total, A.ctas)) return plan;
   }
-  return attn_equal<NQ>(total, A.ctas);
+  const int cost = scan(segments * (s.units + AttnShape<NQ>::kSwitch));
+  if (lane < c.n_seqs) tab.cost[lane + 1] = cost;
+  if (lane == 0) tab.cost[0] = 0;
+  const int whole = __shfl_sync(0xffffffffu, cost, 31);
+  return {whole, min(total, A.ctas), -1};
 }
 
 // Exclusive scan over the values that the threads hold for their sequences; all of them together.
@@ -279,11 +283,21 @@ __device__ __forceinline__ AttnPlan attn_plan_block(const cats_kv8& c, const KvA
         }
       }
     }
-    plan.ctas = attn_scan<kThreads>(mine, tab.ctas, c.n_seqs, s_warp);
+    plan.ctas = attn_scan<kThreads>(mine, tab.cost, c.n_seqs, s_warp);
     largest = all_of(largest, false);
     if (attn_by_segments<NQ>(largest, plan.ctas, total, A.ctas)) return plan;
   }
-  return attn_equal<NQ>(total, A.ctas);
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int b = threadIdx.x * kPer + i;
+    mine[i] = 0;
+    if (b < c.n_seqs) {
+      const AttnSeq s = attn_seq<NQ>(tab, b, group);
+      if (s.units) mine[i] = s.tiles * c.n_kv_heads * (s.units + AttnShape<NQ>::kSwitch);
+    }
+  }
+  const int whole = attn_scan<kThreads>(mine, tab.cost, c.n_seqs, s_warp);
+  return {whole, min(total, A.ctas), -1};
 }
 
 // The plan and its table (called by all threads; ends with a barrier); zeroes the rows of the
@@ -313,18 +327,23 @@ __device__ __forceinline__ AttnPlan attn_table(const cats_kv8& c, const KvAttnAr
   return plan;
 }
 
+// the last sequence that begins at or before x
+__device__ __forceinline__ int attn_find(const int* pre, int n_seqs, int x) {
+  int lo = 0, hi = n_seqs - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (pre[mid] <= x) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
 // Where a unit lies: sequence, head, tile and number of the unit within them.
 struct AttnPlace {
   int b, head, tile, unit;
 };
 template <int NQ>
 __device__ __forceinline__ AttnPlace attn_place(const AttnTable& tab, int n_seqs, int group, int w, AttnSeq* seq) {
-  int lo = 0, hi = n_seqs - 1;                           // last sequence that starts at or before w
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (tab.pre[mid] <= w) lo = mid;
-    else hi = mid - 1;
-  }
+  const int lo = attn_find(tab.pre, n_seqs, w);
   const AttnSeq s = attn_seq<NQ>(tab, lo, group);
   const int r = w - tab.pre[lo];
   AttnPlace p;
@@ -336,46 +355,44 @@ __device__ __forceinline__ AttnPlace attn_place(const AttnTable& tab, int n_seqs
   *seq = s;
   return p;
 }
-// Where the share of CTA c begins.
+// Where the share of CTA c begins, as a unit.
 template <int NQ>
 __device__ __forceinline__ int attn_share(const AttnTable& tab, const AttnPlan& p, int n_seqs, int group, int c) {
+  if (c >= p.ctas) return tab.pre[n_seqs];
   if (p.spare >= 0) {
-    if (c >= p.ctas) return p.total;
-    int lo = 0, hi = n_seqs - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (tab.ctas[mid] <= c) lo = mid;
-      else hi = mid - 1;
-    }
-    const AttnSeq s = attn_seq<NQ>(tab, lo, group);
-    const int n = attn_pieces<NQ>(p, s.units), r = c - tab.ctas[lo], seg = r / n, piece = r - seg * n;
-    const int q = s.units / n;
-    return tab.pre[lo] + seg * s.units + q * piece + min(piece, s.units - q * n);
+    const int b = attn_find(tab.cost, n_seqs, c);
+    const AttnSeq s = attn_seq<NQ>(tab, b, group);
+    const int n = attn_pieces<NQ>(p, s.units), r = c - tab.cost[b], seg = r / n, piece = r - seg * n, q = s.units / n;
+    return tab.pre[b] + seg * s.units + q * piece + min(piece, s.units - q * n);
   }
-  if (c >= p.ctas) return p.total;
+  // (shares cost at least one unit each and differ)
   const int q = p.total / p.ctas, w = q * c + (int)((unsigned)(p.total - q * p.ctas) * (unsigned)c / (unsigned)p.ctas);
+  const int b = attn_find(tab.cost, n_seqs, w);
+  const AttnSeq s = attn_seq<NQ>(tab, b, group);
+  const int each = s.units + AttnShape<NQ>::kSwitch, r = w - tab.cost[b], seg = r / each;
+  int unit = max(r - seg * each - AttnShape<NQ>::kSwitch, 0);
   constexpr int kNear = 256 / AttnShape<NQ>::kUnit;
-  if (q >= 8 * kNear) return w;
-  AttnSeq s;
-  const AttnPlace at = attn_place<NQ>(tab, n_seqs, group, w, &s);
-  if (at.unit <= kNear) return w - at.unit;
-  if (s.units - at.unit <= kNear) return w + s.units - at.unit;
-  return w;
+  if (q < 12 * kNear) {
+    if (unit <= kNear) unit = 0;
+    else if (s.units - unit <= kNear) unit = s.units;
+  }
+  return tab.pre[b] + seg * s.units + unit;
 }
 // The CTAs that have units u0 (a segment's first) and u0 + units - 1.
 template <int NQ>
 __device__ __forceinline__ void attn_owners(const AttnTable& tab, const AttnPlan& p, int n_seqs, int group, int b, int u0,
                                             int units, int* c0, int* c1) {
+  const int seg = (u0 - tab.pre[b]) / units;
   if (p.spare >= 0) {
     const int n = attn_pieces<NQ>(p, units);
-    *c0 = tab.ctas[b] + (u0 - tab.pre[b]) / units * n;
+    *c0 = tab.cost[b] + seg * n;
     *c1 = *c0 + n - 1;
     return;
   }
-#pragma unroll
+  const int each = units + AttnShape<NQ>::kSwitch;
   for (int x = 0; x < 2; ++x) {
-    const int w = x ? u0 + units - 1 : u0;
-    int c = min((int)((float)w * (float)p.ctas / (float)p.total), p.ctas - 1);
+    const int w = x ? u0 + units - 1 : u0, at = tab.cost[b] + seg * each + (x ? each - 1 : 0);
+    int c = min((int)((float)at * (float)p.ctas / (float)p.total), p.ctas - 1);
     while (c > 0 && attn_share<NQ>(tab, p, n_seqs, group, c) > w) --c;
     while (c + 1 < p.ctas && attn_share<NQ>(tab, p, n_seqs, group, c + 1) <= w) ++c;
     *(x ? c1 : c0) = c;
@@ -713,9 +730,9 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
       const float evf = (float)ev, vi = kv_pow2(-ev);
       const bool cut = kb + kAttnTile > lim_min;         // some row does not see all of the tile
       uint32_t p[NQ][2], pl[NQ][2];
+      float top[NQ][2];
 #pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        float top[2];
+      for (int n = 0; n < NQ; ++n)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {                    // s[x], s[2 + x]: positions g, g + 8 of row 2 t + x
           const float by = sc.x * f[n][x];
@@ -725,22 +742,31 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
             if (kb + g >= lim[n][x]) s[n][x] = -INFINITY;
             if (kb + 8 + g >= lim[n][x]) s[n][2 + x] = -INFINITY;
           }
-          top[x] = fmaxf(s[n][x], s[n][2 + x]);
+          top[n][x] = fmaxf(s[n][x], s[n][2 + x]);
         }
 #pragma unroll
-        for (int w = 4; w < 32; w <<= 1) {
-          top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], w));
-          top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], w));
+      for (int w = 4; w < 32; w <<= 1)
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) top[n][x] = fmaxf(top[n][x], __shfl_xor_sync(0xffffffffu, top[n][x], w));
+      // The reference m of the weights follows the running maximum only when that is more than
+      // 2^kAttnSlack ahead: weights up to 256 do half precision no harm, and the accumulators are
+      // rescaled a few times per sequence instead of at every second tile.
+      bool ahead = false;
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          top[n][x] += evf;
+          ahead |= top[n][x] > m[n][x] + kAttnSlack;
         }
-        top[0] += evf;
-        top[1] += evf;
-        // The reference m of the weights follows the running maximum only when that is more than
-        // 2^kAttnSlack ahead: weights up to 256 do half precision no harm, and the accumulators are
-        // rescaled a few times per sequence instead of at every second tile.
-        if (__any_sync(0xffffffffu, top[0] > m[n][0] + kAttnSlack || top[1] > m[n][1] + kAttnSlack)) {
+      if (__any_sync(0xffffffffu, ahead)) {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            const float to = fmaxf(top[x], m[n][x]), by = m[n][x] == -INFINITY ? 0.f : ex2(m[n][x] - to);
+            const float to = fmaxf(top[n][x], m[n][x]), by = m[n][x] == -INFINITY ? 0.f : ex2(m[n][x] - to);
             m[n][x] = to;
             l[n][x] *= by;
 #pragma unroll
@@ -749,7 +775,9 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
               o[i][n][2 + x] *= by;
             }
           }
-        }
+      }
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           // (m - ev) is the same for all tiles whose pages have the same ev: its rounding cancels
