@@ -98,7 +98,7 @@ SIGNATURES = {
     "cats_kv8_grow": (_c_int, [_kv8_p, _c_void_p, _c_int, _c_void_p]),
     "cats_kv8_append": (_c_int, [_kv8_p, _c_int, _c_void_p, _c_longlong, _c_void_p, _c_int, _c_void_p,
                                  _c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_void_p]),
-    "cats_kv8_attend_bytes": (_c_size_t, [_kv8_p]),
+    "cats_kv8_attend_bytes": (_c_size_t, [_kv8_p, _c_int, _c_int]),
     "cats_kv8_attend": (_c_int, [_kv8_p, _c_int, _c_void_p, _c_longlong, _c_void_p, _c_int, _c_int,
                                  _c_float, _c_void_p, _c_void_p, _c_size_t, _c_int, _c_void_p]),
     "cats_kv8_reorder_bytes": (_c_size_t, [_kv8_p]),

@@ -133,6 +133,9 @@ Options& options() {
   return o;
 }
 
+}  // namespace
+
+namespace cats {
 // The wait limit in units of 1024 clock cycles of the current device.
 int wait_kcycles() {
   long long ms = options().wait_ms;
@@ -141,6 +144,9 @@ int wait_kcycles() {
   const long long kc = ms * dev_info().clock_khz / 1024;
   return (int)(kc > 0x7fffffffLL ? 0x7fffffffLL : kc);
 }
+}  // namespace cats
+
+namespace {
 
 // Largest stage count <= smax (looking at most 3 below it) whose largest divisor <= 8 — the
 // number of consumer warps that can stride over the ring — is biggest.

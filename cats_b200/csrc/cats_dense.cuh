@@ -151,7 +151,7 @@ struct DenseStackParams {
 static_assert(sizeof(DenseStackParams) <= kWsTableBytes, "the table must fit its workspace region");
 
 // Copies the parameter block into the workspace table (one CTA; 16 bytes per thread and step).
-__global__ void __launch_bounds__(256)
+static __global__ void __launch_bounds__(256)
 k_dense_table(const __grid_constant__ DenseStackParams P, DenseStackParams* dst) {
   const uint4* src = reinterpret_cast<const uint4*>(&P);
   uint4* d = reinterpret_cast<uint4*>(dst);

@@ -95,6 +95,7 @@ cudaError_t attend(const cats_kv8& c, int layer, const void* q, long long q_ld, 
   A.parts = (float*)ws;
   A.ctas = dev_info().sms < CATS_KV8_STATUS_INTS - 1 ? dev_info().sms : CATS_KV8_STATUS_INTS - 1;
   A.counters = c.status + 1;
+  A.wait_kc = wait_kcycles();
   return inst_kv8_attend<T>(c, A, st);
 }
 
@@ -146,9 +147,9 @@ int cats_kv8_append(const cats_kv8* cache, int layer, const void* qkv, long long
   return launch_status(e);
 }
 
-size_t cats_kv8_attend_bytes(const cats_kv8* cache) {
-  if (!cache || cache->head_dim < 1) return 0;
-  return sizeof(float) * 2 * (size_t)dev_info().sms * attn_part_floats(kAttnMaxRows, cache->head_dim);
+size_t cats_kv8_attend_bytes(const cats_kv8* cache, int n_tokens, int n_heads) {
+  if (check_cache(cache) || n_tokens < 1 || n_heads < 1) return 0;
+  return sizeof(float) * 2 * (size_t)dev_info().sms * attn_part_floats(attn_part_rows(*cache, n_tokens, n_heads), cache->head_dim);
 }
 
 int cats_kv8_attend(const cats_kv8* cache, int layer, const void* q, long long q_ld, const int* cu, int n_tokens,
@@ -162,7 +163,7 @@ int cats_kv8_attend(const cats_kv8* cache, int layer, const void* q, long long q
   if (!q || !out || !ws) return CATS_ERR_NULL;
   if (q_ld < (long long)n_heads * cache->head_dim) return CATS_ERR_RANGE;
   if (!aligned16(q) || (q_ld * esize(dtype)) % 16 || !aligned16(out) || !aligned16(ws)) return CATS_ERR_ALIGN;
-  if (ws_bytes < cats_kv8_attend_bytes(cache)) return CATS_ERR_WORKSPACE;
+  if (ws_bytes < cats_kv8_attend_bytes(cache, n_tokens, n_heads)) return CATS_ERR_WORKSPACE;
   cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e;
   if (dtype == CATS_F32) e = attend<float>(*cache, layer, q, q_ld, cu, n_tokens, n_heads, scale, out, ws, st);

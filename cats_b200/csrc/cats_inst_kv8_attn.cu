@@ -1,33 +1,50 @@
 // The attention kernels of the paged 8-bit cache for ONE element type; compiled once per type with
 // -DCATS_ELEM_ID=0|1|2 (float, __half, __nv_bfloat16).
-#include "cats_kv8_attn.cuh"
+#include "cats_kv8_attn_tc.cuh"
 #include "cats_kv8_run.cuh"
 
 namespace cats {
 
-template <typename T, int HD, int NQ>
-static cudaError_t run_attend(const cats_kv8& c, const KvAttnArgs<T>& A, cudaStream_t st) {
-  using S = AttnShape<NQ>;
-  // (the attribute stays with the kernel: once per device; two threads at once set the same value)
-  static bool ready[64];
+// Launches a kernel that needs much shared memory.  (The attribute stays with the kernel: once per
+// device; two threads at once set the same value.)
+template <typename T>
+static cudaError_t run_large(void (*kernel)(cats_kv8, KvAttnArgs<T>), bool* ready, int threads, size_t smem,
+                             const cats_kv8& c, const KvAttnArgs<T>& A, cudaStream_t st) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !ready[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(k_kv8_attend<T, HD, NQ>),
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize, (int)attn_smem<NQ>());
+    const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) ready[dev] = true;
   }
-  return launch_ready(k_kv8_attend<T, HD, NQ>, dim3(A.ctas), dim3(S::kThreads), attn_smem<NQ>(), st, c, A);
+  return launch_ready(kernel, dim3(A.ctas), dim3(threads), smem, st, c, A);
 }
 
+template <typename T, int HD, int NQ>
+static cudaError_t run_attend(const cats_kv8& c, const KvAttnArgs<T>& A, cudaStream_t st) {
+  static bool ready[64];
+  return run_large<T>(k_kv8_attend<T, HD, NQ>, ready, AttnShape<NQ>::kThreads, attn_smem<NQ>(), c, A, st);
+}
+
+// Up to 8 rows and up to 16 the tiles of cats_kv8_attn.cuh, bound by the codes' bytes; beyond that the
+// products count.  16-bit queries then take tiles of 128 rows on tcgen05, also where only some of the
+// rows are used (2 x 256 tokens x 4 heads per key head, head_dim 128: see the table in the design
+// notes); head_dim 32 and 96, which do not fill a 128-byte swizzle row, tiles of 32 rows; fp32 queries,
+// which are split in two halves and leave no registers for more, tiles of 16.
 template <typename T, int HD>
 static cudaError_t run_attend(const cats_kv8& c, const KvAttnArgs<T>& A, cudaStream_t st) {
-  // rows of a key head: (new tokens) x (query heads per key head), on average over the sequences
-  const long long rows = ((long long)A.tokens + c.n_seqs - 1) / c.n_seqs * (A.nh / c.n_kv_heads);
+  const long long rows = attn_rows(c, A.tokens, A.nh);
   if (rows <= 8) return run_attend<T, HD, 1>(c, A, st);
-  if constexpr (sizeof(T) == 2) {                       // (fp32 queries are two halves: no room)
-    if (rows > 16) return run_attend<T, HD, 4>(c, A, st);
+  if constexpr (sizeof(T) == 2) {
+    if (rows > kAttnFewRows) {
+      if constexpr (HD % 64 == 0) {
+        static bool ready[64];
+        return run_large<T>(k_kv8_attend_tc<T, HD>, ready, 256, attn_tc_smem(HD), c, A, st);
+      } else {
+        return run_attend<T, HD, 4>(c, A, st);
+      }
+    }
   }
   return run_attend<T, HD, 2>(c, A, st);
 }

@@ -19,7 +19,7 @@ constexpr int kKvMaxSeqs = 1024;      // sequences of one cache: one thread each
 constexpr int kPlanThreads = 1024;
 
 // bits of the cache's status word
-enum { KV_POOL_EMPTY = 1, KV_BAD_PAGE = 2, KV_TOO_LONG = 4, KV_BAD_PARENT = 8, KV_BAD_SPAN = 16 };
+enum { KV_POOL_EMPTY = 1, KV_BAD_PAGE = 2, KV_TOO_LONG = 4, KV_BAD_PARENT = 8, KV_BAD_SPAN = 16, KV_WAIT = 32 };
 
 __device__ __forceinline__ void kv_flag(const cats_kv8& c, int bit) { atomicOr(c.status, bit); }
 

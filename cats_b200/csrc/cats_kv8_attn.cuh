@@ -58,11 +58,19 @@ struct KvAttnArgs {
   float* parts;           // [CTAs][2][rows of a tile][hd + 2] parts of (head, tile)s that several CTAs share
   int* counters;          // [CTAs], zero between calls
   const int* cu;
-  int uniform, tokens, nh, layer, ctas;
+  int uniform, tokens, nh, layer, ctas, wait_kc;
   float scale;            // of the scores, times log2(e)
 };
 
-constexpr int kAttnMaxRows = 32;
+// Rows of a key head, (new tokens) x (query heads per key head), on average over the sequences: what
+// the kernels are chosen by, and the rows that a part of theirs can have.
+__host__ __device__ inline long long attn_rows(const cats_kv8& c, int tokens, int nh) {
+  return ((long long)tokens + c.n_seqs - 1) / c.n_seqs * (nh / c.n_kv_heads);
+}
+constexpr int kAttnFewRows = 16;                        // up to here 8 or 16 rows a tile
+inline int attn_part_rows(const cats_kv8& c, int tokens, int nh) {
+  return attn_rows(c, tokens, nh) > kAttnFewRows ? 128 : 16;
+}
 __host__ __device__ inline size_t attn_part_floats(int rows, int hd) { return (size_t)rows * (hd + 2); }
 template <int NQ>
 constexpr size_t attn_smem() {

@@ -18,6 +18,7 @@ struct DevInfo {
 };
 const DevInfo& dev_info();  // per-device properties of the current device (cats_abi.cu)
 int launch_status(cudaError_t e);  // CATS_OK, or CATS_ERR_CUDA with the error kept for cats_last_cuda_error
+int wait_kcycles();         // the "wait_ms" option in units of 1024 clock cycles of the current device
 extern int g_use_pdl;       // cats_set_option("pdl", 0) launches without programmatic dependencies
 
 // Launch with the programmatic-stream-serialisation attribute: the grid may be scheduled while

@@ -32,7 +32,8 @@ _current_device = torch._C._cuda_getDevice
 PAGES, HEAD_DIMS, MAX_SEQS, STATUS_INTS = (16, 32, 64, 128), (32, 64, 96, 128), 1024, 256
 _STATUS = {1: "the pool has no free page left", 2: "a page id is out of range, or a shared page would have been written",
            4: "a sequence is longer than the page table allows, or a length or position is negative",
-           8: "a parent is out of range", 16: "cu does not fit the number of tokens"}
+           8: "a parent is out of range", 16: "cu does not fit the number of tokens",
+           32: "a wait inside a kernel ran out"}
 
 
 def _bad(msg: str) -> RuntimeError:
@@ -92,8 +93,7 @@ class KVCache8:
         self._p = ctypes.byref(self._c)
         self._index = codes.device.index
         lib = _lib.lib()
-        with torch.cuda.device(self._index):
-            self._attend_nbytes = int(lib.cats_kv8_attend_bytes(self._p))
+        self._attend_nbytes = {}                # by (tokens, heads)
         self._reorder_nbytes = int(lib.cats_kv8_reorder_bytes(self._p))
         self._compact_nbytes = int(lib.cats_kv8_compact_bytes(self._p))
 
@@ -198,7 +198,13 @@ class KVCache8:
             raise _bad("out must be contiguous with as many elements as q, of q's type")
         if n == 0:
             return out
-        nbytes = self._attend_nbytes
+        nbytes = self._attend_nbytes.get((n, nh))
+        if nbytes is None:
+            with torch.cuda.device(self._index):
+                nbytes = int(_lib.lib().cats_kv8_attend_bytes(self._p, n, nh))
+            if len(self._attend_nbytes) >= 4096:
+                self._attend_nbytes.clear()
+            self._attend_nbytes[(n, nh)] = nbytes
         ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         self._call("cats_kv8_attend", layer, q.data_ptr(), q.stride(0) if n > 1 else nh * hd, self._cu(cu), n, nh,
                    hd ** -0.5 if scale is None else scale, out.data_ptr(), ws.data_ptr(), nbytes, code)

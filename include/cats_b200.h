@@ -405,7 +405,8 @@ int cats_export_list(const void* ws, size_t ws_bytes, int B, int H, int I, int d
  * (never read or written out of range) and recorded in *status, bits that stay until the caller
  * clears them: 1 the pool has no page left, 2 a page id is out of range or a page that is shared
  * would have been written, 4 a sequence is longer than max_pages pages (or has a negative length or
- * position), 8 a parent is out of range, 16 cu does not fit the number of tokens.
+ * position), 8 a parent is out of range, 16 cu does not fit the number of tokens, 32 a wait inside a
+ * kernel ran out (see "wait_ms"; the results of that call are not to be used).
  * No reference counterpart (the reference leaves the cache to HF's modelling code).
  */
 enum { CATS_KV8_STATUS_INTS = 256 };
@@ -457,7 +458,7 @@ int cats_kv8_append(const cats_kv8* cache, int layer, const void* qkv, long long
  *   out [n_tokens, n_heads, head_dim]; ws: cats_kv8_attend_bytes(...) bytes of scratch, contents
  *   irrelevant before and after.
  */
-size_t cats_kv8_attend_bytes(const cats_kv8* cache);
+size_t cats_kv8_attend_bytes(const cats_kv8* cache, int n_tokens, int n_heads);
 int cats_kv8_attend(const cats_kv8* cache, int layer, const void* q, long long q_ld, const int* cu,
                     int n_tokens, int n_heads, float scale, void* out, void* ws, size_t ws_bytes,
                     int dtype, void* stream);
