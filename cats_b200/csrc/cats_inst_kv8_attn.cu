@@ -40,7 +40,7 @@ static cudaError_t run_attend(const cats_kv8& c, const KvAttnArgs<T>& A, cudaStr
     if (rows > kAttnFewRows) {
       if constexpr (HD % 64 == 0) {
         static bool ready[64];
-        return run_large<T>(k_kv8_attend_tc<T, HD>, ready, 256, attn_tc_smem(HD), c, A, st);
+        return run_large<T>(k_kv8_attend_tc<T, HD>, ready, kTcThreads, attn_tc_smem(HD), c, A, st);
       } else {
         return run_attend<T, HD, 4>(c, A, st);
       }

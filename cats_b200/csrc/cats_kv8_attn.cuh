@@ -41,10 +41,10 @@ constexpr float kAttnSlack = 8.f;                       // see the running maxim
 template <int NQ>
 struct AttnShape {
   static constexpr int kRows = 8 * NQ;
-  static constexpr int kWarps = NQ == 1 ? 16 : 8;
+  static constexpr int kWarps = NQ == 1 || NQ == 16 ? 16 : 8;
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kStages = NQ == 1 ? 3 : 6;       // tiles a warp has in its ring (one of them in use)
-  static constexpr int kUnit = kWarps * kAttnTile;      // positions of a unit
+  static constexpr int kUnit = NQ == 1 ? 256 : 128;     // positions of a unit (a tile for each warp up to NQ = 4)
   static constexpr int kJoin = 512 / kUnit;             // joining parts takes about as long as 512 positions
   static constexpr int kSwitch = 768 / kUnit;           // going over to another segment, as long as 768
   static constexpr bool kQueriesShared = NQ == 4;

@@ -8,7 +8,7 @@
 //     memory: K as it lies, V transposed, both K-major under the 128-byte swizzle;
 //   2 the next step's codes are asked for;
 //   3 one thread issues S = Q K^T;
-//   4 two threads per row take half a row of S each from tensor memory: maximum, exponentials, sum;
+//   4 four threads per row take a quarter of a row of S each from tensor memory: maximum, exponentials, sum;
 //     the weights go to shared memory in half precision;
 //   5 one thread issues O += P V, which runs while the next step's codes are converted (V has two
 //     buffers; the next S is committed behind it, so waiting for S waits for it too).
@@ -25,9 +25,9 @@
 
 namespace cats {
 
-constexpr int kTcRows = 128, kTcKeys = 128;
+constexpr int kTcRows = 128, kTcKeys = 128, kTcThreads = 512;
 using TcShape = AttnShape<16>;
-static_assert(TcShape::kRows == kTcRows && TcShape::kUnit == kTcKeys && TcShape::kThreads == 256, "tile");
+static_assert(TcShape::kRows == kTcRows && TcShape::kUnit == kTcKeys && TcShape::kThreads == kTcThreads, "tile");
 
 constexpr uint32_t kTcBlock = 128 * 128;               // 128 rows of 64 half-precision values
 __host__ __device__ constexpr size_t attn_tc_smem(int hd) {
@@ -72,22 +72,24 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float* v) {
 __host__ __device__ constexpr uint32_t tc_idesc(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24); }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(256, 1) k_kv8_attend_tc(const cats_kv8 c, const KvAttnArgs<T> A) {
-  constexpr int NQ = 16, HB = HD / 64, kChunks = HD / 16, NK = HD / 32;   // NK: 16-byte loads of K per thread
+__global__ void __launch_bounds__(kTcThreads, 1) k_kv8_attend_tc(const cats_kv8 c, const KvAttnArgs<T> A) {
+  constexpr int NQ = 16, HB = HD / 64, kChunks = HD / 16, NK = HD / 64;   // NK: 16-byte loads of K per thread
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ AttnTable s_tab;
   __shared__ AttnPlan s_plan;
-  __shared__ int s_warp[8], s_last, s_owners[2], s_ctl[2];
+  __shared__ int s_warp[kTcThreads / 32], s_last, s_owners[2], s_ctl[2];
   __shared__ uint64_t s_bar;
   __shared__ uint32_t s_tmem;
   __shared__ int s_id[2][8];                             // page of 16 positions each of this and the next step,
   __shared__ float s_ks[2][8], s_ev[2][8];               // scale of its keys, exponent of its values' scale
-  __shared__ float s_x[2][kTcRows];                      // what the two threads of a row tell one another
+  __shared__ float s_x[4][kTcRows];                      // what the four threads of a row tell one another
   __shared__ int s_nan[HD];
   pdl_wait();
   pdl_launch_dependents();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int row = (warp & 3) * 32 + lane, half = warp >> 2;
+  const int row = (warp & 3) * 32 + lane, quarter = warp >> 2;
+  const int page_mask = c.page - 1;                      // (pages are powers of two)
+  const int page_log = 31 - __clz(c.page);
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t q_u = base, k_u = q_u + HB * kTcBlock, v_u = k_u + HB * kTcBlock, p_u = v_u + 2 * 2 * HD * 128;
   const uint32_t bar = smem_u32(&s_bar);
@@ -142,7 +144,7 @@ __global__ void __launch_bounds__(256, 1) k_kv8_attend_tc(const cats_kv8 c, cons
       n_ev = 0.f;
       const int p = unit * kTcKeys + 16 * tid;
       if (tid < 8 && unit < u_end && p < end) {
-        const int id = table[p / c.page];
+        const int id = table[p >> page_log];
         if (id < 0 || id >= c.n_pages) {
           kv_flag(c, KV_BAD_PAGE);
         } else {
@@ -159,48 +161,50 @@ __global__ void __launch_bounds__(256, 1) k_kv8_attend_tc(const cats_kv8 c, cons
         s_ev[unit & 1][tid] = n_ev;
       }
     };
-    // a step's codes: K 16 bytes of rows tid / kChunks + i * (256 / kChunks); V (a warp to 16 channels)
-    // 16 bytes of the four rows 4 lane ..
-    uint4 kc[NK], vc[4];
+    // a step's codes: K 16 bytes of rows tid / kChunks + i * (512 / kChunks); V (a warp to 8 channels)
+    // 8 bytes of the four rows 4 lane .. (L1 keeps the rest of the sectors for the other warps)
+    uint4 kc[NK];
+    uint2 vc[4];
     auto fetch = [&](int unit) {
       const int kb = unit * kTcKeys;
 #pragma unroll
       for (int i = 0; i < NK; ++i) {
-        const int r = tid / kChunks + i * (256 / kChunks);
+        const int r = tid / kChunks + i * (kTcThreads / kChunks);
         const int id = s_id[unit & 1][r >> 4];
         kc[i] = make_uint4(0, 0, 0, 0);
         if (id >= 0 && kb + r < end)
           kc[i] = ldg_stream(reinterpret_cast<const uint4*>(layer_codes + ((size_t)id * 2 * c.n_kv_heads + at.head) * block +
-                                                            (size_t)(r % c.page) * HD) + tid % kChunks);
+                                                            (size_t)(r & page_mask) * HD) + tid % kChunks);
       }
       const int id = s_id[unit & 1][lane >> 2];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int r = 4 * lane + i;
-        vc[i] = make_uint4(0, 0, 0, 0);
-        if (warp < kChunks && id >= 0 && kb + r < end)
-          vc[i] = ldg_stream(reinterpret_cast<const uint4*>(layer_codes + ((size_t)id * 2 * c.n_kv_heads + at.head) * block +
-                                                            v_off + (size_t)(r % c.page) * HD) + warp);
+        vc[i] = make_uint2(0, 0);
+        if (warp < 2 * kChunks && id >= 0 && kb + r < end)
+          vc[i] = __ldg(reinterpret_cast<const uint2*>(layer_codes + ((size_t)id * 2 * c.n_kv_heads + at.head) * block + v_off +
+                                                       (size_t)(r & page_mask) * HD) + warp);
       }
     };
 
     look(u_first);
-    // ---- queries: two threads per row, half the channels each
+    // ---- queries: four threads per row, a quarter of the channels each
     const int rr = at.tile * kTcRows + row, tok = rr / group, hq = at.head * group + rr - tok * group;
     const bool on = row < rows;
     const int lim = on ? min(seq.len, seq.len - seq.count + tok + 1) : 0;
     float f;
     {
-      float q[HD / 2], top = 0.f;
-      const T* src = A.q + (size_t)(seq.first + tok) * A.q_ld + (size_t)hq * HD + half * (HD / 2);
+      constexpr int NC = HD / 4;
+      float q[NC], top = 0.f;
+      const T* src = A.q + (size_t)(seq.first + tok) * A.q_ld + (size_t)hq * HD + quarter * NC;
 #pragma unroll
-      for (int i = 0; i < HD / 2; i += 8) {
+      for (int i = 0; i < NC; i += 8) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) q[i + k] = 0.f;
         if (on) load8_cached(src + i, q + i);
       }
 #pragma unroll
-      for (int i = 0; i < HD / 2; ++i) {
+      for (int i = 0; i < NC; ++i) {
         const float a = fabsf(q[i]);
         if (a <= 3.402823466e38f) top = fmaxf(top, a);
       }
@@ -208,16 +212,16 @@ __global__ void __launch_bounds__(256, 1) k_kv8_attend_tc(const cats_kv8 c, cons
       keep(u_first);
       look(u_first + 1);
       keep(u_first + 1);
-      for (int d = tid; d < HD; d += 256) s_nan[d] = 0x7fffffff;
-      s_x[half][row] = top;
+      for (int d = tid; d < HD; d += kTcThreads) s_nan[d] = 0x7fffffff;
+      s_x[quarter][row] = top;
       __syncthreads();
-      top = fmaxf(top, s_x[half ^ 1][row]);
+      top = fmaxf(fmaxf(s_x[0][row], s_x[1][row]), fmaxf(s_x[2][row], s_x[3][row]));
       const int e = top > 0.f ? min(max(kv_exp_of(top) + 1, -126), 126) : 0;
       const float inv = kv_pow2(-e);
       f = kv_pow2(e) * A.scale;
 #pragma unroll
-      for (int i = 0; i < HD / 2; i += 8) {
-        const int d = half * (HD / 2) + i;
+      for (int i = 0; i < NC; i += 8) {
+        const int d = quarter * NC + i;
         sts16(q_u + (d / 64) * kTcBlock + tc_at(row, (d % 64) / 8), half2_bits(q[i] * inv, q[i + 1] * inv),
               half2_bits(q[i + 2] * inv, q[i + 3] * inv), half2_bits(q[i + 4] * inv, q[i + 5] * inv),
               half2_bits(q[i + 6] * inv, q[i + 7] * inv));
@@ -231,7 +235,7 @@ __global__ void __launch_bounds__(256, 1) k_kv8_attend_tc(const cats_kv8 c, cons
       // ---- 1 codes to half precision
 #pragma unroll
       for (int i = 0; i < NK; ++i) {
-        const int r = tid / kChunks + i * (256 / kChunks), ch = tid % kChunks;
+        const int r = tid / kChunks + i * (kTcThreads / kChunks), ch = tid % kChunks;
         const uint32_t w[4] = {kc[i].x, kc[i].y, kc[i].z, kc[i].w};
         uint32_t h[8];
 #pragma unroll
@@ -248,22 +252,21 @@ __global__ void __launch_bounds__(256, 1) k_kv8_attend_tc(const cats_kv8 c, cons
           sts16(a1, h[0], h[1], h[2], h[3]);
         }
       }
-      if (warp < kChunks) {
-        const uint32_t vb = v_u + (unit & 1) * (2 * HD * 128) + (lane >> 4) * (HD * 128);
+      if (warp < 2 * kChunks) {
+        const uint32_t vb = v_u + (unit & 1) * (2 * HD * 128) + (lane >> 4) * (HD * 128) + (lane & 1) * 8;
+        uint32_t nan = 0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {                    // four channels at a time
-          uint32_t w[4] = {k == 0 ? vc[0].x : k == 1 ? vc[0].y : k == 2 ? vc[0].z : vc[0].w,
-                           k == 0 ? vc[1].x : k == 1 ? vc[1].y : k == 2 ? vc[1].z : vc[1].w,
-                           k == 0 ? vc[2].x : k == 1 ? vc[2].y : k == 2 ? vc[2].z : vc[2].w,
-                           k == 0 ? vc[3].x : k == 1 ? vc[3].y : k == 2 ? vc[3].z : vc[3].w};
-          uint32_t nan = 0;
+        for (int i = 0; i < 4; ++i)
+          nan |= ((vc[i].x & 0x7f7f7f7fu) + 0x01010101u) | ((vc[i].y & 0x7f7f7f7fu) + 0x01010101u);
+        const bool bad = (nan & 0x80808080u) != 0;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) nan |= ((w[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-          if (nan) {
+        for (int k = 0; k < 2; ++k) {                    // four channels at a time
+          uint32_t w[4] = {k ? vc[0].y : vc[0].x, k ? vc[1].y : vc[1].x, k ? vc[2].y : vc[2].x, k ? vc[3].y : vc[3].x};
+          if (bad) {
             for (int i = 0; i < 4; ++i)
               for (int j = 0; j < 4; ++j)
                 if (((w[i] >> (8 * j)) & 0x7fu) == 0x7fu) {
-                  atomicMin(&s_nan[16 * warp + 4 * k + j], kb + 4 * lane + i);
+                  atomicMin(&s_nan[8 * warp + 4 * k + j], kb + 4 * lane + i);
                   w[i] &= ~(0xffu << (8 * j));
                 }
           }
@@ -273,11 +276,10 @@ __global__ void __launch_bounds__(256, 1) k_kv8_attend_tc(const cats_kv8 c, cons
           const uint32_t ch[4] = {__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632), __byte_perm(cc, d, 0x5410),
                                   __byte_perm(cc, d, 0x7632)};
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < 4; ++j) {                  // row 8 warp + 4 k + j: its chunks are exchanged by 4 k + j
             uint32_t lo, hi;
             e4m3x4_to_f16x2(ch[j], lo, hi);
-            const int dd = 16 * warp + 4 * k + j;
-            sts8(vb + tc_at(dd, (lane & 15) >> 1) + (lane & 1) * 8, lo, hi);
+            sts8(vb + (8 * warp + 4 * k + j) * 128 + ((((lane & 15) >> 1) ^ (4 * k + j)) << 4), lo, hi);
           }
         }
       }
@@ -297,49 +299,51 @@ __global__ void __launch_bounds__(256, 1) k_kv8_attend_tc(const cats_kv8 c, cons
       look(unit + 2);
       if (unit + 1 < u_end) fetch(unit + 1);
       wait_mma();
-      // ---- 4 half a row each: weights
-      float s[64];
-      tmem_ld32(t_s + t_lane + 64 * half, s);
-      tmem_ld32(t_s + t_lane + 64 * half + 32, s + 32);
+      // ---- 4 a quarter of a row each: weights
+      float s[32];
+      tmem_ld32(t_s + t_lane + 32 * quarter, s);
       float top = -INFINITY;
-      const bool cut = kb + 64 * half + 64 > lim;
+      const int k0 = kb + 32 * quarter;
+      float ev[2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int z = 4 * half + j;
+      for (int j = 0; j < 2; ++j) {
+        const int z = 2 * quarter + j;
         const float by = s_ks[unit & 1][z] * f;
-        const bool there = s_id[unit & 1][z] >= 0;
+        ev[j] = s_ev[unit & 1][z];
         float t = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float& x = s[16 * j + i];
-          x *= by;
-          if (cut || !there)
-            if (!there || kb + 64 * half + 16 * j + i >= lim) x = -INFINITY;
-          t = fmaxf(t, x);
+        for (int i = 0; i < 16; ++i) s[16 * j + i] *= by;
+        if (k0 + 16 * j + 16 > lim || s_id[unit & 1][z] < 0) {
+          const int sees = s_id[unit & 1][z] < 0 ? 0 : lim - k0 - 16 * j;      // of the sixteen
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (i >= sees) s[16 * j + i] = -INFINITY;
         }
-        top = fmaxf(top, t + s_ev[unit & 1][z]);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) t = fmaxf(t, s[16 * j + i]);
+        top = fmaxf(top, t + ev[j]);
       }
-      s_x[half][row] = top;
-      asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");     // the two warps of these rows
-      top = fmaxf(top, s_x[half ^ 1][row]);
+      s_x[quarter][row] = top;
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + (warp & 3)) : "memory");    // the four warps of these rows
+      top = fmaxf(fmaxf(s_x[0][row], s_x[1][row]), fmaxf(s_x[2][row], s_x[3][row]));
       if (__any_sync(0xffffffffu, top > m + kAttnSlack)) {
         const float to = fmaxf(top, m), by = m == -INFINITY ? 0.f : ex2(m - to);
         m = to;
         l *= by;
         if (unit > u_first) {
 #pragma unroll
-          for (int d = 0; d < HD / 2; d += 16) {
+          for (int d = 0; d < HD / 4; d += 16) {
             float o[16];
-            tmem_ld16(t_o + t_lane + half * (HD / 2) + d, o);
+            tmem_ld16(t_o + t_lane + quarter * (HD / 4) + d, o);
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[i] *= by;
-            tmem_st16(t_o + t_lane + half * (HD / 2) + d, o);
+            tmem_st16(t_o + t_lane + quarter * (HD / 4) + d, o);
           }
         }
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float ev = s_ev[unit & 1][4 * half + j], ref = m == -INFINITY ? 0.f : m - ev;
+      for (int j = 0; j < 2; ++j) {
+        const float ref = m == -INFINITY ? 0.f : m - ev[j];
         float part = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -347,12 +351,12 @@ __global__ void __launch_bounds__(256, 1) k_kv8_attend_tc(const cats_kv8 c, cons
           x = ex2(x - ref);
           part += x;
         }
-        l = fmaf(part, kv_pow2(-(int)ev), l);
+        l = fmaf(part, kv_pow2(-(int)ev[j]), l);
 #pragma unroll
         for (int i = 0; i < 16; i += 8) {
           const float* x = s + 16 * j + i;
-          sts16(p_u + half * kTcBlock + tc_at(row, 2 * j + i / 8), half2_bits(x[0], x[1]), half2_bits(x[2], x[3]),
-                half2_bits(x[4], x[5]), half2_bits(x[6], x[7]));
+          sts16(p_u + (quarter >> 1) * kTcBlock + tc_at(row, 4 * (quarter & 1) + 2 * j + i / 8), half2_bits(x[0], x[1]),
+                half2_bits(x[2], x[3]), half2_bits(x[4], x[5]), half2_bits(x[6], x[7]));
         }
       }
       fence_proxy_async_smem();
@@ -374,19 +378,19 @@ __global__ void __launch_bounds__(256, 1) k_kv8_attend_tc(const cats_kv8 c, cons
 
     // ---- the segment's end
     __syncthreads();
-    s_x[half][row] = l;
+    s_x[quarter][row] = l;
     __syncthreads();
-    l += s_x[half ^ 1][row];
+    l = (s_x[0][row] + s_x[1][row]) + (s_x[2][row] + s_x[3][row]);
     const bool whole = u_first == 0 && u_end == seq.units;
     float* part = A.parts + (size_t)(blockIdx.x * 2 + (first_seg ? 0 : 1)) * attn_part_floats(kTcRows, HD);
 #pragma unroll
-    for (int d0 = 0; d0 < HD / 2; d0 += 16) {
+    for (int d0 = 0; d0 < HD / 4; d0 += 16) {
       float o[16];
-      tmem_ld16(t_o + t_lane + half * (HD / 2) + d0, o);
+      tmem_ld16(t_o + t_lane + quarter * (HD / 4) + d0, o);
       if (on) {
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
-          const int d = half * (HD / 2) + d0 + i;
+          const int d = quarter * (HD / 4) + d0 + i;
           float4 v = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
           const float bad = __uint_as_float(0x7fc00000u);
           if (s_nan[d] < lim) v.x = bad;
@@ -420,7 +424,7 @@ __global__ void __launch_bounds__(256, 1) k_kv8_attend_tc(const cats_kv8 c, cons
         __threadfence();
         const int c0 = s_owners[0], c1 = s_owners[1];
         const int first_begins = attn_share<NQ>(s_tab, plan, c.n_seqs, group, c0);
-        for (int e = tid; e < rows * (HD / 4); e += 256) {
+        for (int e = tid; e < rows * (HD / 4); e += kTcThreads) {
           const int r = e / (HD / 4), d = (e - r * (HD / 4)) * 4;
           float top = -INFINITY, sum = 0.f;
           float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
