@@ -4,8 +4,9 @@
 // the codes' bytes but by the two products, and both fill a tcgen05 tile: S = Q K^T and O += P V, 128
 // rows x 128 positions, accumulators in tensor memory (S 128 columns, O head_dim columns).  A CTA
 // takes a tile of rows through its positions, 128 at a time:
-//   1 codes (in registers since the last step) become half precision, exactly, and go to shared
-//     memory: K as it lies, V transposed, both K-major under the 128-byte swizzle;
+//   1 codes become half precision, exactly, and go to shared memory, both K-major under the 128-byte
+//     swizzle: K, in registers since the last step, as it lies; V, copied to shared memory meanwhile (a
+//     gather of four positions per lane from global memory costs L1 a lookup per row), transposed;
 //   2 the next step's codes are asked for;
 //   3 one thread issues S = Q K^T;
 //   4 four threads per row take a quarter of a row of S each from tensor memory: maximum, exponentials, sum;
@@ -31,8 +32,8 @@ static_assert(TcShape::kRows == kTcRows && TcShape::kUnit == kTcKeys && TcShape:
 
 constexpr uint32_t kTcBlock = 128 * 128;               // 128 rows of 64 half-precision values
 __host__ __device__ constexpr size_t attn_tc_smem(int hd) {
-  // Q, K: hd / 64 blocks; V: two buffers of two blocks of hd rows; P: two blocks
-  return 1024 + (size_t)(hd / 64) * kTcBlock * 2 + (size_t)2 * 2 * hd * 128 + 2 * kTcBlock;
+  // Q, K: hd / 64 blocks; V: two buffers of two blocks of hd rows; P: two blocks; V's codes
+  return 1024 + (size_t)(hd / 64) * kTcBlock * 2 + (size_t)2 * 2 * hd * 128 + 2 * kTcBlock + kTcBlock;
 }
 
 // byte of 16-byte chunk `chunk` of row `row` in a block under the 128-byte swizzle
@@ -92,6 +93,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_kv8_attend_tc(const cats_kv8 
   const int page_log = 31 - __clz(c.page);
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t q_u = base, k_u = q_u + HB * kTcBlock, v_u = k_u + HB * kTcBlock, p_u = v_u + 2 * 2 * HD * 128;
+  const uint32_t raw_u = p_u + 2 * kTcBlock;               // rows 128 bytes apart, chunks exchanged by row / 4
   const uint32_t bar = smem_u32(&s_bar);
 
   const AttnPlan plan = attn_table<NQ, HD>(c, A, s_tab, &s_plan, s_warp);
@@ -161,31 +163,25 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_kv8_attend_tc(const cats_kv8 
         s_ev[unit & 1][tid] = n_ev;
       }
     };
-    // a step's codes: K 16 bytes of rows tid / kChunks + i * (512 / kChunks); V (a warp to 8 channels)
-    // 8 bytes of the four rows 4 lane .. (L1 keeps the rest of the sectors for the other warps)
+    // a step's codes: 16 bytes of rows tid / kChunks + i * (512 / kChunks)
     uint4 kc[NK];
-    uint2 vc[4];
     auto fetch = [&](int unit) {
-      const int kb = unit * kTcKeys;
+      const int kb = unit * kTcKeys, ch = tid % kChunks;
 #pragma unroll
       for (int i = 0; i < NK; ++i) {
         const int r = tid / kChunks + i * (kTcThreads / kChunks);
         const int id = s_id[unit & 1][r >> 4];
+        const bool in = id >= 0 && kb + r < end;
+        const uint8_t* src = layer_codes + ((size_t)(in ? id : 0) * 2 * c.n_kv_heads + at.head) * block +
+                             (size_t)(r & page_mask) * HD + 16 * ch;
         kc[i] = make_uint4(0, 0, 0, 0);
-        if (id >= 0 && kb + r < end)
-          kc[i] = ldg_stream(reinterpret_cast<const uint4*>(layer_codes + ((size_t)id * 2 * c.n_kv_heads + at.head) * block +
-                                                            (size_t)(r & page_mask) * HD) + tid % kChunks);
+        if (in) kc[i] = ldg_stream(reinterpret_cast<const uint4*>(src));
+        const uint32_t to = raw_u + r * 128 + ((ch ^ ((r >> 2) & 7)) << 4);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src + v_off), "r"(in ? 16 : 0) : "memory");
       }
-      const int id = s_id[unit & 1][lane >> 2];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 4 * lane + i;
-        vc[i] = make_uint2(0, 0);
-        if (warp < 2 * kChunks && id >= 0 && kb + r < end)
-          vc[i] = __ldg(reinterpret_cast<const uint2*>(layer_codes + ((size_t)id * 2 * c.n_kv_heads + at.head) * block + v_off +
-                                                       (size_t)(r & page_mask) * HD) + warp);
-      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    auto settle = [&]() { asm volatile("cp.async.wait_all;" ::: "memory"); };   // (then a barrier)
 
     look(u_first);
     // ---- queries: four threads per row, a quarter of the channels each
@@ -228,6 +224,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_kv8_attend_tc(const cats_kv8 
       }
     }
     fetch(u_first);
+    settle();
+    __syncthreads();
     float m = -INFINITY, l = 0.f;
 
     for (int unit = u_first; unit < u_end; ++unit) {
@@ -254,6 +252,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_kv8_attend_tc(const cats_kv8 
       }
       if (warp < 2 * kChunks) {
         const uint32_t vb = v_u + (unit & 1) * (2 * HD * 128) + (lane >> 4) * (HD * 128) + (lane & 1) * 8;
+        uint2 vc[4];                                     // 8 channels of positions 4 lane ..
+#pragma unroll
+        for (int i = 0; i < 4; ++i) vc[i] = lds2(raw_u + (4 * lane + i) * 128 + (((warp >> 1) ^ (lane & 7)) << 4) + (warp & 1) * 8);
         uint32_t nan = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -359,6 +360,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_kv8_attend_tc(const cats_kv8 
                 half2_bits(x[2], x[3]), half2_bits(x[4], x[5]), half2_bits(x[6], x[7]));
         }
       }
+      settle();
       fence_proxy_async_smem();
       tc_fence_before();
       __syncthreads();
@@ -424,18 +426,36 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_kv8_attend_tc(const cats_kv8 
         __threadfence();
         const int c0 = s_owners[0], c1 = s_owners[1];
         const int first_begins = attn_share<NQ>(s_tab, plan, c.n_seqs, group, c0);
-        for (int e = tid; e < rows * (HD / 4); e += kTcThreads) {
-          const int r = e / (HD / 4), d = (e - r * (HD / 4)) * 4;
-          float top = -INFINITY, sum = 0.f;
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        const int items = rows * (HD / 4);
+        for (int e0 = tid; e0 < items; e0 += 4 * kTcThreads) {         // four at a time: their loads go together
+          float top[4], sum[4];
+          float4 v[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            top[k] = -INFINITY;
+            sum[k] = 0.f;
+            v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          }
           for (int x = c0; x <= c1; ++x) {
             const int slot = x > c0 || first_begins >= u0 ? 0 : 1;
-            const float* src = A.parts + (size_t)(2 * x + slot) * attn_part_floats(kTcRows, HD) + (size_t)r * (HD + 2);
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + HD));
-            const float2 a = __ldcg(reinterpret_cast<const float2*>(src + d)), b = __ldcg(reinterpret_cast<const float2*>(src + d + 2));
-            attn_add(ml.x, ml.y, make_float4(a.x, a.y, b.x, b.y), top, sum, v);
+            const float* src = A.parts + (size_t)(2 * x + slot) * attn_part_floats(kTcRows, HD);
+            float2 ml[4], a[4], b[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int e = min(e0 + k * kTcThreads, items - 1), r = e / (HD / 4), d = (e - r * (HD / 4)) * 4;
+              const float* p = src + (size_t)r * (HD + 2);
+              ml[k] = __ldcg(reinterpret_cast<const float2*>(p + HD));
+              a[k] = __ldcg(reinterpret_cast<const float2*>(p + d));
+              b[k] = __ldcg(reinterpret_cast<const float2*>(p + d + 2));
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) attn_add(ml[k].x, ml[k].y, make_float4(a[k].x, a[k].y, b[k].x, b[k].y), top[k], sum[k], v[k]);
           }
-          attn_store(A, seq, at, group, kTcRows, r, d, HD, sum, v);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int e = e0 + k * kTcThreads, r = e / (HD / 4), d = (e - r * (HD / 4)) * 4;
+            if (e < items) attn_store(A, seq, at, group, kTcRows, r, d, HD, sum[k], v[k]);
+          }
         }
       }
     }
