@@ -185,15 +185,21 @@ int cats_kv8_reorder(const cats_kv8* cache, const int* parents, void* ws, size_t
   cudaStream_t st = (cudaStream_t)stream;
   int* n_copies = (int*)ws;
   KvCopy* copies = (KvCopy*)ws + 1;
-  // a strip holds `width` columns of every row (at most 64 KB with the two arrays beside it)
+  // a strip holds `width` columns of every row (at most 48 KB with the two arrays beside it); a table
+  // that fits one strip of 4096 entries is dealt with by the CTA that hands out the pages
   const int n = cache->n_seqs;
-  int width = 32;
-  while (width > 8 && (size_t)n * (width + 2) * 4 > 48 * 1024) width >>= 1;
-  const size_t smem = (size_t)n * (width + 2) * sizeof(int);
-  cudaError_t e = launch(k_kv8_reorder_table, dim3((cache->max_pages + width - 1) / width), dim3(256), smem, st,
-                         *cache, parents, width);
+  const bool small = (long long)n * cache->max_pages <= 4096;
+  cudaError_t e = cudaSuccess;
+  if (!small) {
+    int width = 32;
+    while (width > 8 && (size_t)n * (width + 2) * 4 > 48 * 1024) width >>= 1;
+    e = launch(k_kv8_reorder_table, dim3((cache->max_pages + width - 1) / width), dim3(256),
+               (size_t)n * (width + 2) * sizeof(int), st, *cache, parents, width);
+  }
   if (e == cudaSuccess)
-    e = launch(k_kv8_reorder_plan, dim3(1), dim3(kPlanThreads), 0, st, *cache, parents, n_copies, copies);
+    e = launch(k_kv8_reorder_plan, dim3(1), dim3(kPlanThreads),
+               small ? (size_t)n * (cache->max_pages + 2) * sizeof(int) : 0, st, *cache, parents, n_copies, copies,
+               small ? 1 : 0);
   if (e == cudaSuccess)
     e = launch(k_kv8_copy, dim3(dev_info().sms * 4), dim3(256), 0, st, *cache, (const int*)n_copies,
                (const KvCopy*)copies);

@@ -321,7 +321,7 @@ __device__ __forceinline__ int plan_free(const cats_kv8& c, int want, int* s_war
     unsigned free_bits = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (id0 + i < c.n_pages && c.refs[id0 + i] == 0) free_bits |= 1u << i;
+      if (id0 + i < c.n_pages && __ldcg(c.refs + id0 + i) == 0) free_bits |= 1u << i;
     int total;
     int rank = found + plan_scan(__popc(free_bits), s_warp, &total);
     while (free_bits && rank < want) {
@@ -392,10 +392,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv8_grow(const cats_kv8 c, con
 // reorder, step 1: strips of the page table.  Row i of the new table is row parents[i] of the old
 // one, which an in-place update can only do column by column with the old column at hand; the
 // counts of pages that gain or lose holders change here too.
-__global__ void __launch_bounds__(256)
-k_kv8_reorder_table(const cats_kv8 c, const int* __restrict__ parents, int width) {
-  pdl_wait();
-  extern __shared__ int sm[];
+__device__ __forceinline__ void reorder_table(const cats_kv8& c, const int* parents, int width, int strip, int* sm) {
   const int n = c.n_seqs;
   int* s_children = sm;                                // [n]
   int* s_parent = sm + n;                              // [n]
@@ -412,7 +409,7 @@ k_kv8_reorder_table(const cats_kv8 c, const int* __restrict__ parents, int width
     if (p >= 0) atomicAdd(&s_children[p], 1);
   }
   __syncthreads();
-  const int j0 = blockIdx.x * width;
+  const int j0 = strip * width;
   for (int k = threadIdx.x; k < n * width; k += blockDim.x) {
     const int i = k / width, j = j0 + k - i * width;
     if (j >= c.max_pages) continue;
@@ -430,6 +427,13 @@ k_kv8_reorder_table(const cats_kv8 c, const int* __restrict__ parents, int width
     c.table[(size_t)i * c.max_pages + j] = p < 0 ? -1 : s_tile[p * width + j - j0];
   }
 }
+__global__ void __launch_bounds__(256)
+k_kv8_reorder_table(const cats_kv8 c, const int* __restrict__ parents, int width) {
+  pdl_wait();
+  pdl_launch_dependents();
+  extern __shared__ int sm[];
+  reorder_table(c, parents, width, blockIdx.x, sm);
+}
 
 // What the copying CTAs are told: one entry per page to copy.
 struct KvCopy {
@@ -438,9 +442,17 @@ struct KvCopy {
 
 // reorder, step 2: lengths, and a page of its own for every child but the first of a parent whose
 // last page is still being filled.
+// table: this one CTA does step 1 as well (a table that is one strip: a launch less).
 __global__ void __launch_bounds__(kPlanThreads)
-k_kv8_reorder_plan(const cats_kv8 c, const int* __restrict__ parents, int* n_copies, KvCopy* copies) {
+k_kv8_reorder_plan(const cats_kv8 c, const int* __restrict__ parents, int* n_copies, KvCopy* copies, int table) {
   pdl_wait();
+  pdl_launch_dependents();
+  if (table) {
+    extern __shared__ int sm[];
+    reorder_table(c, parents, c.max_pages, 0, sm);
+    __threadfence();                                   // the counts' atomics, before they are read below
+    __syncthreads();
+  }
   __shared__ int s_warp[32];
   __shared__ int s_first[kKvMaxSeqs], s_order[kKvMaxSeqs];
   const int i = threadIdx.x, n = c.n_seqs;

@@ -432,36 +432,56 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, done: Option
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda or logits.dim() != 3:
         raise RuntimeError("cats_b200: logits must be a CUDA tensor (n, beams, vocab) (there is no CPU path)")
     dev = logits.device
+    code = _DTYPES[logits.dtype] if logits.dtype in _DTYPES else dtype_code(logits.dtype)
     n, beams, vocab = logits.shape
     s0, s1, s2 = logits.stride()
     ld = s1 if beams > 1 else s0
     if (s2 != 1 and vocab > 1) or (n > 1 and beams > 1 and s0 != beams * s1):
         raise RuntimeError("cats_b200: logits must have contiguous rows at one distance from each other")
-    if n * beams <= 1:
+    rows = n * beams
+    if rows <= 1:
         ld = vocab
     _req(scores, "scores", torch.float32, dev)
-    if scores.numel() != n * beams:
+    if scores.numel() != rows:
         raise RuntimeError(f"cats_b200: scores must hold {n} x {beams} values")
+    ended = None
     if done is not None:
         if done.dtype not in (torch.bool, torch.uint8) or done.device != dev or not done.is_contiguous() \
-                or done.numel() != n * beams:
+                or done.numel() != rows:
             raise RuntimeError(f"cats_b200: done must be a contiguous bool/uint8 tensor with {n} x {beams} values")
         if not 0 <= eos < vocab:
             raise RuntimeError("cats_b200: done needs eos, a token of the vocabulary")
+        ended = done.data_ptr()
     if n < 1 or not 1 <= beams <= 32 or not 1 <= k <= min(32, beams * vocab):
         raise RuntimeError(f"cats_b200: beam selection takes 1 .. 32 beams and 1 .. 32 results (got {n} x {beams}, k {k})")
-    size, stride, new = (n, k), (k, 1), torch.empty_strided
+    size, stride, new, i = (n, k), (k, 1), torch.empty_strided, dev.index
     out_scores = new(size, stride, dtype=torch.float32, device=dev)
     out_rows = new(size, stride, dtype=torch.int32, device=dev)
     out_tokens = new(size, stride, dtype=torch.int64, device=dev)
     out_done = new(size, stride, dtype=torch.bool, device=dev)
     L = _lib.lib()
-    with _on(dev):
-        nbytes = L.cats_beam_select_bytes(n, beams, vocab, k)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        st = L.cats_beam_select(logits.data_ptr(), ld, scores.data_ptr(), _ptr(done), n, beams, vocab, k, eos,
-                                dtype_code(logits.dtype), out_scores.data_ptr(), out_rows.data_ptr(),
-                                out_tokens.data_ptr(), out_done.data_ptr(), ws.data_ptr(), nbytes, _raw_stream(dev.index))
+    if torch._C._cuda_getDevice() != i:
+        with torch.cuda.device(i):
+            return _beam_select(L, logits, ld, scores, ended, k, eos, code, out_scores, out_rows, out_tokens, out_done)
+    return _beam_select(L, logits, ld, scores, ended, k, eos, code, out_scores, out_rows, out_tokens, out_done)
+
+
+_beam_bytes = {}   # scratch of a selection by (device, n, beams, vocab, k)
+
+
+def _beam_select(L, logits, ld, scores, ended, k, eos, code, out_scores, out_rows, out_tokens, out_done):
+    dev = logits.device
+    n, beams, vocab = logits.shape
+    key = (dev.index, n, beams, vocab, k)
+    nbytes = _beam_bytes.get(key)
+    if nbytes is None:
+        if len(_beam_bytes) >= 4096:
+            _beam_bytes.clear()
+        nbytes = _beam_bytes[key] = int(L.cats_beam_select_bytes(n, beams, vocab, k))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    st = L.cats_beam_select(logits.data_ptr(), ld, scores.data_ptr(), ended, n, beams, vocab, k, eos, code,
+                            out_scores.data_ptr(), out_rows.data_ptr(), out_tokens.data_ptr(), out_done.data_ptr(),
+                            ws.data_ptr(), nbytes, _raw_stream(dev.index))
     if st:
         _lib.check(st, "cats_beam_select")
     return out_scores, out_rows, out_tokens, out_done
