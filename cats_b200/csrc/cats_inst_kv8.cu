@@ -36,7 +36,7 @@ int check_tokens(const cats_kv8* c, const int* cu, int tokens, int n_heads) {
 
 // The units of a call have to fit 32 bits (cats_kv8_attn.cuh).
 bool units_fit(const cats_kv8* c, int tokens, int n_heads) {
-  const double units = (double)c->max_pages * c->page / AttnShape<2>::kUnit + 1;
+  const double units = (double)c->max_pages * c->page / AttnShape<2>::kUnit + 1 + AttnShape<2>::kSwitch;
   return units * ((double)tokens * n_heads / AttnShape<1>::kRows + (double)c->n_kv_heads * c->n_seqs) < 2147483648.0;
 }
 
@@ -237,7 +237,8 @@ int cats_beam_select(const void* logits, long long ld, const float* scores, cons
                      int vocab, int k, int eos, int dtype, float* out_scores, int* out_rows, long long* out_tokens,
                      uint8_t* out_done, void* ws, size_t ws_bytes, void* stream) {
   if (!known_dtype(dtype)) return CATS_ERR_DTYPE;
-  if (n < 1 || beams < 1 || beams > kBeamMaxBeams || vocab < 1 || k < 1 || k > kBeamMaxK || ld < vocab)
+  if (n < 1 || beams < 1 || beams > kBeamMaxBeams || vocab < 1 || vocab > (1 << 30) || k < 1 ||
+      k > kBeamMaxK || ld < vocab)
     return CATS_ERR_RANGE;
   if ((long long)n * beams > 65535 || (long long)beams * vocab < k) return CATS_ERR_RANGE;
   if (done && (eos < 0 || eos >= vocab)) return CATS_ERR_RANGE;

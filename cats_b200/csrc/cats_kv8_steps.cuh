@@ -92,21 +92,22 @@ __device__ __forceinline__ void append_queries(const cats_kv8& c, const KvAppend
 #pragma unroll
   for (int k = 0; k < kAhead; ++k)
     if (h0 + k < h1) x[k].load(src + (size_t)(h0 + k) * hd, half);
+  int b;
+  if (!A.cu) {
+    b = t / A.uniform;
+  } else {                                               // last b with cu[b] <= t
+    int lo = 0, hi = c.n_seqs - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (__ldg(A.cu + mid) <= t) lo = mid;
+      else hi = mid - 1;
+    }
+    b = lo;
+  }
+  const KvSpan sp = kv_span(A.cu, A.uniform, b);
+  if (t < sp.first || t - sp.first >= sp.count) return;  // behind the last sequence: left as it is
   bool turn = A.cosv != nullptr;
   if (turn) {
-    int b;
-    if (!A.cu) {
-      b = t / A.uniform;
-    } else {                                             // last b with cu[b] <= t
-      int lo = 0, hi = c.n_seqs - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (__ldg(A.cu + mid) <= t) lo = mid;
-        else hi = mid - 1;
-      }
-      b = lo;
-    }
-    const KvSpan sp = kv_span(A.cu, A.uniform, b);
     const int pos = c.lens[b] - sp.count + (t - sp.first);
     turn = pos >= 0 && pos < c.max_pages * c.page;
     if (turn) rot.load(A.cosv + (size_t)pos * hd + col, A.sinv + (size_t)pos * hd + col, half);

@@ -347,6 +347,8 @@ class CatsDecoder:
                 logs.append(self.logits.clone())
         t1.record(stream)
         t1.synchronize()
+        if self.kv is not None:
+            self.kv.check()
         dt_ms = t0.elapsed_time(t1)
         tps = (n_tokens - 1) * self.B / (dt_ms * 1e-3) if n_tokens > 1 and dt_ms > 0 else float("nan")
         return torch.stack(toks, 1), tps, logs
@@ -360,7 +362,8 @@ class CatsDecoder:
         (``ops.beam_select``); the beams' caches follow by sharing pages (``KVCache8.reorder``).  A beam
         that has produced ``eos`` keeps its score and its place.  Returns (tokens (P, beams, n_tokens),
         ``eos`` behind the end; scores (P, beams), summed log-probability over length **
-        length_penalty), best first.  Steps run on the device alone; nothing is read back."""
+        length_penalty), best first.  The steps run on the device alone; the cache's status is read at
+        the end."""
         if self.kv is None:
             raise RuntimeError('cats_b200.decoder: beam search needs cache="paged8"')
         P, T = input_ids.shape
@@ -417,6 +420,7 @@ class CatsDecoder:
             ended = (tokens == end).int().cumsum(-1) > 0
             lengths = (n_tokens + 1 - ended.sum(-1)).clamp(max=n_tokens)
         final = state[0] / lengths.to(torch.float32) ** length_penalty
+        self.kv.check()
         order = final.argsort(dim=-1, descending=True, stable=True)
         return tokens.gather(1, order[..., None].expand_as(tokens)), final.gather(1, order)
 

@@ -442,7 +442,8 @@ int cats_kv8_grow(const cats_kv8* cache, const int* cu, int n_new, void* stream)
  * The rotation is computed in fp32; q_out is rounded once, keys and values are quantised from fp32.
  * A page's exponent is the least that holds its largest finite magnitude within 448 codes; where a
  * page already holds rows it only grows, and the older codes are rescaled (exact but for codes that
- * become subnormal).  Rows must be 16-byte aligned (qkv, ld, tables, q_out).
+ * become subnormal).  Rows must be 16-byte aligned (qkv, ld, tables, q_out).  Rows behind the last
+ * sequence's (a padded call) are left as they are in q_out.
  */
 int cats_kv8_append(const cats_kv8* cache, int layer, const void* qkv, long long ld, const int* cu,
                     int n_tokens, const void* cos_table, const void* sin_table, int rope_len,
@@ -454,7 +455,8 @@ int cats_kv8_append(const cats_kv8* cache, int layer, const void* qkv, long long
  *   out = sum_p softmax_p(scale * q . k_p) v_p   over the positions p of the token's sequence up to
  * its own; key head h / (n_heads / n_kv_heads).  Scores, softmax and sums in fp32.  A token without
  * any position (an empty sequence) gives zeros; pages listed as -1 are left out (status bit 2).
- * Positions behind the token are never read into its result, whatever they hold.
+ * Positions behind the token never reach its result, whatever they hold; rows behind the last
+ * sequence's are left as they are in out.
  *   out [n_tokens, n_heads, head_dim]; ws: cats_kv8_attend_bytes(...) bytes of scratch, contents
  *   irrelevant before and after.
  */
@@ -492,7 +494,7 @@ int cats_kv8_compact(const cats_kv8* cache, int* n_live, void* ws, size_t ws_byt
  * the token is eos.  Tokens at -inf come last; a beam whose score or log-sum-exp is not finite (a NaN
  * or +inf among its logits, all of them -inf) has only candidates at -inf.  The log-sum-exp is summed
  * in fp32 over at most a few thousand values and in fp64 above that; candidates are compared in fp64.
- *   beams <= 32, k <= 32, k <= beams * vocab, n * beams <= 65535.  ws: cats_beam_select_bytes(...) bytes of scratch.
+ *   beams <= 32, k <= 32, k <= beams * vocab, vocab <= 2^30, n * beams <= 65535.  ws: cats_beam_select_bytes(...) bytes of scratch.
  */
 size_t cats_beam_select_bytes(int n, int beams, int vocab, int k);
 int cats_beam_select(const void* logits, long long ld, const float* scores, const uint8_t* done, int n,

@@ -80,6 +80,7 @@ def test_bad_selections_are_refused(buf):
     assert sel(done=buf, eos=-1) == -9 and sel(done=buf, eos=100) == -9
     assert sel(x=None) == -4 and sel(sc=None) == -4
     assert sel(x=buf + 1) == -3 and sel(nb=16) == -5
+    assert sel(n=65536, beams=1) == -9 and sel(vocab=(1 << 30) + 1, ld=1 << 31) == -9
 
 
 def test_python_front_end_refuses_cpu_tensors():
@@ -92,6 +93,17 @@ def test_python_front_end_refuses_cpu_tensors():
         kv8.KVCache8.from_tensors(z(1, 4, 2, 2, 16, 64, dt=torch.uint8), z(1, 4, 2, 2, dt=torch.float32), z(2, 4), z(2), z(4))
     with pytest.raises(RuntimeError, match="codes"):
         kv8.KVCache8.from_tensors(z(1, 4, 2, 2, 16, 64), z(1, 4, 2, 2, dt=torch.float32), z(2, 4), z(2), z(4))
+
+
+def test_the_decoders_paged_cache_needs_a_gpu():
+    from transformers import MistralConfig, MistralForCausalLM
+
+    from cats_b200 import decoder as D
+
+    cfg = MistralConfig(hidden_size=64, intermediate_size=96, num_hidden_layers=1, num_attention_heads=2,
+                        num_key_value_heads=1, vocab_size=64, max_position_embeddings=64)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        D.CatsDecoder(MistralForCausalLM(cfg), 1, 64, mlp="dense", cache="paged8")
 
 
 def test_the_oracles_e4m3_is_the_format():

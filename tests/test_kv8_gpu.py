@@ -126,6 +126,37 @@ def test_many_short_sequences(n, cuda_device):
     attend_and_compare(c, [1] * n, 2, torch.float16, uniform=True)
 
 
+@pytest.mark.parametrize("dt", list(TYPES))
+@pytest.mark.parametrize("hd,page,group", [(32, 16, 3), (96, 32, 6), (64, 128, 1), (128, 16, 2)])
+def test_many_sequences_with_several_tokens(hd, page, group, dt, cuda_device):
+    lens = [5 + 53 * i % 211 for i in range(40)]
+    c = filled(cuda_device, lens, page, 1, hd)
+    attend_and_compare(c, [min(n, 1 + 29 * i % 37) for i, n in enumerate(lens)], group, TYPES[dt])
+
+
+@pytest.mark.parametrize("dt", ["f16", "f32"])
+@pytest.mark.parametrize("hd,counts", [(128, [130, 40, 1]), (64, [64, 300, 7]), (32, [40, 33, 9]), (96, [2, 2, 1])])
+def test_long_sequences_with_many_tokens(hd, counts, dt, cuda_device):
+    """Several tiles of rows, split over CTAs and joined."""
+    c = filled(cuda_device, [3000, 411, 9], 64, 2, hd)
+    attend_and_compare(c, counts, 2, TYPES[dt])
+
+
+def test_a_padded_call_leaves_the_rows_behind(cuda_device):
+    for dt in TYPES.values():
+        for counts in ([1, 0, 1], [20, 3, 1]):
+            c = filled(cuda_device, [40, 33, 7], 16, 2, 64)
+            n = sum(counts)
+            cu, cos = cu_of(counts, cuda_device), tables(c.max_len, 64, dt, cuda_device)
+            qkv = torch.randn((n + 5, 8 * 64), device=cuda_device).to(dt)
+            q = torch.full((n + 5, 4, 64), 7.0, device=cuda_device, dtype=dt)
+            out = torch.full_like(q, 9.0)
+            c.append(0, qkv, 4, *cos, cu=cu, q_out=q)
+            c.attend(0, q, cu=cu, out=out)
+            assert (q[n:] == 7).all() and (out[n:] == 9).all() and (out[:n] != 9).any()
+            c.check()
+
+
 def test_scores_of_any_size(cuda_device):
     """Peaked and flat softmax, large and tiny scales of pages, queries beyond half precision's range."""
     c = filled(cuda_device, [150, 90], 16, 2, 64)
