@@ -18,6 +18,10 @@ namespace cats {
 // Rounding: products and sums of the rotation are each rounded to fp32 (no contraction), the query
 // once more to its type; keys and values go from fp32 straight to e4m3.  Infinities are stored as
 // NaN (e4m3 has none) and neither sets a scale.
+// Measured: a decode step of eight sequences 2.8 us, all of it the launch and three dependent loads
+// (length, page, row); four prompts of 700 .. 4096 tokens, 32 + 2 x 32 heads of 128, bf16, 346 MB: 80 us,
+// 4.3 TB/s, bound by instructions (rotation, unpacking and packing of 10 to 14 per element) beside the
+// loads; with one block of rows per CTA and no loads under way it was 130 us.
 template <typename T>
 struct KvAppendArgs {
   const T* qkv;
@@ -289,6 +293,8 @@ __global__ void __launch_bounds__(RPT == 1 ? 32 : 256, RPT == 1 ? 16 : RPT == 2 
 // ---------------------------------------------------------------------------------------------
 // Free pages are those with refs == 0; the lowest ids are handed out first, in the order of the
 // sequences, so that the result does not depend on the order in which threads run.
+// Measured: 16 beams, five copies of the filled part of a page in 32 layers, 22 MB copied: 12.5 us (three
+// launches 13.1); a compaction that moves 258 MB: 101 us, 5.3 TB/s read and written.
 
 // exclusive block scan over kPlanThreads values; total through *sum
 __device__ __forceinline__ int plan_scan(int v, int* s_warp, int* sum) {
