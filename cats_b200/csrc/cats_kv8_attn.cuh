@@ -149,7 +149,12 @@ struct AttnPlan {
 // than the joining costs.
 template <int NQ>
 __device__ __forceinline__ int attn_pieces(const AttnPlan& p, int units) {
-  const int n = min(1 + (int)((float)units * (float)p.spare / (float)p.total), units);
+  int n = min(1 + (int)((float)units * (float)p.spare / (float)p.total), units);
+  // parts of 128 rows (66 KB) are joined one after the other, about two to the time of a unit: n parts
+  // cost units / n + n / 2 (548 rows over 9000 positions: 84 us with 28 parts a segment)
+  // small parts cost a thirtieth of a unit (one sequence of 131000 positions with one key head: 35 us
+  // with 148 parts)
+  n = min(n, (int)sqrtf((NQ == 16 ? 2.f : 16.f) * (float)units) + 1);
   return (units + n - 1) / n + AttnShape<NQ>::kJoin >= units ? 1 : n;
 }
 // the time of a segment's CTA, in units
@@ -384,7 +389,7 @@ __device__ __forceinline__ int attn_share(const AttnTable& tab, const AttnPlan& 
   const int each = s.units + AttnShape<NQ>::kSwitch, r = w - tab.cost[b], seg = r / each;
   int unit = max(r - seg * each - AttnShape<NQ>::kSwitch, 0);
   constexpr int kNear = 256 / AttnShape<NQ>::kUnit;
-  if (q < 12 * kNear) {
+  if (q < 16 * kNear) {
     if (unit <= kNear) unit = 0;
     else if (s.units - unit <= kNear) unit = s.units;
   }
@@ -925,13 +930,34 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
             if (e < items && set < sets) {
               const int r = e / (HD / 4), d = (e - r * (HD / 4)) * 4;
+              auto part_of = [&](int x) {                // (only c0 can have another segment first)
+                const int slot = x > c0 || first_begins >= u0 ? 0 : 1;
+                return A.parts + (size_t)(2 * x + slot) * attn_part_floats(S::kRows, HD) + (size_t)r * (HD + 2);
+              };
+              if (c1 - c0 < 8) {
+                for (int x = c0 + set; x <= c1; x += sets) {
+                  const float* src = part_of(x);
+                  const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + HD));
+                  const float2 a = __ldcg(reinterpret_cast<const float2*>(src + d)), b = __ldcg(reinterpret_cast<const float2*>(src + d + 2));
+                  attn_add(ml.x, ml.y, make_float4(a.x, a.y, b.x, b.y), top, sum, v);
+                }
+              } else {                                   // many: the largest reference first, then the parts'
+                                                         // weights do not wait for one another
+#pragma unroll 8
+                for (int x = c0 + set; x <= c1; x += sets) top = fmaxf(top, __ldcg(part_of(x) + HD));
+                const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll 4
-              for (int x = c0 + set; x <= c1; x += sets) {
-                const int slot = x > c0 || first_begins >= u0 ? 0 : 1;     // only c0 can have another segment first
-                const float* src = A.parts + (size_t)(2 * x + slot) * attn_part_floats(S::kRows, HD) + (size_t)r * (HD + 2);
-                const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + HD));
-                const float2 a = __ldcg(reinterpret_cast<const float2*>(src + d)), b = __ldcg(reinterpret_cast<const float2*>(src + d + 2));
-                attn_add(ml.x, ml.y, make_float4(a.x, a.y, b.x, b.y), top, sum, v);
+                for (int x = c0 + set; x <= c1; x += sets) {
+                  const float* src = part_of(x);
+                  const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + HD));
+                  const float2 a = __ldcg(reinterpret_cast<const float2*>(src + d)), b = __ldcg(reinterpret_cast<const float2*>(src + d + 2));
+                  const float by = ex2(ml.x - ref);      // saw nothing: 0 (and a NaN sum stays one)
+                  sum = fmaf(ml.y, by, sum);
+                  v.x = fmaf(a.x, by, v.x);
+                  v.y = fmaf(a.y, by, v.y);
+                  v.z = fmaf(b.x, by, v.z);
+                  v.w = fmaf(b.y, by, v.w);
+                }
               }
             }
             if (sets > 1) {

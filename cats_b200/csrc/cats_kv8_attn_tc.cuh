@@ -436,6 +436,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_kv8_attend_tc(const cats_kv8 
             sum[k] = 0.f;
             v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
           }
+#pragma unroll 2
           for (int x = c0; x <= c1; ++x) {
             const int slot = x > c0 || first_begins >= u0 ? 0 : 1;
             const float* src = A.parts + (size_t)(2 * x + slot) * attn_part_floats(kTcRows, HD);
