@@ -28,11 +28,10 @@ static cudaError_t run_attend(const cats_kv8& c, const KvAttnArgs<T>& A, cudaStr
 }
 
 // Up to 8 rows and up to 16 the tiles of cats_kv8_attn.cuh, bound by the codes' bytes; beyond that the
-// products count.  16-bit queries then take tiles of 128 rows on tcgen05, also where only some of the
-// rows are used (a step of 128 positions takes 3.2 us there whatever the rows; tiles of 32 rows take
-// about as long for 32 rows and in proportion for more: 2 x 256 tokens x 4 heads per key head 212 us
-// against 125); head_dim 32 and 96, which do not fill a 128-byte swizzle row, tiles of 32 rows; fp32
-// queries, which are split in two halves and leave no registers for more, tiles of 16.
+// products count.  A CTA takes 128 positions of 32 rows in 1.9 us with those tiles, and of up to 128
+// rows in 3.2 us on tcgen05 (2 x 256 tokens x 4 heads per key head, head_dim 128: 212 and 125 us): 16-bit
+// queries with more than 32 rows go there, but for head_dim 32 and 96, which do not fill a 128-byte
+// swizzle row.  fp32 queries are split in two halves, which leaves registers for 16 rows.
 template <typename T, int HD>
 static cudaError_t run_attend(const cats_kv8& c, const KvAttnArgs<T>& A, cudaStream_t st) {
   const long long rows = attn_rows(c, A.tokens, A.nh);
@@ -41,10 +40,10 @@ static cudaError_t run_attend(const cats_kv8& c, const KvAttnArgs<T>& A, cudaStr
     if (rows > kAttnFewRows) {
       if constexpr (HD % 64 == 0) {
         static bool ready[64];
-        return run_large<T>(k_kv8_attend_tc<T, HD>, ready, kTcThreads, attn_tc_smem(HD), c, A, st);
-      } else {
-        return run_attend<T, HD, 4>(c, A, st);
+        if (rows > kAttnSomeRows)
+          return run_large<T>(k_kv8_attend_tc<T, HD>, ready, kTcThreads, attn_tc_smem(HD), c, A, st);
       }
+      return run_attend<T, HD, 4>(c, A, st);
     }
   }
   return run_attend<T, HD, 2>(c, A, st);

@@ -71,7 +71,7 @@ struct KvAttnArgs {
 __host__ __device__ inline long long attn_rows(const cats_kv8& c, int tokens, int nh) {
   return ((long long)tokens + c.n_seqs - 1) / c.n_seqs * (nh / c.n_kv_heads);
 }
-constexpr int kAttnFewRows = 16;                        // up to here 8 or 16 rows a tile
+constexpr int kAttnFewRows = 16, kAttnSomeRows = 32;    // up to here 8 or 16, 32 rows a tile
 inline int attn_part_rows(const cats_kv8& c, int tokens, int nh) {
   return attn_rows(c, tokens, nh) > kAttnFewRows ? 128 : 16;
 }
