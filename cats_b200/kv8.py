@@ -14,8 +14,9 @@ excepted), so a decode step over the cache can sit in a CUDA graph::
         o = cache.attend(l, q)                      # causal attention over it
     cache.reorder(parents)                          # sequence i continues sequence parents[i]
 
-The calls on one cache have to be ordered: one stream, or events between streams.  Its tensors keep
-their addresses; they may be read and filled in place.
+The calls on one cache have to be ordered, those that only read it too (they share scratch): one
+stream, or events between streams; so do the replays of graphs that hold them.  Its tensors keep their
+addresses; they may be read and filled in place.
 """
 from __future__ import annotations
 
@@ -93,9 +94,14 @@ class KVCache8:
         self._p = ctypes.byref(self._c)
         self._index = codes.device.index
         lib = _lib.lib()
-        self._attend_nbytes = {}                # by (tokens, heads)
-        self._reorder_nbytes = int(lib.cats_kv8_reorder_bytes(self._p))
-        self._compact_nbytes = int(lib.cats_kv8_compact_bytes(self._p))
+        # Scratch of the calls, which are ordered anyway (see the module docstring), for the cache's life.
+        # Only attention of many rows per key head (new tokens x heads) needs more: a buffer of its own.
+        with torch.cuda.device(self._index):
+            small = int(lib.cats_kv8_attend_bytes(self._p, self.n_seqs, nkv))
+        self._attend_nbytes = {(self.n_seqs, nkv): small}     # by (tokens, heads)
+        self._ws = torch.empty(max(small, int(lib.cats_kv8_reorder_bytes(self._p)), int(lib.cats_kv8_compact_bytes(self._p))),
+                               dtype=torch.uint8, device=codes.device)
+        self._ws_ptr, self._ws_nbytes = self._ws.data_ptr(), self._ws.numel()
 
     def _call(self, what: str, *args) -> None:
         """One C call on the current stream of the cache's device."""
@@ -205,9 +211,12 @@ class KVCache8:
             if len(self._attend_nbytes) >= 4096:
                 self._attend_nbytes.clear()
             self._attend_nbytes[(n, nh)] = nbytes
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        ws = self._ws_ptr
+        if nbytes > self._ws_nbytes:
+            large = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+            ws = large.data_ptr()
         self._call("cats_kv8_attend", layer, q.data_ptr(), q.stride(0) if n > 1 else nh * hd, self._cu(cu), n, nh,
-                   hd ** -0.5 if scale is None else scale, out.data_ptr(), ws.data_ptr(), nbytes, code)
+                   hd ** -0.5 if scale is None else scale, out.data_ptr(), ws, nbytes, code)
         return out
 
     # ---- pages --------------------------------------------------------------------------------------------
@@ -218,8 +227,7 @@ class KVCache8:
         if not isinstance(parents, torch.Tensor) or parents.dtype != torch.int32 or parents.device != self.device \
                 or not parents.is_contiguous() or parents.numel() != self.n_seqs:
             raise _bad(f"parents must be a contiguous int32 tensor of {self.n_seqs} elements on {self.device}")
-        ws = torch.empty(self._reorder_nbytes, dtype=torch.uint8, device=self.device)
-        self._call("cats_kv8_reorder", parents.data_ptr(), ws.data_ptr(), self._reorder_nbytes)
+        self._call("cats_kv8_reorder", parents.data_ptr(), self._ws_ptr, self._ws_nbytes)
 
     def _host_parents(self, changes) -> torch.Tensor:
         parents = list(range(self.n_seqs))
@@ -246,8 +254,7 @@ class KVCache8:
         """Move the live pages to the front of the pool (``cats_kv8_compact``).  Returns their number
         as a 0-dim int32 device tensor; the page ids from there on are free."""
         n = torch.empty((), dtype=torch.int32, device=self.device)
-        ws = torch.empty(self._compact_nbytes, dtype=torch.uint8, device=self.device)
-        self._call("cats_kv8_compact", n.data_ptr(), ws.data_ptr(), self._compact_nbytes)
+        self._call("cats_kv8_compact", n.data_ptr(), self._ws_ptr, self._ws_nbytes)
         return n
 
     def reset(self) -> None:

@@ -710,6 +710,25 @@ def test_two_searches_at_once_on_two_streams(cuda_device):
             assert all(torch.equal(u, v) for u, v in zip(x, y))
 
 
+def test_work_handed_to_another_stream(cuda_device):
+    """Work handed over by an event to another stream, on scratch that the cache keeps."""
+    c, d = (filled(cuda_device, [700, 31, 90], 64, 2, 128, seed=3) for _ in range(2))
+    q = torch.randn((3, 8, 128), device=cuda_device).half()
+    many = torch.randn((60, 8, 128), device=cuda_device).half()
+    cu = cu_of([25, 5, 30], cuda_device)
+    want = [c.attend(0, q), c.attend(0, many, cu=cu)]
+    side = torch.cuda.Stream(cuda_device)
+    side.wait_stream(torch.cuda.current_stream(cuda_device))
+    with torch.cuda.stream(side):
+        got = [d.attend(0, q), d.attend(0, many, cu=cu)]
+        d.reorder(torch.tensor([1, 1, 0], dtype=torch.int32).to(cuda_device))
+        d.compact()
+    torch.cuda.current_stream(cuda_device).wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    assert d.lens.tolist() == [31, 31, 700]
+    d.check()
+
+
 def test_results_do_not_depend_on_the_run(cuda_device):
     c = filled(cuda_device, [5000, 31, 700], 64, 2, 128)
     q = torch.randn((3, 8, 128), device=cuda_device).half()
