@@ -18,7 +18,7 @@
 // p' = exp2(s + ev - m) with m the running maximum of s + ev, so that p' <= 1 whatever the scales,
 // and the softmax's sum is that of p' 2^-ev.
 //
-// Work: a unit is 16 positions for each warp of one tile (8 or 16 rows) of one key head.  All units
+// Work: a unit is 16 positions for each warp of one tile (8, 16 or 32 rows) of one key head.  All units
 // of the call in a row - sequences, heads, tiles, positions - are dealt out to one CTA per SM in
 // equal, contiguous shares, whatever the lengths of the sequences, and computed from the lengths on
 // the device; a (head, tile) that one CTA has whole is written at once, the parts of the others are
@@ -26,7 +26,7 @@
 //
 // Measured (head_dim 128, 8 key heads): 16 sequences of 32768 positions 171 us, 6.27 TB/s of codes (0.95
 // of a plain copy's rate); 32 sequences of 1000 .. 32000, 603 MB: 108 to 115 us; 8 sequences of 512 ..
-// 1536: 13.8 us, where the chain launch - lengths - page - codes - join is what takes the time.
+// 1536: 14 us, where the chain launch - lengths - page - codes - join is what takes the time.
 #pragma once
 
 #include "cats_kv8.cuh"
