@@ -14,14 +14,15 @@ namespace cats {
 // rows are read once and stay in registers between the two (at most RPT rows of a thread).  hd / 16
 // threads share a row; a thread holds eight values of the row's first half and the eight that the
 // rotation pairs them with.  Further CTAs of the same launch rotate the queries: a thread keeps its
-// token's cosines and sines and goes through the heads, two of them on their way.
+// token's cosines and sines and goes through the heads, four of them on their way.
 // Rounding: products and sums of the rotation are each rounded to fp32 (no contraction), the query
 // once more to its type; keys and values go from fp32 straight to e4m3.  Infinities are stored as
 // NaN (e4m3 has none) and neither sets a scale.
 // Measured: a decode step of eight sequences 2.8 us, all of it the launch and three dependent loads
-// (length, page, row); four prompts of 700 .. 4096 tokens, 32 + 2 x 32 heads of 128, bf16, 346 MB: 80 us,
-// 4.3 TB/s, bound by instructions (rotation, unpacking and packing of 10 to 14 per element) beside the
-// loads; with one block of rows per CTA and no loads under way it was 130 us.
+// (length, page, row); four prompts of 700 .. 4096 tokens, 32 + 2 x 32 heads of 128, bf16, 346 MB: 73 us,
+// 4.7 TB/s (the queries alone 28 us, 5 TB/s; keys and values, 256-byte pieces of far rows, 66 us); with one
+// block of rows per CTA and no loads under way it was 130 us.  Two CTAs of 256 threads an SM: with three,
+// 80 registers each, values are spilled (80 us; 8000 fp32 tokens of 32 + 2 x 8 heads: 92 us, 62 with two).
 template <typename T>
 struct KvAppendArgs {
   const T* qkv;
@@ -90,7 +91,7 @@ __device__ __forceinline__ void append_queries(const cats_kv8& c, const KvAppend
   if (r0 >= side || t >= A.tokens) return;
   const T* src = A.qkv + (size_t)t * A.ld + col;
   T* dst = A.q_out + (size_t)t * A.nh * hd + col;
-  constexpr int kAhead = 2;                              // heads on their way
+  constexpr int kAhead = 4;                              // heads on their way
   Raw16<T> x[kAhead];
   Turn rot;
 #pragma unroll
@@ -132,14 +133,14 @@ __device__ __forceinline__ void append_queries(const cats_kv8& c, const KvAppend
 }
 
 template <typename T, int RPT>
-__global__ void __launch_bounds__(RPT == 1 ? 32 : 256, RPT == 1 ? 16 : RPT == 2 ? 3 : 2) k_kv8_append(const cats_kv8 c, const KvAppendArgs<T> A) {
+__global__ void __launch_bounds__(RPT == 1 ? 32 : 256, RPT == 1 ? 16 : 2) k_kv8_append(const cats_kv8 c, const KvAppendArgs<T> A) {
   pdl_wait();
   pdl_launch_dependents();
   if ((int)blockIdx.x >= A.kv_blocks) {
     append_queries(c, A, blockIdx.x - A.kv_blocks);
     return;
   }
-  __shared__ float s_max[8];
+  __shared__ __align__(16) float s_max[2][8];
   const int hd = c.head_dim, half = hd >> 1, tpr = hd >> 4, nkv = c.n_kv_heads;
   const int side = blockDim.x / tpr;
   const int r0 = threadIdx.x / tpr, col = (threadIdx.x - r0 * tpr) * 8;
@@ -203,14 +204,17 @@ __global__ void __launch_bounds__(RPT == 1 ? 32 : 256, RPT == 1 ? 16 : RPT == 2 
     if (threadIdx.x == 0) kv_flag(c, KV_BAD_PAGE);
     return;
   }
+  // (magnitudes: their order is that of their bits; the words of the call before last are free again)
+  if (threadIdx.x < 16 && (threadIdx.x & 7) >= (blockDim.x >> 5)) s_max[threadIdx.x >> 3][threadIdx.x & 7] = 0.f;
+  int turn_of = 0;
   auto block_max = [&](float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    v = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
     if (RPT > 1) {
+      if ((threadIdx.x & 31) == 0) s_max[turn_of][threadIdx.x >> 5] = v;
       __syncthreads();
-      if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = v;
-      __syncthreads();
-      for (int w = 0; w < (int)(blockDim.x >> 5); ++w) v = fmaxf(v, s_max[w]);
+      const float4 a = *reinterpret_cast<const float4*>(s_max[turn_of]), b = *reinterpret_cast<const float4*>(s_max[turn_of] + 4);
+      v = fmaxf(fmaxf(fmaxf(a.x, a.y), fmaxf(a.z, a.w)), fmaxf(fmaxf(b.x, b.y), fmaxf(b.z, b.w)));
+      turn_of ^= 1;
     }
     return v;
   };
