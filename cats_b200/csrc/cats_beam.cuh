@@ -137,8 +137,8 @@ __global__ void __launch_bounds__(kBeamThreads, 4) k_beam_rows(const BeamArgs A)
       for (int i = 0; i < N; ++i) top = fmaxf(top, f[k][i]);     // (drops NaN)
     if (top > m) {
       const float to = top * kLog2e;
-      sum *= beam_exp2(fabsf(ref) <= kFar && fabsf(to) <= kFar ? ref - to : (m - top) * kLog2e);
-      if (m == -CUDART_INF_F && sum == sum) sum = 0.f;
+      // (while nothing has been summed there is no m to come from: the sum is 0, or NaN after a NaN)
+      if (m > -CUDART_INF_F) sum *= beam_exp2(fabsf(ref) <= kFar && fabsf(to) <= kFar ? ref - to : (m - top) * kLog2e);
       m = top;
       ref = to;
     }
