@@ -57,7 +57,10 @@ constexpr int kBeamPer = 16;                           // values of a thread and
 constexpr int kBeamTile = kBeamThreads * kBeamPer;
 constexpr int kBeamCap = 1024;                         // candidates that a CTA can hold
 
-constexpr float kLog2e = 1.4426950408889634f, kFar = 1e37f;
+// Up to kFar a reference ref = rn(m log2e) is off from m log2e by at most 2^-4 (half a step of fp32), so that
+// 2^(x log2e - ref) is at most 2^(1/16) and its sum can be put right at the end; beyond it the steps grow to where
+// that exponential is infinite or 0 at x = m, and the difference x - m is taken first.
+constexpr float kLog2e = 1.4426950408889634f, kFar = 1048576.f;
 __device__ __forceinline__ float beam_exp2(float d) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
@@ -138,12 +141,17 @@ __global__ void __launch_bounds__(kBeamThreads, 4) k_beam_rows(const BeamArgs A)
     if (top > m) {
       const float to = top * kLog2e;
       // (while nothing has been summed there is no m to come from: the sum is 0, or NaN after a NaN)
-      if (m > -CUDART_INF_F) sum *= beam_exp2(fabsf(ref) <= kFar && fabsf(to) <= kFar ? ref - to : (m - top) * kLog2e);
+      if (m > -CUDART_INF_F) {
+        const bool was = fabsf(ref) <= kFar, is = fabsf(to) <= kFar;
+        float by = was && is ? ref - to : (m - top) * kLog2e;
+        if (was != is) by += was ? -fmaf(m, kLog2e, -ref) : fmaf(top, kLog2e, -to);   // relative to 2^ref on one side only
+        sum *= beam_exp2(by);
+      }
       m = top;
       ref = to;
     }
     // 2^(x log2e - ref), one rounding: ref is only near m log2e, which the end of the kernel makes up
-    // for.  Next to the type's ends (masks of its lowest value) m log2e is not a number any more.
+    // for.  Far from zero (masks of large negative numbers) the difference comes first.
     float part = 0.f;
     if (fabsf(ref) <= kFar) {
 #pragma unroll

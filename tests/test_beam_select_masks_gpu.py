@@ -30,3 +30,31 @@ def test_finite_masks_leave_the_beam_in(mask, dt, cuda_device):
         select_and_compare(x, s, 7)
     x, s = masked(TYPES[dt], 9000, [], mask, cuda_device)
     select_and_compare(x, s, 5)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("size", [7e5, 3e6, 1e10, 3e12, 1e20, 1e30])
+def test_logits_far_from_zero(size, dt, cuda_device):
+    """Masks that a threshold near zero does not catch, and rows that lie far from zero as a whole."""
+    for sign in (1, -1):
+        for vocab, kept in ((700, [5, 333]), (40000, [3, 39990]), (5000, list(range(0, 5000, 7)))):
+            if sign < 0:                                   # masked by a large negative number
+                x, s = masked(TYPES[dt], vocab, kept, -size, cuda_device)
+                select_and_compare(x, s, 2)
+                select_and_compare(x, s, 6)
+            g = torch.Generator().manual_seed(vocab)       # all of the row there
+            x = torch.full((1, 3, vocab), sign * size)
+            x[0, 1] *= 1 - 0.5 * torch.rand(vocab, generator=g)
+            x[0, 2, ::3] *= 0.75
+            select_and_compare(x.to(TYPES[dt]).to(cuda_device), (-torch.rand((1, 3), generator=g)).to(cuda_device), 6)
+
+
+def test_rows_across_the_border_of_the_two_exponentials(cuda_device):
+    """Maxima that rise from tile to tile through 2^20 / log2(e) = 726817, up and down, half a unit a tile."""
+    n = 60000
+    ramp = 726817 + (torch.arange(n) // 4096 - 7).float() * 0.5
+    x = torch.stack((ramp, ramp.flip(0), -ramp, -ramp.flip(0)))[None]
+    for at in (0, 5000, 59000):
+        y = x.clone()
+        y[:, :, at] = y.amax(-1) + 0.25
+        select_and_compare(y.to(cuda_device), torch.tensor([[-1.0, -1.25, -1.5, -1.75]], device=cuda_device), 5)
