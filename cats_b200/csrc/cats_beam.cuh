@@ -55,6 +55,9 @@ struct BeamArgs {
 
 constexpr int kBeamPer = 16;                           // values of a thread and tile
 constexpr int kBeamTile = kBeamThreads * kBeamPer;
+// A thread adds up this many tiles (512 values) in fp32, the rest in fp64: at most 48 roundings in a row, 2^-18 of
+// the sum.
+constexpr int kBeamFold = 32;
 constexpr int kBeamCap = 1024;                         // candidates that a CTA can hold
 
 // Up to kFar a reference ref = rn(m log2e) is off from m log2e by at most 2^-4 (half a step of fp32), so that
@@ -121,6 +124,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4) k_beam_rows(const BeamArgs A)
   };
   fetch(v0);
   float m = -CUDART_INF_F, ref = 0.f, sum = 0.f, tau = -CUDART_INF_F;
+  double whole_sum = 0;                                // of the tiles before the last few (kBeamFold)
   for (int base = v0; base < v1; base += kBeamThreads * NV) {
     float f[NV][N];
 #pragma unroll
@@ -145,7 +149,9 @@ __global__ void __launch_bounds__(kBeamThreads, 4) k_beam_rows(const BeamArgs A)
         const bool was = fabsf(ref) <= kFar, is = fabsf(to) <= kFar;
         float by = was && is ? ref - to : (m - top) * kLog2e;
         if (was != is) by += was ? -fmaf(m, kLog2e, -ref) : fmaf(top, kLog2e, -to);   // relative to 2^ref on one side only
-        sum *= beam_exp2(by);
+        by = beam_exp2(by);
+        sum *= by;
+        whole_sum *= by;
       }
       m = top;
       ref = to;
@@ -213,8 +219,12 @@ __global__ void __launch_bounds__(kBeamThreads, 4) k_beam_rows(const BeamArgs A)
         if (at < kBeamCap) s_keys[at] = beam_key(VecT<T>::to_f(x[e]), e);
       }
     }
-    // after 2, 4, 8 ... tiles: the k-th largest so far is the threshold of the next
     const int tiles = (base - v0) / (kBeamThreads * NV) + 1;
+    if (tiles % kBeamFold == 0) {
+      whole_sum += sum;
+      sum = 0.f;
+    }
+    // after 2, 4, 8 ... tiles: the k-th largest so far is the threshold of the next
     if (tiles > 1 && (tiles & (tiles - 1)) == 0 && base + kBeamThreads * NV < v1) {
       __syncthreads();
       const int n = s_count;
@@ -231,12 +241,13 @@ __global__ void __launch_bounds__(kBeamThreads, 4) k_beam_rows(const BeamArgs A)
   }
   // Sum relative to m instead of 2^ref: both products are with the same constant, so what is left of
   // its error is a factor of (x - m)
-  if (m > -CUDART_INF_F && fabsf(ref) <= kFar) sum *= beam_exp2(-fmaf(m, kLog2e, -ref));
+  whole_sum += sum;
+  if (m > -CUDART_INF_F && fabsf(ref) <= kFar) whole_sum *= beam_exp2(-fmaf(m, kLog2e, -ref));
   // maximum and sum of the part
   float top = m;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  double all = top == -CUDART_INF_F ? (sum == sum ? 0.0 : (double)sum) : (double)(sum * beam_exp2((m - top) * kLog2e));
+  double all = top == -CUDART_INF_F ? (whole_sum == whole_sum ? 0.0 : whole_sum) : whole_sum * beam_exp2((m - top) * kLog2e);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
   if (lane == 0) {

@@ -58,3 +58,25 @@ def test_rows_across_the_border_of_the_two_exponentials(cuda_device):
         y = x.clone()
         y[:, :, at] = y.amax(-1) + 0.25
         select_and_compare(y.to(cuda_device), torch.tensor([[-1.0, -1.25, -1.5, -1.75]], device=cuda_device), 5)
+
+
+def test_sums_of_very_many_values(cuda_device):
+    """Thirty-two rows of 16.8 M equal logits with a few larger ones, one to a thread and part: a thread adds
+    thousands of values, always with the same rounding.  Of a sum of positive numbers: exponentials 2^-21, 48
+    roundings in fp32 (32 tiles and the 16 values of one) 2^-18.4, fp64 above that, the part's sum as fp32 2^-24."""
+    from cats_b200 import ops
+
+    parts, tiles = 6, 683
+    vocab = 4096 * parts * tiles
+    low = (-0.5 - torch.arange(32) * 0.17).half()          # of each beam
+    x = low.to(cuda_device).view(1, 32, 1).expand(1, 32, vocab).contiguous()
+    first = (torch.arange(parts)[:, None] * (4096 * tiles) + torch.arange(256) * 8).view(-1)
+    x[:, :, first.to(cuda_device)] = 0
+    x[:, :, 0] = 1
+    lse = torch.log(torch.e + (len(first) - 1) + (vocab - len(first)) * torch.exp(low.double()))
+    scores = (lse - 1).float().view(1, 32)                 # every beam's best comes out near zero
+    got = ops.beam_select(x, scores.to(cuda_device), 32)
+    rows = got[1].view(-1).long().cpu()
+    want = (scores.double().view(-1) + 1 - lse)[rows]
+    assert sorted(rows.tolist()) == list(range(32)) and int(got[2].abs().max()) == 0
+    assert float((got[0].double().view(-1).cpu() - want).abs().max()) <= 2.0 ** -18 + 2.0 ** -21 + 2.0 ** -23
