@@ -258,15 +258,16 @@ class KVCache8:
         return n
 
     def reset(self) -> None:
-        """All sequences empty, all pages free."""
+        """All sequences empty, all pages free, nothing recorded (see ``check``)."""
         self.table.fill_(-1)
         self.lens.zero_()
         self.refs.zero_()
+        self._state.zero_()
 
     # ---- host side ---------------------------------------------------------------------------------------------
     def check(self) -> None:
         """Raise if a kernel found device data that does not fit (synchronises).  The status word
-        stays set until ``status.zero_()``."""
+        stays set until ``status.zero_()`` or ``reset()``."""
         bits = int(self.status.item())
         if bits:
             raise _bad("; ".join(text for b, text in _STATUS.items() if bits & b) + f" (status {bits})")
