@@ -93,7 +93,7 @@ cudaError_t attend(const cats_kv8& c, int layer, const void* q, long long q_ld, 
   A.layer = layer;
   A.scale = scale * 1.4426950408889634f;
   A.parts = (float*)ws;
-  A.ctas = dev_info().sms < CATS_KV8_STATUS_INTS - 1 ? dev_info().sms : CATS_KV8_STATUS_INTS - 1;
+  A.ctas = dev_info().sms < kKvRefusedAt - 1 ? dev_info().sms : kKvRefusedAt - 1;   // (a counter each)
   A.counters = c.status + 1;
   A.wait_kc = wait_kcycles();
   return inst_kv8_attend<T>(c, A, st);

@@ -19,9 +19,22 @@ constexpr int kKvMaxSeqs = 1024;      // sequences of one cache: one thread each
 constexpr int kPlanThreads = 1024;
 
 // bits of the cache's status word
-enum { KV_POOL_EMPTY = 1, KV_BAD_PAGE = 2, KV_TOO_LONG = 4, KV_BAD_PARENT = 8, KV_BAD_SPAN = 16, KV_WAIT = 32 };
+enum { KV_POOL_EMPTY = 1, KV_BAD_PAGE = 2, KV_TOO_LONG = 4, KV_BAD_PARENT = 8, KV_BAD_SPAN = 16, KV_WAIT = 32, KV_REFUSED = 64 };
 
 __device__ __forceinline__ void kv_flag(const cats_kv8& c, int bit) { atomicOr(c.status, bit); }
+
+// The last words of the status array, a bit for every sequence: the last grow that had tokens for it did
+// not lengthen it, so that its last positions are older tokens', which append must not take for the new.
+constexpr int kKvRefusedAt = CATS_KV8_STATUS_INTS - kKvMaxSeqs / 32;
+__device__ __forceinline__ bool kv_refused(const cats_kv8& c, int b) { return (c.status[kKvRefusedAt + (b >> 5)] >> (b & 31)) & 1; }
+// Called by all lanes of a warp, lane = sequence: the bits of the sequences in `set` become `refused`.
+__device__ __forceinline__ void kv_set_refused(const cats_kv8& c, int b, bool set, bool refused) {
+  const unsigned which = __ballot_sync(0xffffffffu, set), bits = __ballot_sync(0xffffffffu, set && refused);
+  if ((b & 31) == 0 && which) {
+    int* w = c.status + kKvRefusedAt + (b >> 5);
+    *w = (int)(((unsigned)*w & ~which) | bits);
+  }
+}
 
 // bytes of one head's rows in a page / of a page in one layer
 __device__ __forceinline__ size_t kv_block(const cats_kv8& c) { return (size_t)c.page * c.head_dim; }

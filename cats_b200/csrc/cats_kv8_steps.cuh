@@ -179,6 +179,10 @@ __global__ void __launch_bounds__(RPT == 1 ? 32 : 256, RPT == 1 ? 16 : 2) k_kv8_
   const int len = c.lens[b], start = len - sp.count;   // rows [start, len) are new
   const int page_i = start / c.page + j;
   if (sp.count < 1 || (long long)page_i * c.page >= len) return;
+  if (kv_refused(c, b)) {                              // rows [start, len) are not the new tokens'
+    if (threadIdx.x == 0) kv_flag(c, KV_REFUSED);
+    return;
+  }
   if (start < 0 || len > max_len || sp.first < 0 || (long long)sp.first + sp.count > A.tokens) {
     if (threadIdx.x == 0) kv_flag(c, start < 0 || len > max_len ? KV_TOO_LONG : KV_BAD_SPAN);
     return;
@@ -398,6 +402,8 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv8_grow(const cats_kv8 c, con
     __syncthreads();                                   // lens are read above, written below
   }
   if (grows) c.lens[b] = len + count;
+  const bool asked = b < c.n_seqs && count > 0;
+  kv_set_refused(c, b, asked, asked && !grows);
 }
 
 // reorder, step 1: strips of the page table.  Row i of the new table is row parents[i] of the old
@@ -470,11 +476,13 @@ k_kv8_reorder_plan(const cats_kv8 c, const int* __restrict__ parents, int* n_cop
   s_first[i] = n;
   __syncthreads();
   int p = -1, len = 0;
+  bool refused = false;
   if (i < n) {
     p = parents[i];
     if (p < 0 || p >= n) p = -1;
     if (p >= 0) {
       len = c.lens[p];
+      refused = kv_refused(c, p);
       atomicMin(&s_first[p], i);
     }
   }
@@ -490,6 +498,7 @@ k_kv8_reorder_plan(const cats_kv8 c, const int* __restrict__ parents, int* n_cop
     copies[rank] = mine;
   }
   if (i < n) c.lens[i] = len;                          // (every old length was read before the barriers)
+  kv_set_refused(c, i, i < n, refused);
   if (i == 0) *n_copies = total;
   if (total == 0) return;
   __syncthreads();

@@ -34,7 +34,7 @@ PAGES, HEAD_DIMS, MAX_SEQS, STATUS_INTS = (16, 32, 64, 128), (32, 64, 96, 128), 
 _STATUS = {1: "the pool has no free page left", 2: "a page id is out of range, or a shared page would have been written",
            4: "a sequence is longer than the page table allows, or a length or position is negative",
            8: "a parent is out of range", 16: "cu does not fit the number of tokens",
-           32: "a wait inside a kernel ran out"}
+           32: "a wait inside a kernel ran out", 64: "tokens of a sequence that grow had not lengthened were left out"}
 
 
 def _bad(msg: str) -> RuntimeError:
@@ -137,7 +137,9 @@ class KVCache8:
 
     # ---- steps ------------------------------------------------------------------------------------------
     def grow(self, n_new: int = 1, cu: Optional[torch.Tensor] = None) -> None:
-        """``lens += n_new`` (or the counts of ``cu``), taking the pages that needs (``cats_kv8_grow``)."""
+        """``lens += n_new`` (or the counts of ``cu``), taking the pages that needs (``cats_kv8_grow``).  A
+        sequence that cannot have its pages keeps its length (see ``check``), and ``append`` leaves its tokens
+        out until it grows."""
         if cu is None and n_new < 1:
             raise _bad("n_new must be positive")
         self._call("cats_kv8_grow", self._cu(cu), n_new)

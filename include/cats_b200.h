@@ -406,7 +406,8 @@ int cats_export_list(const void* ws, size_t ws_bytes, int B, int H, int I, int d
  * clears them: 1 the pool has no page left, 2 a page id is out of range or a page that is shared
  * would have been written, 4 a sequence is longer than max_pages pages (or has a negative length or
  * position), 8 a parent is out of range, 16 cu does not fit the number of tokens, 32 a wait inside a
- * kernel ran out (see "wait_ms"; the results of that call are not to be used).
+ * kernel ran out (see "wait_ms"; the results of that call are not to be used), 64 tokens of a sequence
+ * that cats_kv8_grow had not lengthened were left out of a cats_kv8_append.
  * No reference counterpart (the reference leaves the cache to HF's modelling code).
  */
 enum { CATS_KV8_STATUS_INTS = 256 };
@@ -417,7 +418,8 @@ typedef struct cats_kv8 {
   int* lens;      /* [n_seqs]                                                */
   int* refs;      /* [n_pages]                                               */
   int* status;    /* [CATS_KV8_STATUS_INTS], zero at first: the status word, then scratch */
-                  /* that the calls leave zero                               */
+                  /* that the calls leave zero; the last 32: a bit for every sequence that */
+                  /* cats_kv8_grow could not lengthen                        */
   int n_layers, n_pages, n_seqs, max_pages, n_kv_heads, page, head_dim;
 } cats_kv8;
 
@@ -426,7 +428,8 @@ typedef struct cats_kv8 {
  * in the order of the sequences.  n_i = cu[i + 1] - cu[i] (device memory, [n_seqs + 1], ascending
  * from 0), or n_new for every sequence when cu is NULL.  Called once per step, before the layers'
  * cats_kv8_append.  A sequence that does not get its pages keeps its length (status bit 1 or 4); so
- * do those after it that need a page.
+ * do those after it that need a page.  Until a later cats_kv8_grow lengthens it (or reorder puts another
+ * in its place), cats_kv8_append leaves its tokens out, so that what was cached stays as it was.
  */
 int cats_kv8_grow(const cats_kv8* cache, const int* cu, int n_new, void* stream);
 
