@@ -6,6 +6,7 @@
 
 #include <stdlib.h>
 
+#include <atomic>
 #include <mutex>
 
 #include "cats_run.cuh"
@@ -38,6 +39,33 @@ const DevInfo& dev_info() {
     info[dev].sms = sms > 0 ? sms : 148;
   }
   return info[dev];
+}
+
+// The limit belongs to the kernel, not to a launch: set to what one launch needs, another thread's smaller
+// need could take it away in between.  So it is set to the most there is, always the same value, once per
+// kernel and device; the table only saves the calls after the first (full: they are made again).
+cudaError_t allow_smem(const void* kernel) {
+  static std::atomic<uint64_t> done[1024];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t key = (uint64_t)reinterpret_cast<uintptr_t>(kernel) * 64 + (uint64_t)(dev & 63) + 1;
+  const bool known = dev >= 0 && dev < 64;
+  unsigned at = (unsigned)((key * 0x9e3779b97f4a7c15ull) >> 54);
+  for (int i = 0; known && i < 1024; ++i, at = (at + 1) & 1023) {
+    const uint64_t k = done[at].load(std::memory_order_acquire);
+    if (k == key) return cudaSuccess;
+    if (k == 0) break;
+  }
+  cudaFuncAttributes a;
+  if ((e = cudaFuncGetAttributes(&a, kernel)) != cudaSuccess) return e;
+  const int most = dev_info().max_smem_optin - (int)a.sharedSizeBytes;
+  if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most)) != cudaSuccess) return e;
+  for (int i = 0; known && i < 1024; ++i, at = (at + 1) & 1023) {
+    uint64_t free_slot = 0;
+    if (done[at].compare_exchange_strong(free_slot, key, std::memory_order_release) || free_slot == key) break;
+  }
+  return cudaSuccess;
 }
 
 // the per-type launchers are instantiated in cats_inst_stage.cu / cats_inst_mega.cu

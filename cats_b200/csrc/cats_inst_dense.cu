@@ -81,8 +81,7 @@ template <typename T, bool STACK, typename... Args>
 cudaError_t launch_coop(const DensePlan& p, cudaStream_t st, Args... args) {
   // cooperative: the CTAs wait for one another at grid barriers
   auto kernel = k_dense<T, STACK>;
-  cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smemf);
+  const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel));
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));

@@ -5,26 +5,15 @@
 
 namespace cats {
 
-// Launches a kernel that needs much shared memory.  (The attribute stays with the kernel: once per
-// device; two threads at once set the same value.)
 template <typename T>
-static cudaError_t run_large(void (*kernel)(cats_kv8, KvAttnArgs<T>), bool* ready, int threads, size_t smem,
-                             const cats_kv8& c, const KvAttnArgs<T>& A, cudaStream_t st) {
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64 || !ready[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-    if (dev >= 0 && dev < 64) ready[dev] = true;
-  }
-  return launch_ready(kernel, dim3(A.ctas), dim3(threads), smem, st, c, A);
+static cudaError_t run(void (*kernel)(cats_kv8, KvAttnArgs<T>), int threads, size_t smem, const cats_kv8& c,
+                       const KvAttnArgs<T>& A, cudaStream_t st) {
+  return launch(kernel, dim3(A.ctas), dim3(threads), smem, st, c, A);
 }
 
 template <typename T, int HD, int NQ>
 static cudaError_t run_attend(const cats_kv8& c, const KvAttnArgs<T>& A, cudaStream_t st) {
-  static bool ready[64];
-  return run_large<T>(k_kv8_attend<T, HD, NQ>, ready, AttnShape<NQ>::kThreads, attn_smem<NQ>(), c, A, st);
+  return run<T>(k_kv8_attend<T, HD, NQ>, AttnShape<NQ>::kThreads, attn_smem<NQ>(), c, A, st);
 }
 
 // Up to 8 rows and up to 16 the tiles of cats_kv8_attn.cuh, bound by the codes' bytes; beyond that the
@@ -39,9 +28,7 @@ static cudaError_t run_attend(const cats_kv8& c, const KvAttnArgs<T>& A, cudaStr
   if constexpr (sizeof(T) == 2) {
     if (rows > kAttnFewRows) {
       if constexpr (HD % 64 == 0) {
-        static bool ready[64];
-        if (rows > kAttnSomeRows)
-          return run_large<T>(k_kv8_attend_tc<T, HD>, ready, kTcThreads, attn_tc_smem(HD), c, A, st);
+        if (rows > kAttnSomeRows) return run<T>(k_kv8_attend_tc<T, HD>, kTcThreads, attn_tc_smem(HD), c, A, st);
       }
       return run_attend<T, HD, 4>(c, A, st);
     }

@@ -18,15 +18,20 @@ struct DevInfo {
 };
 const DevInfo& dev_info();  // per-device properties of the current device (cats_abi.cu)
 int launch_status(cudaError_t e);  // CATS_OK, or CATS_ERR_CUDA with the error kept for cats_last_cuda_error
+// Lets the kernel have all the dynamic shared memory that the current device can give it (cats_abi.cu).
+cudaError_t allow_smem(const void* kernel);
 int wait_kcycles();         // the "wait_ms" option in units of 1024 clock cycles of the current device
 extern int g_use_pdl;       // cats_set_option("pdl", 0) launches without programmatic dependencies
 
 // Launch with the programmatic-stream-serialisation attribute: the grid may be scheduled while
 // its predecessor drains; every kernel here calls griddepcontrol.wait before touching data.
-// launch_ready: the kernel's shared-memory limit is already set.
 template <typename... KArgs, typename... Args>
-cudaError_t launch_ready(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
+cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
                    cudaStream_t stream, Args... args) {
+  if (smem > 48 * 1024) {
+    const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel));
+    if (e != cudaSuccess) return e;
+  }
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = grid;
@@ -39,17 +44,6 @@ cudaError_t launch_ready(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t
   cfg.attrs = attr;
   cfg.numAttrs = g_use_pdl ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
-}
-
-template <typename... KArgs, typename... Args>
-cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
-                   cudaStream_t stream, Args... args) {
-  if (smem > 48 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-  }
-  return launch_ready(kernel, grid, block, smem, stream, args...);
 }
 
 inline int batch_tile(int B) { return B <= 1 ? 1 : B <= 2 ? 2 : B <= 4 ? 4 : B <= 8 ? 8 : 16; }
