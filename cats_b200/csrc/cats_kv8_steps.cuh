@@ -488,14 +488,21 @@ k_kv8_reorder_plan(const cats_kv8 c, const int* __restrict__ parents, int* n_cop
   }
   __syncthreads();
   const int rows = len % c.page, at = len / c.page;
-  const bool more = p >= 0 && rows > 0 && s_first[p] != i && at < c.max_pages;
+  bool more = p >= 0 && rows > 0 && s_first[p] != i && at < c.max_pages;
+  int src = -1;
+  if (more) {
+    src = c.table[(size_t)s_first[p] * c.max_pages + at];
+    if (src < 0 || src >= c.n_pages) {                 // the parent lacks the page: so does the child
+      more = false;
+      c.table[(size_t)i * c.max_pages + at] = -1;
+      kv_flag(c, KV_BAD_PAGE);
+    }
+  }
   int total;
   const int rank = plan_scan(more ? 1 : 0, s_warp, &total);
-  KvCopy mine = {-1, -1, rows, 0};
   if (more) {
     s_order[rank] = i;
-    mine.src = c.table[(size_t)s_first[p] * c.max_pages + at];
-    copies[rank] = mine;
+    copies[rank] = {src, -1, rows, 0};
   }
   if (i < n) c.lens[i] = len;                          // (every old length was read before the barriers)
   kv_set_refused(c, i, i < n, refused);

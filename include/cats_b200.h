@@ -474,7 +474,7 @@ int cats_kv8_attend(const cats_kv8* cache, int layer, const void* q, long long q
  * (parents[i] = -1) and a beam search's reordering are all this call.  Full pages are shared; a page
  * that is still being filled goes to the first child, and every other child gets the lowest free page
  * and a copy of the filled rows in all layers.  Without a free page the child's entry is -1 (status
- * bit 1).  ws: cats_kv8_reorder_bytes(cache) bytes of scratch.
+ * bit 1), and so is that of a child whose parent lacks that page (bit 2).  ws: cats_kv8_reorder_bytes(cache) bytes of scratch.
  */
 size_t cats_kv8_reorder_bytes(const cats_kv8* cache);
 int cats_kv8_reorder(const cats_kv8* cache, const int* parents, void* ws, size_t ws_bytes, void* stream);

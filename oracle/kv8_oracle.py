@@ -170,7 +170,7 @@ class Cache:
             if part and eldest[p] != i:
                 copies.append((i, full, table[p, full], part))
         for i, full, src, part in copies:
-            dst = self._free()
+            dst = self._free() if src >= 0 else -1          # (a page that the parent lacks, the child lacks too)
             self.table[i, full] = dst
             if dst >= 0:
                 self.refs[dst] = 1

@@ -129,3 +129,29 @@ def test_reset_forgets_what_was_recorded(cuda_device):
     c.reset()
     c.check()
     assert c.lens.tolist() == [0, 0] and int(c.refs.sum()) == 0 and int((c.table >= 0).sum()) == 0
+
+
+# ---- a parent whose last page is missing
+def test_a_missing_page_is_not_handed_on_as_another(cuda_device):
+    """Sequence 1 lacks its last page (an earlier reorder found none free).  Who continues it lacks the
+    page too; it gets no page with somebody else's rows."""
+    c = filled(cuda_device, [20, 37, 5, 16], 16, 1, 32, layers=2, spare=4)
+    lost = int(c.table[1, 2])
+    c.table[1, 2] = -1
+    c.refs[lost] = 0
+    o = K.Cache.of(c)
+    o.reorder([1, 0, 1, 1])
+    c.reorder(torch.tensor([1, 0, 1, 1], dtype=torch.int32, device=cuda_device))
+    same_state(c, o, layers=False)
+    assert c.lens.tolist() == [37, 20, 37, 37]
+    assert c.table[:, 2].tolist() == [-1, -1, -1, -1]
+    assert torch.equal(c.table[[0, 2, 3], :2], c.table[:1, :2].expand(3, 2)) and c.table[0, :2].min() >= 0
+    held = torch.zeros_like(c.refs)
+    t = c.table[c.table >= 0].long()
+    held.index_add_(0, t, torch.ones_like(t, dtype=torch.int32))
+    assert torch.equal(held, c.refs)
+    k, v = c.read(0, 1)
+    ko, vo = o.rows(0, 1, 20)
+    assert np.array_equal(np64(k), ko) and np.array_equal(np64(v), vo)
+    with pytest.raises(RuntimeError, match="page id"):
+        c.check()
