@@ -275,12 +275,17 @@ class KVCache8:
             raise _bad("; ".join(text for b, text in _STATUS.items() if bits & b) + f" (status {bits})")
 
     def read(self, layer: int, seq: int) -> Tuple[torch.Tensor, torch.Tensor]:
-        """(keys, values) of one sequence, fp32 [kv_heads, len, head_dim] (synchronises)."""
+        """(keys, values) of one sequence, fp32 [kv_heads, len, head_dim] (synchronises).  Raises if not
+        all of its pages are there."""
         self._layer(layer)
         if not 0 <= seq < self.n_seqs:
             raise _bad(f"sequence {seq} is out of range (0 .. {self.n_seqs - 1})")
         n = int(self.lens[seq])
+        if not 0 <= n <= self.max_len:
+            raise _bad(f"sequence {seq} is {n} tokens long, the table holds up to {self.max_len}")
         ids = self.table[seq, :(n + self.page - 1) // self.page].long()
+        if ids.numel() and not (0 <= int(ids.min()) and int(ids.max()) < self.n_pages):
+            raise _bad(f"sequence {seq} lacks a page, or a page id is out of range")
         kv = self.codes.view(torch.float8_e4m3fn)[layer].view(torch.uint8)[ids].view(torch.float8_e4m3fn).float()
         kv = (kv * self.scales[layer][ids][..., None, None]).permute(1, 2, 0, 3, 4)
         kv = kv.reshape(2, self.n_kv_heads, ids.numel() * self.page, self.head_dim)[:, :, :n]
