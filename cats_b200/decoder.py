@@ -293,33 +293,38 @@ class CatsDecoder:
         self._capture(sorted({self._bucket(p) for p in range(first_pos, last_pos + 1)}), first_pos, self._step)
 
     def _capture(self, keys, first_pos: int, step) -> None:
-        """``step(key)`` into ``self.graphs[key]``, for every key that is not there yet."""
+        """``step(key)`` into ``self.graphs[key]``, for every key that is not there yet.  State and cache are
+        what they were afterwards, also if a step raises."""
         state = [self.tok, self.pos, self.h, self.x]
         keep = [t.clone() for t in state]
         kv = self.kv
         side = torch.cuda.Stream(self.dev)
         side.wait_stream(torch.cuda.current_stream(self.dev))
-        with torch.cuda.stream(side):
-            self.pos.fill_(min(first_pos, self.max_len - 3))
-            if kv is not None:
-                # the warm-up's tokens go into a cache of their own: rows that leave a page again may
-                # have raised its scale
-                self.kv = kv8.KVCache8(self.L, self.B, self.B, kv.page, self.nkv, self.hd, kv.page, self.dev)
-            for _ in range(2):
-                step(keys[0])
+        try:
+            with torch.cuda.stream(side):
+                self.pos.fill_(min(first_pos, self.max_len - 3))
+                if kv is not None:
+                    # the warm-up's tokens go into a cache of their own: rows that leave a page again may
+                    # have raised its scale
+                    self.kv = kv8.KVCache8(self.L, self.B, self.B, kv.page, self.nkv, self.hd, kv.page, self.dev)
+                for _ in range(2):
+                    step(keys[0])
             self.kv = kv
-        torch.cuda.current_stream(self.dev).wait_stream(side)
-        torch.cuda.synchronize(self.dev)
-        for k in keys:
-            if k in self.graphs:
-                continue
-            g = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(g):
-                step(k)
-            self.graphs[k] = g
-        for t, v in zip(state, keep):
-            t.copy_(v)
-        torch.cuda.synchronize(self.dev)
+            torch.cuda.current_stream(self.dev).wait_stream(side)
+            torch.cuda.synchronize(self.dev)
+            for k in keys:
+                if k in self.graphs:
+                    continue
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g):
+                    step(k)
+                self.graphs[k] = g
+        finally:
+            self.kv = kv
+            torch.cuda.current_stream(self.dev).wait_stream(side)
+            for t, v in zip(state, keep):
+                t.copy_(v)
+            torch.cuda.synchronize(self.dev)
 
     @torch.no_grad()
     def decode(self, n_tokens: int, use_graph: bool = True, keep_logits: bool = False):

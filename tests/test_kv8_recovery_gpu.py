@@ -155,3 +155,27 @@ def test_a_missing_page_is_not_handed_on_as_another(cuda_device):
     assert np.array_equal(np64(k), ko) and np.array_equal(np64(v), vo)
     with pytest.raises(RuntimeError, match="page id"):
         c.check()
+
+
+# ---- a capture that fails
+def test_a_step_that_fails_while_it_is_captured_leaves_the_cache(cuda_device):
+    """The warm-up of a capture runs over a cache of its own; the decoder's comes back even if a step raises."""
+    from cats_b200 import decoder as D
+    from test_decoder_paged8_gpu import SMALL, small_model
+
+    dec = D.CatsDecoder(small_model(cuda_device), 2, 200, mlp="dense", cache="paged8", page=16)
+    ids = torch.randint(0, SMALL["vocab_size"], (2, 30), device=cuda_device)
+    kv = dec.kv
+    dec.prefill(ids)
+    tok, pos = dec.tok.clone(), dec.pos.clone()
+
+    def step(_):
+        dec.pos.add_(1)
+        raise MemoryError("nothing left")
+
+    with pytest.raises(MemoryError):
+        dec._capture([dec.max_len], 30, step)
+    assert dec.kv is kv and not dec.graphs
+    assert torch.equal(dec.tok, tok) and torch.equal(dec.pos, pos)
+    dec.decode(3)
+    assert kv.lens.tolist() == [33, 33]
