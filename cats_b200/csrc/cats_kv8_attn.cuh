@@ -15,8 +15,10 @@
 // softmax weights are rounded to half precision, 2^-11, below the rounding of a 16-bit result.
 // fp32 queries and weights are each split in two halves (22 bits) and take two products.
 // The scale of V's page is a power of two and joins the exponent: weights are
-// p' = exp2(s + ev - m) with m the running maximum of s + ev, so that p' <= 1 whatever the scales,
-// and the softmax's sum is that of p' 2^-ev.
+// p' = exp2(s - m + ev - ec) with m the running maximum of s, ev the page's exponent and ec the one that the
+// accumulators are held at; the softmax's sum is that of p' 2^(ec - ev).  ec follows ev when they are more than
+// kAttnSpan apart (the accumulators are rescaled, exactly), so that what half precision loses of a weight does not
+// depend on the scales of other pages: 2^-11 of it, or 2^-21 of the largest weight of the row for a small one.
 //
 // Work: a unit is 16 positions for each warp of one tile (8, 16 or 32 rows) of one key head.  All units
 // of the call in a row - sequences, heads, tiles, positions - are dealt out to one CTA per SM in
@@ -36,6 +38,12 @@ namespace cats {
 constexpr int kAttnTile = 16;                           // positions of a warp's tile
 constexpr int kAttnStageBytes = 2 * kAttnTile * 128;    // keys, values (rows 128 bytes apart)
 constexpr float kAttnSlack = 8.f;                       // see the running maximum
+// How far a page's exponent may be from the accumulators'.  (These go down by up to 84, the range of scales; a sum of
+// 2^21 products of weights up to 2^12 and codes up to 2^9 is still a number of fp32 then.)
+constexpr int kAttnSpan = 4;
+constexpr int kAttnNoExp = -1000;                       // nothing in the accumulators yet
+// (a scale outside the cache's range counts as the nearest inside)
+__device__ __forceinline__ int attn_exp_of(float scale) { return min(max(kv_exp_of(scale), kKvExpMin), kKvExpMax); }
 
 // NQ columns of eight rows ((token, query head of the group) pairs) per tile.  Eight rows leave room
 // for 16 warps of 128 registers, which hide the latency of the chain load - convert - multiply -
@@ -632,6 +640,7 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
   float o[MT][NQ][4];
   float m[NQ][2], l[NQ][2], f[NQ][2];
   int lim[NQ][2], lim_min = 0;                           // positions that a row sees, and the least of them
+  int ec = kAttnNoExp;                                   // exponent that o is held at
   AttnSeq seq;
   AttnPlace at = attn_place<NQ>(s_tab, c.n_seqs, group, share0, &seq);
   bool first_seg = true, begins_here = at.unit == 0, fresh = true;
@@ -639,6 +648,7 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
   for (int u = 0; u < n_units; ++u) {
     if (fresh) {                                         // a new (sequence, head, tile): its queries
       fresh = false;
+      ec = kAttnNoExp;
       const int rows = min(S::kRows, seq.count * group - at.tile * S::kRows);
       lim_min = min(seq.len, seq.len - seq.count + at.tile * S::kRows / group + 1);
 #pragma unroll
@@ -743,8 +753,19 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
           }
         }
       }
-      const int ev = kv_exp_of(sc.y);
-      const float evf = (float)ev, vi = kv_pow2(-ev);
+      int ev = kv_exp_of(sc.y);
+      if ((unsigned)(ev - ec + kAttnSpan) > 2u * kAttnSpan) {          // (the same for all lanes)
+        ev = attn_exp_of(sc.y);
+        const float by = kv_pow2(max(ec - ev, -126));    // (the first time o is zero)
+        ec = ev;
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[i][n][x] *= by;
+      }
+      const float evf = (float)(ev - ec), vi = kv_pow2(ec - ev);
       const bool cut = kb + kAttnTile > lim_min;         // some row does not see all of the tile
       uint32_t p[NQ][2], pl[NQ][2];
       float top[NQ][2];
@@ -768,16 +789,13 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
 #pragma unroll
           for (int x = 0; x < 2; ++x) top[n][x] = fmaxf(top[n][x], __shfl_xor_sync(0xffffffffu, top[n][x], w));
       // The reference m of the weights follows the running maximum only when that is more than
-      // 2^kAttnSlack ahead: weights up to 256 do half precision no harm, and the accumulators are
-      // rescaled a few times per sequence instead of at every second tile.
+      // 2^kAttnSlack ahead: weights up to 2^(kAttnSlack + kAttnSpan) do half precision no harm, and the
+      // accumulators are rescaled a few times per sequence instead of at every second tile.
       bool ahead = false;
 #pragma unroll
       for (int n = 0; n < NQ; ++n)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          top[n][x] += evf;
-          ahead |= top[n][x] > m[n][x] + kAttnSlack;
-        }
+        for (int x = 0; x < 2; ++x) ahead |= top[n][x] > m[n][x] + kAttnSlack;
       if (__any_sync(0xffffffffu, ahead)) {
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
@@ -797,7 +815,7 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
       for (int n = 0; n < NQ; ++n) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          // (m - ev) is the same for all tiles whose pages have the same ev: its rounding cancels
+          // (the same for all tiles whose pages have the same ev, while m and ec stay: its rounding cancels)
           const float ref = m[n][x] == -INFINITY ? 0.f : m[n][x] - evf;
           s[n][x] = ex2(s[n][x] - ref);
           s[n][2 + x] = ex2(s[n][2 + x] - ref);
@@ -849,6 +867,7 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
       // eight rows at a time, in the codes' bytes of the stage that this tile was in (free until the
       // next call of issue): [8][HD] floats of each warp
       const size_t pitch = (size_t)S::kStages * kAttnStageBytes;
+      const float held = kv_pow2(max(ec, -126));         // (no tile seen: o is zero)
       __syncwarp();
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
@@ -867,7 +886,8 @@ __global__ void __launch_bounds__(AttnShape<NQ>::kThreads, 1) k_kv8_attend(const
 #pragma unroll
             for (int i = 0; i < MT; i += 2) {
               const int d = i < 4 * (HD / 64) ? 64 * (i / 4) + 8 * g + 2 * (i % 4) : HD / 64 * 64 + 4 * g;
-              *reinterpret_cast<float4*>(dst + d) = make_float4(o[i][n][x], o[i][n][2 + x], o[i + 1][n][x], o[i + 1][n][2 + x]);
+              *reinterpret_cast<float4*>(dst + d) = make_float4(o[i][n][x] * held, o[i][n][2 + x] * held, o[i + 1][n][x] * held,
+                                                                o[i + 1][n][2 + x] * held);
             }
           }
         }

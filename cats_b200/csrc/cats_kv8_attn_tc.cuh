@@ -86,7 +86,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_kv8_attend_tc(const cats_kv8 
   __shared__ uint64_t s_bar;
   __shared__ uint32_t s_tmem;
   __shared__ int s_id[2][8];                             // page of 16 positions each of this and the next step,
-  __shared__ float s_ks[2][8], s_ev[2][8];               // scale of its keys, exponent of its values' scale
+  __shared__ __align__(8) float s_ks[2][8];              // scale of its keys,
+  __shared__ __align__(8) int s_ev[2][8];                // exponent of its values' scale (kAttnNoExp: no page)
+  __shared__ int2 s_span[2];                             // and a step's largest and least of them
   __shared__ float s_x[4][kTcRows];                      // what the four threads of a row tell one another
   __shared__ int s_nan[HD];
   pdl_wait();
@@ -142,12 +144,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_kv8_attend_tc(const cats_kv8 
     const int* table = c.table + (size_t)at.b * c.max_pages;
 
     // pages of a step: looked up by the first eight threads, one step before its codes are asked for
-    int n_id = -1;
-    float n_ks = 0.f, n_ev = 0.f;
+    int n_id = -1, n_ev = kAttnNoExp;
+    float n_ks = 0.f;
     auto look = [&](int unit) {
       n_id = -1;
       n_ks = 0.f;
-      n_ev = 0.f;
+      n_ev = kAttnNoExp;
       const int p = unit * kTcKeys + 16 * tid;
       if (tid < 8 && unit < u_end && p < end) {
         const int id = table[p >> page_log];
@@ -156,7 +158,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_kv8_attend_tc(const cats_kv8 
         } else {
           n_id = id;
           n_ks = layer_scales[(size_t)id * 2 * c.n_kv_heads + at.head];
-          n_ev = (float)kv_exp_of(layer_scales[((size_t)id * 2 + 1) * c.n_kv_heads + at.head]);
+          n_ev = attn_exp_of(layer_scales[((size_t)id * 2 + 1) * c.n_kv_heads + at.head]);
         }
       }
     };
@@ -165,6 +167,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_kv8_attend_tc(const cats_kv8 
         s_id[unit & 1][tid] = n_id;
         s_ks[unit & 1][tid] = n_ks;
         s_ev[unit & 1][tid] = n_ev;
+        const int high = __reduce_max_sync(0xffu, n_ev), low = __reduce_min_sync(0xffu, n_id >= 0 ? n_ev : -kAttnNoExp);
+        s_span[unit & 1] = make_int2(high, low);         // (the same from all eight)
       }
     };
     // a step's codes: 16 bytes of rows tid / kChunks + i * (512 / kChunks)
@@ -231,6 +235,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_kv8_attend_tc(const cats_kv8 
     settle();
     __syncthreads();
     float m = -INFINITY, l = 0.f;
+    int ec = kAttnNoExp;                                 // exponent that O is held at
 
     for (int unit = u_first; unit < u_end; ++unit) {
       const int kb = unit * kTcKeys;
@@ -303,82 +308,128 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_kv8_attend_tc(const cats_kv8 
       // ---- 2 the next step's codes (and the page numbers of the one after it)
       look(unit + 2);
       if (unit + 1 < u_end) fetch(unit + 1);
+      int high = s_span[unit & 1].x;
+      const int low = s_span[unit & 1].y;
+      const float2 ks = *reinterpret_cast<const float2*>(&s_ks[unit & 1][2 * quarter]);
+      const int2 evs = *reinterpret_cast<const int2*>(&s_ev[unit & 1][2 * quarter]);
       wait_mma();
       // ---- 4 a quarter of a row each: weights
-      float s[32];
-      tmem_ld32(t_s + t_lane + 32 * quarter, s);
-      float top = -INFINITY;
       const int k0 = kb + 32 * quarter;
-      float ev[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int z = 2 * quarter + j;
-        const float by = s_ks[unit & 1][z] * f;
-        ev[j] = s_ev[unit & 1][z];
-        float t = -INFINITY;
+      float s[32];
+      // scores of sixteen positions (the same page for all), -inf where the row does not see them
+      auto score = [&](int j) {
+        const float by = (j ? ks.y : ks.x) * f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[16 * j + i] *= by;
-        if (k0 + 16 * j + 16 > lim || s_id[unit & 1][z] < 0) {
-          const int sees = s_id[unit & 1][z] < 0 ? 0 : lim - k0 - 16 * j;      // of the sixteen
+        const bool none = (j ? evs.y : evs.x) == kAttnNoExp;
+        if (k0 + 16 * j + 16 > lim || none) {
+          const int sees = none ? 0 : lim - k0 - 16 * j;                       // of the sixteen
 #pragma unroll
           for (int i = 0; i < 16; ++i)
             if (i >= sees) s[16 * j + i] = -INFINITY;
         }
+      };
+      auto rescale = [&](float by) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) t = fmaxf(t, s[16 * j + i]);
-        top = fmaxf(top, t + ev[j]);
+        for (int d = 0; d < HD / 4; d += 16) {
+          float o[16];
+          tmem_ld16(t_o + t_lane + quarter * (HD / 4) + d, o);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] *= by;
+          tmem_st16(t_o + t_lane + quarter * (HD / 4) + d, o);
+        }
+      };
+      // The exponent of O for the positions whose exponents are `high` and less, and the least that can go with
+      // them: sixteen positions are a k-step of the product, those within kAttnSpan of O's exponent take part, the
+      // others' weights are 0.  In earnest all of them take part.
+      int least = kAttnNoExp + 1;
+      auto follow = [&](int high) {
+        float by = 1.f;
+        least = kAttnNoExp + 1;
+        if (high > ec + kAttnSpan || low < ec - kAttnSpan) {
+          const int to = low < high - kAttnSpan ? high - kAttnSpan : high;
+          least = to - kAttnSpan;
+          by = kv_pow2(max(ec - to, -126));
+          ec = to;
+        }
+        return by;
+      };
+      auto weigh = [&](int j, int high) {
+        const int ev = j ? evs.y : evs.x;
+        const uint32_t to = p_u + (quarter >> 1) * kTcBlock;
+        const uint32_t p0 = to + tc_at(row, 4 * (quarter & 1) + 2 * j), p1 = to + tc_at(row, 4 * (quarter & 1) + 2 * j + 1);
+        if (ev < least || ev > high) {                   // (the same for all lanes of a warp)
+          sts16(p0, 0, 0, 0, 0);
+          sts16(p1, 0, 0, 0, 0);
+          return;
+        }
+        const float ref = m == -INFINITY ? 0.f : m - (float)(ev - ec);
+        float part = 0.f;
+        float* x = s + 16 * j;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          x[i] = ex2(x[i] - ref);
+          part += x[i];
+        }
+        l = fmaf(part, kv_pow2(ec - ev), l);
+        sts16(p0, half2_bits(x[0], x[1]), half2_bits(x[2], x[3]), half2_bits(x[4], x[5]), half2_bits(x[6], x[7]));
+        sts16(p1, half2_bits(x[8], x[9]), half2_bits(x[10], x[11]), half2_bits(x[12], x[13]), half2_bits(x[14], x[15]));
+      };
+      // ---- 5 O += P V
+      auto multiply = [&](bool add) {
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncthreads();
+        if (tid == 0) {
+          tc_fence_after();
+          const uint32_t vb = v_u + (unit & 1) * (2 * HD * 128);
+#pragma unroll
+          for (int k = 0; k < kTcKeys / 16; ++k)
+            umma_f16(t_o, umma_desc_k128(p_u + (k / 4) * kTcBlock) + 2 * (k % 4), umma_desc_k128(vb + (k / 4) * (HD * 128)) + 2 * (k % 4),
+                     tc_idesc(HD), add || k > 0);
+        }
+      };
+      tmem_ld32(t_s + t_lane + 32 * quarter, s);
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        score(j);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[16 * j + i]);
       }
       s_x[quarter][row] = top;
       asm volatile("bar.sync %0, 128;" ::"r"(1 + (warp & 3)) : "memory");    // the four warps of these rows
       top = fmaxf(fmaxf(s_x[0][row], s_x[1][row]), fmaxf(s_x[2][row], s_x[3][row]));
-      if (__any_sync(0xffffffffu, top > m + kAttnSlack)) {
-        const float to = fmaxf(top, m), by = m == -INFINITY ? 0.f : ex2(m - to);
+      const float by = follow(high);
+      if (__any_sync(0xffffffffu, top > m + kAttnSlack || by != 1.f)) {
+        const float to = fmaxf(top, m), down = m == -INFINITY ? 0.f : ex2(m - to);
         m = to;
-        l *= by;
-        if (unit > u_first) {
-#pragma unroll
-          for (int d = 0; d < HD / 4; d += 16) {
-            float o[16];
-            tmem_ld16(t_o + t_lane + quarter * (HD / 4) + d, o);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] *= by;
-            tmem_st16(t_o + t_lane + quarter * (HD / 4) + d, o);
-          }
-        }
+        l *= down;
+        if (unit > u_first) rescale(by * down);
       }
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float ref = m == -INFINITY ? 0.f : m - ev[j];
-        float part = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float& x = s[16 * j + i];
-          x = ex2(x - ref);
-          part += x;
-        }
-        l = fmaf(part, kv_pow2(-(int)ev[j]), l);
-#pragma unroll
-        for (int i = 0; i < 16; i += 8) {
-          const float* x = s + 16 * j + i;
-          sts16(p_u + (quarter >> 1) * kTcBlock + tc_at(row, 4 * (quarter & 1) + 2 * j + i / 8), half2_bits(x[0], x[1]),
-                half2_bits(x[2], x[3]), half2_bits(x[4], x[5]), half2_bits(x[6], x[7]));
-        }
-      }
+      for (int j = 0; j < 2; ++j) weigh(j, high);
       settle();
-      fence_proxy_async_smem();
-      tc_fence_before();
-      __syncthreads();
-      keep(unit + 2);                                    // (this step's are read; the next barrier is before their use)
-      // ---- 5 O += P V
-      if (tid == 0) {
-        tc_fence_after();
-        const uint32_t vb = v_u + (unit & 1) * (2 * HD * 128);
+      multiply(unit > u_first);
+      // pages of this step whose exponents lie far below the others': one class of them after the other
+      while (least > low) {
+        int next = kAttnNoExp;
+        for (int z = 0; z < 8; ++z)
+          if (s_ev[unit & 1][z] < least) next = max(next, s_ev[unit & 1][z]);
+        high = next;
+        if (tid == 0) umma_commit(bar);
+        wait_mma();                                      // before P and O change
+        rescale(follow(high));
+        tmem_ld32(t_s + t_lane + 32 * quarter, s);
 #pragma unroll
-        for (int k = 0; k < kTcKeys / 16; ++k)
-          umma_f16(t_o, umma_desc_k128(p_u + (k / 4) * kTcBlock) + 2 * (k % 4), umma_desc_k128(vb + (k / 4) * (HD * 128)) + 2 * (k % 4),
-                   tc_idesc(HD), unit > u_first || k > 0);
-        if (unit + 1 == u_end) umma_commit(bar);
+        for (int j = 0; j < 2; ++j) {
+          score(j);
+          weigh(j, high);
+        }
+        multiply(true);
       }
+      if (tid == 0 && unit + 1 == u_end) umma_commit(bar);
+      keep(unit + 2);                                    // (this step's are read; the next barrier is before their use)
     }
     wait_mma();
 
@@ -388,6 +439,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_kv8_attend_tc(const cats_kv8 
     __syncthreads();
     l = (s_x[0][row] + s_x[1][row]) + (s_x[2][row] + s_x[3][row]);
     const bool whole = u_first == 0 && u_end == seq.units;
+    const float held = kv_pow2(max(ec, -126));           // (no page seen: O is zero)
     float* part = A.parts + (size_t)(blockIdx.x * 2 + (first_seg ? 0 : 1)) * attn_part_floats(kTcRows, HD);
 #pragma unroll
     for (int d0 = 0; d0 < HD / 4; d0 += 16) {
@@ -397,7 +449,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_kv8_attend_tc(const cats_kv8 
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
           const int d = quarter * (HD / 4) + d0 + i;
-          float4 v = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          float4 v = make_float4(o[i] * held, o[i + 1] * held, o[i + 2] * held, o[i + 3] * held);
           const float bad = __uint_as_float(0x7fc00000u);
           if (s_nan[d] < lim) v.x = bad;
           if (s_nan[d + 1] < lim) v.y = bad;

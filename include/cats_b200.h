@@ -456,7 +456,10 @@ int cats_kv8_append(const cats_kv8* cache, int layer, const void* qkv, long long
  * Causal attention of the newest tokens over the cache: for each of n_tokens (order and cu as for
  * cats_kv8_append; q rows q_ld elements apart, [n_heads, head_dim] each) and each head h
  *   out = sum_p softmax_p(scale * q . k_p) v_p   over the positions p of the token's sequence up to
- * its own; key head h / (n_heads / n_kv_heads).  Scores, softmax and sums in fp32.  A token without
+ * its own; key head h / (n_heads / n_kv_heads).  Scores, softmax and sums in fp32; the products take
+ * queries and softmax weights in half precision (queries scaled by a power of two per row, weights off by
+ * 2^-11 of themselves or 2^-21 of the row's largest, whatever the scales of the pages), for fp32 queries in
+ * two halves each (22 bits).  A token without
  * any position (an empty sequence) gives zeros; pages listed as -1 are left out (status bit 2).
  * Positions behind the token never reach its result, whatever they hold; rows behind the last
  * sequence's are left as they are in out.
