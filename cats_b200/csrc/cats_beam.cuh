@@ -124,7 +124,17 @@ __global__ void __launch_bounds__(kBeamThreads, 4) k_beam_rows(const BeamArgs A)
   };
   fetch(v0);
   float m = -CUDART_INF_F, ref = 0.f, sum = 0.f, tau = -CUDART_INF_F;
-  double whole_sum = 0;                                // of the tiles before the last few (kBeamFold)
+  float whole_m = -CUDART_INF_F;                       // of the tiles before the last few (kBeamFold): their maximum
+  double whole_sum = 0;                                // and their sum relative to it
+  // Sum relative to m instead of 2^ref: both products are with the same constant, so what is left of
+  // its error is a factor of (x - m)
+  auto fold = [&]() {
+    if (m > -CUDART_INF_F && fabsf(ref) <= kFar) sum *= beam_exp2(-fmaf(m, kLog2e, -ref));
+    if (whole_m < m) whole_sum *= beam_exp2((whole_m - m) * kLog2e);   // (nothing yet: 0 times 0, or a NaN that stays)
+    whole_m = m;
+    whole_sum += sum;
+    sum = 0.f;
+  };
   for (int base = v0; base < v1; base += kBeamThreads * NV) {
     float f[NV][N];
 #pragma unroll
@@ -149,9 +159,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4) k_beam_rows(const BeamArgs A)
         const bool was = fabsf(ref) <= kFar, is = fabsf(to) <= kFar;
         float by = was && is ? ref - to : (m - top) * kLog2e;
         if (was != is) by += was ? -fmaf(m, kLog2e, -ref) : fmaf(top, kLog2e, -to);   // relative to 2^ref on one side only
-        by = beam_exp2(by);
-        sum *= by;
-        whole_sum *= by;
+        sum *= beam_exp2(by);
       }
       m = top;
       ref = to;
@@ -220,10 +228,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4) k_beam_rows(const BeamArgs A)
       }
     }
     const int tiles = (base - v0) / (kBeamThreads * NV) + 1;
-    if (tiles % kBeamFold == 0) {
-      whole_sum += sum;
-      sum = 0.f;
-    }
+    if (tiles % kBeamFold == 0) fold();
     // after 2, 4, 8 ... tiles: the k-th largest so far is the threshold of the next
     if (tiles > 1 && (tiles & (tiles - 1)) == 0 && base + kBeamThreads * NV < v1) {
       __syncthreads();
@@ -239,10 +244,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4) k_beam_rows(const BeamArgs A)
       tau = t == 0 ? -CUDART_INF_F : beam_value((uint32_t)(t >> 32));
     }
   }
-  // Sum relative to m instead of 2^ref: both products are with the same constant, so what is left of
-  // its error is a factor of (x - m)
-  whole_sum += sum;
-  if (m > -CUDART_INF_F && fabsf(ref) <= kFar) whole_sum *= beam_exp2(-fmaf(m, kLog2e, -ref));
+  fold();
   // maximum and sum of the part
   float top = m;
 #pragma unroll

@@ -177,9 +177,10 @@ __global__ void __launch_bounds__(RPT == 1 ? 32 : 256, RPT == 1 ? 16 : 2) k_kv8_
   }
   const KvSpan sp = kv_span(A.cu, A.uniform, b);
   const int len = c.lens[b], start = len - sp.count;   // rows [start, len) are new
+  const bool refused = kv_refused(c, b);
   const int page_i = start / c.page + j;
   if (sp.count < 1 || (long long)page_i * c.page >= len) return;
-  if (kv_refused(c, b)) {                              // rows [start, len) are not the new tokens'
+  if (refused) {                                       // rows [start, len) are not the new tokens'
     if (threadIdx.x == 0) kv_flag(c, KV_REFUSED);
     return;
   }
