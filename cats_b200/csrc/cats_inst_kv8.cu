@@ -22,7 +22,7 @@ int check_cache(const cats_kv8* c) {
     return CATS_ERR_RANGE;
   if (c->page != 16 && c->page != 32 && c->page != 64 && c->page != 128) return CATS_ERR_RANGE;
   if (c->head_dim != 32 && c->head_dim != 64 && c->head_dim != 96 && c->head_dim != 128) return CATS_ERR_RANGE;
-  if ((long long)c->max_pages * c->page > 0x7fffffffLL) return CATS_ERR_RANGE;
+  if ((long long)c->max_pages * c->page > 0x7fffffffLL || (long long)c->max_pages * c->n_seqs > 0x7fffffffLL) return CATS_ERR_RANGE;
   return CATS_OK;
 }
 

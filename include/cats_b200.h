@@ -400,7 +400,8 @@ int cats_export_list(const void* ws, size_t ws_bytes, int B, int H, int I, int d
  * still being filled belongs to one; cats_kv8_reorder keeps that so.
  * All arrays live in device memory, the struct itself in host memory.  A zero-initialised pool with
  * table -1 is an empty cache.  Calls on one cache have to be ordered (one stream, or events).
- *   page 16, 32, 64 or 128; head_dim 32, 64, 96 or 128; n_seqs <= 1024; codes 16-byte aligned.
+ *   page 16, 32, 64 or 128; head_dim 32, 64, 96 or 128; n_seqs <= 1024; codes 16-byte aligned;
+ *   max_pages * page and max_pages * n_seqs below 2^31.
  * Ids and lengths are device data and are checked on the device: what does not fit is left out
  * (never read or written out of range) and recorded in *status, bits that stay until the caller
  * clears them: 1 the pool has no page left, 2 a page id is out of range or a page that is shared
