@@ -95,12 +95,14 @@ struct KvSpan {
 __device__ __forceinline__ KvSpan kv_span(const int* cu, int uniform, int b) {
   if (!cu) return {b * uniform, uniform};
   const int a = __ldg(cu + b), z = __ldg(cu + b + 1);
-  return {a, z > a ? z - a : 0};
+  return {a, z > a ? (int)min((unsigned)z - (unsigned)a, 0x7fffffffu) : 0};
 }
+// cu goes down behind sequence b: the spans could overlap, and be more than the call's tokens together
+__device__ __forceinline__ bool kv_descends(const int* cu, int b) { return __ldg(cu + b + 1) < __ldg(cu + b); }
 
 // pages that `count` new tokens can touch
 __host__ __device__ inline int kv_units(int count, int page) {
-  return count < 1 ? 0 : (count + page - 2) / page + 1;
+  return count < 1 ? 0 : (int)(((unsigned)count + page - 2u) / page) + 1;
 }
 
 // eight elements, 16-byte aligned: read once (streaming) or shared by several warps (cached)

@@ -177,11 +177,12 @@ __device__ __forceinline__ bool attn_by_segments(int largest, int dealt, int tot
 }
 
 // Sequence b into the table; its units and segments.  A sequence whose length or span does not fit
-// counts as one that holds nothing.
+// counts as one that holds nothing; with `drop` (spans that are not in order) none has any tokens.
 template <int NQ, typename T>
-__device__ __forceinline__ AttnSeq attn_enter(const cats_kv8& c, const KvAttnArgs<T>& A, AttnTable& tab, int b, int group) {
+__device__ __forceinline__ AttnSeq attn_enter(const cats_kv8& c, const KvAttnArgs<T>& A, AttnTable& tab, int b, int group,
+                                              bool drop) {
   const KvSpan sp = kv_span(A.cu, A.uniform, b);
-  int len = c.lens[b], first = sp.first, count = sp.count;
+  int len = c.lens[b], first = sp.first, count = drop ? 0 : sp.count;
   const bool long_ok = len >= 0 && len <= c.max_pages * c.page;
   const bool span_ok = first >= 0 && (long long)first + count <= A.tokens;
   if (count > 0 && !(long_ok && span_ok)) {
@@ -203,7 +204,9 @@ template <int NQ, typename T>
 __device__ __forceinline__ AttnPlan attn_plan_warp(const cats_kv8& c, const KvAttnArgs<T>& A, AttnTable& tab, int group) {
   const int lane = threadIdx.x & 31;
   AttnSeq s = {0, 0, 0, 0, 0};
-  if (lane < c.n_seqs) s = attn_enter<NQ>(c, A, tab, lane, group);
+  const bool drop = __any_sync(0xffffffffu, A.cu && lane < c.n_seqs && kv_descends(A.cu, lane));
+  if (drop && blockIdx.x == 0 && lane == 0) kv_flag(c, KV_BAD_SPAN);
+  if (lane < c.n_seqs) s = attn_enter<NQ>(c, A, tab, lane, group, drop);
   auto scan = [&](int v) {
     int incl = v;
 #pragma unroll
@@ -270,12 +273,22 @@ __device__ __forceinline__ AttnPlan attn_plan_block(const cats_kv8& c, const KvA
                                                     int* s_warp) {
   constexpr int kThreads = AttnShape<NQ>::kThreads, kPer = kKvMaxSeqs / kThreads;
   int mine[kPer], segments = 0;
+  bool drop = false;
+  if (A.cu) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int b = threadIdx.x * kPer + i;
+      drop = drop || (b < c.n_seqs && kv_descends(A.cu, b));
+    }
+    drop = __syncthreads_or(drop);
+    if (drop && blockIdx.x == 0 && threadIdx.x == 0) kv_flag(c, KV_BAD_SPAN);
+  }
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int b = threadIdx.x * kPer + i;
     mine[i] = 0;
     if (b < c.n_seqs) {
-      const AttnSeq s = attn_enter<NQ>(c, A, tab, b, group);
+      const AttnSeq s = attn_enter<NQ>(c, A, tab, b, group, drop);
       mine[i] = s.units * s.tiles * c.n_kv_heads;
       if (s.units) segments += s.tiles * c.n_kv_heads;
     }

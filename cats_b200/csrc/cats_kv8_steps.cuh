@@ -178,8 +178,8 @@ __global__ void __launch_bounds__(RPT == 1 ? 32 : 256, RPT == 1 ? 16 : 2) k_kv8_
   const KvSpan sp = kv_span(A.cu, A.uniform, b);
   const int len = c.lens[b], start = len - sp.count;   // rows [start, len) are new
   const bool refused = kv_refused(c, b);
-  const int page_i = start / c.page + j;
-  if (sp.count < 1 || (long long)page_i * c.page >= len) return;
+  const long long at = (long long)start / c.page + j;  // (spans that do not fit can give any j)
+  if (sp.count < 1 || j < 0 || at * c.page >= len) return;
   if (refused) {                                       // rows [start, len) are not the new tokens'
     if (threadIdx.x == 0) kv_flag(c, KV_REFUSED);
     return;
@@ -188,6 +188,7 @@ __global__ void __launch_bounds__(RPT == 1 ? 32 : 256, RPT == 1 ? 16 : 2) k_kv8_
     if (threadIdx.x == 0) kv_flag(c, start < 0 || len > max_len ? KV_TOO_LONG : KV_BAD_SPAN);
     return;
   }
+  const int page_i = (int)at;
   const int row0 = page_i * c.page;                    // position of the page's first row
   const int first = max(start - row0, 0), last = min(len - row0, c.page);   // its new rows
 

@@ -406,7 +406,8 @@ int cats_export_list(const void* ws, size_t ws_bytes, int B, int H, int I, int d
  * (never read or written out of range) and recorded in *status, bits that stay until the caller
  * clears them: 1 the pool has no page left, 2 a page id is out of range or a page that is shared
  * would have been written, 4 a sequence is longer than max_pages pages (or has a negative length or
- * position), 8 a parent is out of range, 16 cu does not fit the number of tokens, 32 a wait inside a
+ * position), 8 a parent is out of range, 16 cu does not fit the number of tokens (where it is not
+ * ascending, cats_kv8_attend leaves the whole call out), 32 a wait inside a
  * kernel ran out (see "wait_ms"; the results of that call are not to be used), 64 tokens of a sequence
  * that cats_kv8_grow had not lengthened were left out of a cats_kv8_append.
  * No reference counterpart (the reference leaves the cache to HF's modelling code).
