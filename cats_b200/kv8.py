@@ -124,8 +124,8 @@ class KVCache8:
         return cu.data_ptr()
 
     def _tokens(self, t: torch.Tensor, name: str, cu) -> int:
-        if not isinstance(t, torch.Tensor) or t.device != self.device:
-            raise _bad(f"{name} must be a tensor on {self.device}")
+        if not isinstance(t, torch.Tensor) or t.device != self.device or t.dim() < 1:
+            raise _bad(f"{name} must be a tensor of rows on {self.device}")
         n = t.shape[0]
         if cu is None and n % self.n_seqs:
             raise _bad(f"{name} has {n} rows, not a multiple of the {self.n_seqs} sequences: pass cu")
@@ -177,8 +177,8 @@ class KVCache8:
             q_out = None
         elif q_out is None:
             q_out = torch.empty_strided((n, n_heads, hd), (n_heads * hd, hd, 1), dtype=dt, device=self.device)
-        elif q_out.dtype != dt or q_out.device != self.device or not q_out.is_contiguous() \
-                or q_out.numel() != n * n_heads * hd:
+        elif not isinstance(q_out, torch.Tensor) or q_out.dtype != dt or q_out.device != self.device \
+                or not q_out.is_contiguous() or q_out.numel() != n * n_heads * hd:
             raise _bad("q_out must be contiguous with tokens * n_heads * head_dim elements of qkv's type")
         if n == 0:
             return q_out
@@ -202,7 +202,8 @@ class KVCache8:
         self._layer(layer)
         if out is None:
             out = torch.empty_strided((n, nh, hd), (nh * hd, hd, 1), dtype=dt, device=self.device)
-        elif out.dtype != dt or out.device != self.device or not out.is_contiguous() or out.numel() != n * nh * hd:
+        elif not isinstance(out, torch.Tensor) or out.dtype != dt or out.device != self.device \
+                or not out.is_contiguous() or out.numel() != n * nh * hd:
             raise _bad("out must be contiguous with as many elements as q, of q's type")
         if n == 0:
             return out

@@ -446,8 +446,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, done: Option
         raise RuntimeError(f"cats_b200: scores must hold {n} x {beams} values")
     ended = None
     if done is not None:
-        if done.dtype not in (torch.bool, torch.uint8) or done.device != dev or not done.is_contiguous() \
-                or done.numel() != rows:
+        if not isinstance(done, torch.Tensor) or done.dtype not in (torch.bool, torch.uint8) or done.device != dev \
+                or not done.is_contiguous() or done.numel() != rows:
             raise RuntimeError(f"cats_b200: done must be a contiguous bool/uint8 tensor with {n} x {beams} values")
         if not 0 <= eos < vocab:
             raise RuntimeError("cats_b200: done needs eos, a token of the vocabulary")
