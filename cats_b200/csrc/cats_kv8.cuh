@@ -105,19 +105,7 @@ __host__ __device__ inline int kv_units(int count, int page) {
   return count < 1 ? 0 : (int)(((unsigned)count + page - 2u) / page) + 1;
 }
 
-// eight elements, 16-byte aligned: read once (streaming) or shared by several warps (cached)
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float* f) {
-  if (sizeof(T) == 4) {
-    const uint4 a = ldg_stream(reinterpret_cast<const uint4*>(p));
-    const uint4 b = ldg_stream(reinterpret_cast<const uint4*>(p) + 1);
-    VecT<T>::unpack(a, f);
-    VecT<T>::unpack(b, f + VecT<T>::N % 8);
-  } else {
-    const uint4 a = ldg_stream(reinterpret_cast<const uint4*>(p));
-    VecT<T>::unpack(a, f);
-  }
-}
+// eight elements, 16-byte aligned
 template <typename T>
 __device__ __forceinline__ void load8_cached(const T* p, float* f) {
   const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
