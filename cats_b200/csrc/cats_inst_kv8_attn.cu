@@ -17,8 +17,10 @@ static cudaError_t run_attend(const cats_kv8& c, const KvAttnArgs<T>& A, cudaStr
 }
 
 // Up to 8 rows and up to 16 the tiles of cats_kv8_attn.cuh, bound by the codes' bytes; beyond that the
-// products count.  A CTA takes 128 positions of 32 rows in 1.9 us with those tiles, and of up to 128
-// rows in 3.2 us on tcgen05 (2 x 256 tokens x 4 heads per key head, head_dim 128: 212 and 125 us): 16-bit
+// products count.  (Rows of a key head, on average over all sequences of the cache: idle ones count too, so that a
+// long span among many of them gets small tiles, right but slower.)  A CTA takes 128 positions of 32 rows in 1.9 us
+// with those tiles, and of up to 128 rows in 3.3 us on tcgen05 (2 x 256 tokens x 4 heads per key head: 217 and 128 us
+// at head_dim 128, 162 and 101 us at 64): 16-bit
 // queries with more than 32 rows go there, but for head_dim 32 and 96, which do not fill a 128-byte
 // swizzle row.  fp32 queries are split in two halves, which leaves registers for 16 rows.
 template <typename T, int HD>

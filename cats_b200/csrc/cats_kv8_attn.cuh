@@ -27,8 +27,9 @@
 // joined by the CTA that finishes last (nobody waits).
 //
 // Measured (head_dim 128, 8 key heads): 16 sequences of 32768 positions 171 us, 6.27 TB/s of codes (0.95
-// of a plain copy's rate); 32 sequences of 1000 .. 32000, 603 MB: 108 to 115 us; 8 sequences of 512 ..
-// 1536: 14 us, where the chain launch - lengths - page - codes - join is what takes the time.
+// of a plain copy's rate); 32 sequences of 1000 .. 32000, 603 MB: 110 to 115 us replayed from a graph, 120 to 124 us a
+// call; 8 sequences of 512 .. 1536: 14.3 us, on 80 of 148 SMs (units of 256 positions, of which joining two parts
+// costs as much, leave most segments to one CTA), one sequence of 640 with 32 key heads: 9.8 us on 32 of them.
 #pragma once
 
 #include "cats_kv8.cuh"
@@ -147,7 +148,7 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnTable& tab, int b, int gro
 // join of its warps: a batch of uneven lengths took 130 us with shares of as many units each, since
 // some CTAs had a dozen short segments); a share's border gives way to a segment's border that is
 // next to it while shares are short.  A unit takes 1.3 us, joining parts 2.7 us and a second segment in a CTA
-// 3.7 us (measured, head_dim 128): equal shares, where a CTA mostly has two segments and joins one, win
+// 3.7 us (measured, head_dim 128; the smaller heads go by the same numbers): equal shares, where a CTA mostly has two segments and joins one, win
 // only where dealing out by segments makes the largest share that much larger (measured: 64 segments
 // of 1024 positions 16.7 us in equal shares, 12.1 us by segments).
 struct AttnPlan {

@@ -17,11 +17,15 @@
 // exponents), and so is the way the positions are dealt out to the CTAs.  A NaN among the values must
 // only reach the rows that see its position: it is taken out of the product, and the least such
 // position of every channel is kept for the end.
-// Bound: latency.  A step takes 3.2 us (head_dim 128; 2 x 256 tokens x 4 heads per key head over 2000 ..
-// 6000 positions: 125 us, 260 TFLOP/s): conversions 0.6, asking for the next codes 0.45, exponentials 0.35,
+// A page whose values' exponent lies far below the others' of a step would lose its weights in half precision: the
+// positions of a step go in classes of pages that lie close together, one product for each (nearly always one).
+// Bound: latency.  A step takes 3.3 us (head_dim 128; 2 x 256 tokens x 4 heads per key head over 2000 ..
+// 6000 positions: 128 us, 254 TFLOP/s): conversions 0.6, asking for the next codes 0.45, exponentials 0.35,
 // the exchange of maxima 0.3, S 0.2, writing the weights 0.1 and the rest barriers and round trips, which
 // follow one another in all 16 warps; the MMA pipe is busy 14 % of the time and instructions are issued
-// 40 % of it.  Slower: S issued a step ahead into a second S (135 us), two CTAs an SM with steps of 64
+// 41 % of it.  A tile goes through all positions of its sequence, also those behind its last row (their codes are not
+// loaded): a prompt into an empty cache takes twice the steps that it needs (four of 700 .. 4096 tokens: 1163 us, 169
+// TFLOP/s).  Slower: S issued a step ahead into a second S (135 us), two CTAs an SM with steps of 64
 // positions (137 us: as many instructions a step and thread for half the positions).
 #pragma once
 

@@ -18,11 +18,11 @@ namespace cats {
 // Rounding: products and sums of the rotation are each rounded to fp32 (no contraction), the query
 // once more to its type; keys and values go from fp32 straight to e4m3.  Infinities are stored as
 // NaN (e4m3 has none) and neither sets a scale.
-// Measured: a decode step of eight sequences 2.8 us, all of it the launch and three dependent loads
+// Measured: a decode step of eight sequences 2.9 us, all of it the launch and three dependent loads
 // (length, page, row); four prompts of 700 .. 4096 tokens, 32 + 2 x 32 heads of 128, bf16, 346 MB: 73 us,
 // 4.7 TB/s (the queries alone 28 us, 5 TB/s; keys and values, 256-byte pieces of far rows, 66 us); with one
 // block of rows per CTA and no loads under way it was 130 us.  Two CTAs of 256 threads an SM: with three,
-// 80 registers each, values are spilled (80 us; 8000 fp32 tokens of 32 + 2 x 8 heads: 92 us, 62 with two).
+// 80 registers each, values are spilled (80 us; 8000 fp32 tokens of 32 + 2 x 8 heads: 92 us, 65 with two).
 template <typename T>
 struct KvAppendArgs {
   const T* qkv;
@@ -303,8 +303,9 @@ __global__ void __launch_bounds__(RPT == 1 ? 32 : 256, RPT == 1 ? 16 : 2) k_kv8_
 // ---------------------------------------------------------------------------------------------
 // Free pages are those with refs == 0; the lowest ids are handed out first, in the order of the
 // sequences, so that the result does not depend on the order in which threads run.
-// Measured: 16 beams, five copies of the filled part of a page in 32 layers, 22 MB copied: 12.5 us (three
-// launches 13.1); a compaction that moves 258 MB: 101 us, 5.3 TB/s read and written.
+// Measured: 16 beams, five copies of the filled part of a page in 32 layers, 22 MB copied: 12.9 us; a
+// compaction that moves 258 MB: 102 us, 5.3 TB/s read and written; grow by a token 1.9 us for 8 sequences, 10 us for
+// 1024 over 60000 pages (one CTA goes through the counts twice).
 
 // exclusive block scan over kPlanThreads values; total through *sum
 __device__ __forceinline__ int plan_scan(int v, int* s_warp, int* sum) {

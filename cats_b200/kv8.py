@@ -14,9 +14,14 @@ excepted), so a decode step over the cache can sit in a CUDA graph::
         o = cache.attend(l, q)                      # causal attention over it
     cache.reorder(parents)                          # sequence i continues sequence parents[i]
 
+Lengths, ids and counts are checked on the device, where they live: what does not fit is left out and recorded
+(``check``), and what was cached stays as it was.  A page's scale serves all of its rows and channels of a head, so one
+very large value costs its page's others their codes, but no other page anything.
+
 The calls on one cache have to be ordered, those that only read it too (they share scratch): one
 stream, or events between streams; so do the replays of graphs that hold them.  Its tensors keep their
-addresses; they may be read and filled in place.
+addresses; they may be read and filled in place (after ``reset`` where the cache has been used: it forgets
+which sequences ``grow`` refused).
 """
 from __future__ import annotations
 

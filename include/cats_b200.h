@@ -501,7 +501,8 @@ int cats_kv8_compact(const cats_kv8* cache, int* n_live, void* ws, size_t ws_byt
  * cats_kv8_reorder), out_tokens [n, k] int64, out_done [n, k] (may be NULL) = the beam had ended or
  * the token is eos.  Tokens at -inf come last; a beam whose score or log-sum-exp is not finite (a NaN
  * or +inf among its logits, all of them -inf) has only candidates at -inf.  The log-sum-exp is summed
- * in fp32 over 512 values at a time and in fp64 above that; candidates are compared in fp64.
+ * in fp32 over 512 values at a time and in fp64 above that.  Of a beam its k largest logits are candidates;
+ * they are compared in fp64.
  *   beams <= 32, k <= 32, k <= beams * vocab, vocab <= 2^30, n * beams <= 65535.  ws: cats_beam_select_bytes(...) bytes of scratch.
  */
 size_t cats_beam_select_bytes(int n, int beams, int vocab, int k);
